@@ -278,6 +278,111 @@ int rswa_event_wait(void* ev, void* stream);
 /* milliseconds between two recorded events, after synchronising on `stop`; negative on error */
 float rswa_event_elapsed_ms(void* start, void* stop);
 
+/* ---------------------------------------------------------------------------------------------------------
+ * Decoding: a key/value cache in 8 bits, filled, read, attended to and thinned out.  No counterpart in the
+ * reference, which has whole sequences only (StreamingLLM, whose mask it computes, is a way to decode).
+ *
+ * The cache: k and v [num_blocks, n_kv_heads, block_size, head_dim], one byte per element, and for each block and
+ * head one float scale: value = stored * scale.  kind RSWA_CACHE_INT8: two's complement, -127..127; kind
+ * RSWA_CACHE_E4M3: 4 exponent and 3 mantissa bits (no infinities, up to 448).  rswa_cache_append and
+ * rswa_cache_evict write scales that are powers of two; the others take any positive ones.
+ * block_size: 16, 32, 64 or 128 tokens; head_dim: 64 or 128; every base 16-byte aligned.
+ *
+ * Sequence b's tokens lie, in order, in the blocks named by row b of a block table (int32, device memory; rows
+ * table_stride entries apart, max_blocks of them each); its slot t is token t % block_size of the row's entry
+ * t / block_size.  Entries behind the last one that a length reaches are not looked at.  An entry that is looked
+ * at and is no block of the cache, and a length that is negative or beyond the table, raise the status word: the call
+ * then reads and writes nothing out of bounds, and what it returns for that sequence means nothing.
+ */
+#define RSWA_CACHE_INT8 0
+#define RSWA_CACHE_E4M3 1
+
+typedef struct rswa_cache {
+  void* k;
+  void* v;
+  float* k_scale; /* [num_blocks, n_kv_heads] */
+  float* v_scale;
+  int64_t num_blocks;
+  int32_t n_kv_heads, block_size, head_dim, kind;
+} rswa_cache_t;
+
+typedef struct rswa_block_table {
+  const int32_t* entries; /* [batch, max_blocks] */
+  int64_t stride;
+  int32_t batch, max_blocks;
+} rswa_block_table_t;
+
+/* Quantises new tokens behind the `lens[b]` ones that sequence b has (lens itself is left as it is: the caller
+ * counts).  k and v are 16-bit, [tokens, n_kv_heads, head_dim] packed with cu_seqlens (batch + 1 entries, device
+ * memory), or without it [batch, tokens / batch, n_kv_heads, head_dim].  A block that the call begins gets the least
+ * scale that holds its tokens; one that already holds older tokens keeps its scale if the new ones fit, else the
+ * scale grows and the older tokens are rounded to it.  A block that takes an infinity or a NaN reads as NaN.
+ * The blocks written to must not be shared between sequences. */
+typedef struct rswa_cache_append_params {
+  rswa_cache_t cache;
+  rswa_block_table_t table;
+  const int32_t* lens;
+  int32_t dtype;
+  int32_t reserved;
+  int64_t tokens;            /* new tokens in all */
+  const int32_t* cu_seqlens; /* or NULL */
+  const void* k;
+  int64_t k_stride_b, k_stride_t, k_stride_h; /* in elements; stride_b only without cu_seqlens */
+  const void* v;
+  int64_t v_stride_b, v_stride_t, v_stride_h;
+  int32_t* status;
+} rswa_cache_append_params_t;
+
+int rswa_cache_append(const rswa_cache_append_params_t* p, void* stream);
+
+/* The first min(lens[b], rows) tokens of every sequence in 16 bits: k, v [batch, rows, n_kv_heads, head_dim],
+ * contiguous, zero behind them. */
+typedef struct rswa_cache_read_params {
+  rswa_cache_t cache;
+  rswa_block_table_t table;
+  const int32_t* lens;
+  int32_t dtype;
+  int32_t rows;
+  void* k;
+  void* v;
+  int32_t* status;
+} rswa_cache_read_params_t;
+
+int rswa_cache_read(const rswa_cache_read_params_t* p, void* stream);
+
+/* Attention of the newest q_len tokens of every sequence (query i of sequence b is the token in slot
+ * p = lens[b] - q_len + i, which the cache holds already): it sees slot t iff t <= p and (p - t <= window or
+ * t < n_sink), with window < 0 every t <= p.  q [batch, q_len, Hq, head_dim] 16-bit, strides in elements (head
+ * dimension contiguous, all multiples of 8, 16-byte aligned); out [batch, q_len, Hq, head_dim] contiguous; lse
+ * [batch, Hq, q_len] float (natural log) or NULL.  A query before the sequence's start, or of an empty one, gives a
+ * zero row and lse -inf.
+ * weights (or NULL): float [batch, n_kv_heads, >= max_blocks * block_size], tokens contiguous; every slot seen has
+ * the softmax weights added that it got from the queries and heads of its key/value head.  Needs lse.
+ * `workspace`: rswa_cache_attn_workspace_bytes() of device memory, 256-byte aligned, for the time of the call. */
+typedef struct rswa_cache_attn_params {
+  rswa_cache_t cache;
+  rswa_block_table_t table;
+  const int32_t* lens;
+  int32_t dtype;
+  int32_t q_len, n_q_heads;
+  int32_t window, n_sink;
+  float softmax_scale;
+  const void* q;
+  int64_t q_stride_b, q_stride_t, q_stride_h;
+  void* out;
+  float* lse;
+  float* weights;
+  int64_t w_stride_b, w_stride_h;
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* status;
+} rswa_cache_attn_params_t;
+
+/* Looks at the sizes only (cache, table, q_len, n_q_heads, window, n_sink, whether there are weights); negative: an
+ * error code. */
+int64_t rswa_cache_attn_workspace_bytes(const rswa_cache_attn_params_t* p);
+int rswa_cache_attn(const rswa_cache_attn_params_t* p, void* stream);
+
 /* Kernels of this library launched by the process so far. */
 int64_t rswa_launch_count(void);
 

@@ -18,9 +18,11 @@ CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "ring_swa", "librswa.so")
 NATIVE_OUT = os.path.join(HERE, "ring_swa", "_native.so")
 NATIVE_STAMP = NATIVE_OUT + ".stamp"
-NATIVE_SOURCE = os.path.join(CSRC, "rswa_torch.cpp")
-SOURCES = ["rswa_api.cu", "rswa_fwd.cu", "rswa_bwd.cu", "rswa_dq.cu", "rswa_aux.cu", "rswa_selftest.cu", "rswa_noalloc.cu", "rswa_peer.cu"]
-HEADERS = ["tc05.cuh", "rswa_common.cuh", "rswa_tiles.cuh", os.path.join("..", "..", "include", "rswa.h")]
+NATIVE_SOURCES = [os.path.join(CSRC, s) for s in ("rswa_torch.cpp", "rswa_cache_torch.cpp")]
+NATIVE_HEADERS = [os.path.join(CSRC, "rswa_torch.h"), os.path.join(CSRC, "..", "..", "include", "rswa.h")]
+SOURCES = ["rswa_api.cu", "rswa_fwd.cu", "rswa_bwd.cu", "rswa_dq.cu", "rswa_aux.cu", "rswa_selftest.cu", "rswa_noalloc.cu", "rswa_peer.cu", "rswa_cache.cu",
+           "rswa_cache_attn.cu"]
+HEADERS = ["tc05.cuh", "rswa_common.cuh", "rswa_tiles.cuh", "rswa_cache.cuh", os.path.join("..", "..", "include", "rswa.h")]
 
 
 def _nvcc() -> str:
@@ -54,7 +56,7 @@ def native_is_stale() -> bool:
     with open(NATIVE_STAMP) as f:
         if f.read() != _native_abi():
             return True
-    deps = [NATIVE_SOURCE, os.path.join(CSRC, "..", "..", "include", "rswa.h"), os.path.abspath(__file__)]
+    deps = NATIVE_SOURCES + NATIVE_HEADERS + [os.path.abspath(__file__)]
     return os.path.getmtime(NATIVE_OUT) <= max(os.path.getmtime(d) for d in deps)
 
 
@@ -65,7 +67,7 @@ def build_native(force: bool = False) -> str:
     import torch
     root = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
-    cmd = ["g++", "-std=c++17", "-O2", "-shared", "-fPIC", "-fvisibility=hidden", "-o", NATIVE_OUT, NATIVE_SOURCE,
+    cmd = ["g++", "-std=c++17", "-O2", "-shared", "-fPIC", "-fvisibility=hidden", "-o", NATIVE_OUT, *NATIVE_SOURCES,
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-I", os.path.join(root, "include"), "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"),
            "-I", sysconfig.get_paths()["include"], "-I", os.path.join(cuda, "include"),
@@ -84,7 +86,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         build_native()
         return OUT
     cmd = [
-        _nvcc(), "-std=c++17", "-O3", "-lineinfo",
+        _nvcc(), "-std=c++17", "-O3", "-lineinfo", "--threads", "0",
         "-gencode", "arch=compute_100a,code=sm_100a",
         "-shared", "-Xcompiler", "-fPIC",
         "-o", OUT,

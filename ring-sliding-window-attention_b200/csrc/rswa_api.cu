@@ -145,6 +145,61 @@ int make_tile_map(CUtensorMap* map, const void* base, int dtype, int batch, int 
   return RSWA_OK;
 }
 
+// 2-D map over rows of `row_bytes` (64 or 128) bytes, boxes of box_rows rows, swizzled over the row's length; cached like
+// the maps above (a decoding step presents the same cache layer by layer).
+namespace {
+struct RowsKey {
+  const void* base;
+  long long rows;
+  int row_bytes, box_rows;
+  bool operator==(const RowsKey& o) const { return base == o.base && rows == o.rows && row_bytes == o.row_bytes && box_rows == o.box_rows; }
+};
+constexpr int kRowsCacheSize = 256;  // (K and V of 128 layers)
+struct RowsCache {
+  RowsKey key[kRowsCacheSize];
+  CUtensorMap map[kRowsCacheSize];
+  int used = 0, next = 0, last = 0;
+};
+thread_local RowsCache t_rows_cache;
+}  // namespace
+
+int make_rows_map(CUtensorMap* map, const void* base, long long rows, int row_bytes, int box_rows) {
+  EncodeTiledFn enc = get_encode();
+  if (!enc) return RSWA_E_CUDA;
+  static thread_local bool t_context_bound = false;  // (see make_tile_map)
+  if (!t_context_bound) {
+    cudaFree(nullptr);
+    t_context_bound = true;
+  }
+  const RowsKey key{base, rows, row_bytes, box_rows};
+  RowsCache& cache = t_rows_cache;
+  // (from the entry behind the last hit on: layers come in order)
+  for (int i = 0; i < cache.used; ++i) {
+    const int at = (cache.last + 1 + i) % cache.used;
+    if (cache.key[at] == key) {
+      *map = cache.map[at];
+      cache.last = at;
+      return RSWA_OK;
+    }
+  }
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(row_bytes), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_bytes)};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(row_bytes), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed with code %d (%lld rows of %d bytes)", static_cast<int>(r), rows, row_bytes);
+    return RSWA_E_CUDA;
+  }
+  const int slot = cache.used < kRowsCacheSize ? cache.used++ : (cache.next++ % kRowsCacheSize);
+  cache.key[slot] = key;
+  cache.map[slot] = *map;
+  cache.last = slot;
+  return RSWA_OK;
+}
+
 int check_geom(const rswa_geom_t& g, bool need_grads, int head_dim) {
   if (g.dtype != RSWA_DTYPE_BF16 && g.dtype != RSWA_DTYPE_FP16) {
     set_error("dtype must be bf16 (0) or fp16 (1), got %d", g.dtype);

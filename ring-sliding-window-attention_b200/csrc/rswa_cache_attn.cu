@@ -1,0 +1,853 @@
+// Attention of the newest token(s) of every sequence over its cached tokens (see rswa_cache_attn in rswa.h).
+//
+//   out = sum_t p_t v_t,  p_t = exp(scale * q.k_t - lse)  over the visible slots t
+//
+// in one pass over K and V: running maximum and sum per row, K and V brought in by TMA and never in any form but the
+// stored bytes until they are operands.  What has to be moved is 2 * head_dim bytes per visible token and key/value
+// head, 1/64 of what a 16-bit, ungrouped cache of 32 heads on 8 would need; the products are 4 * head_dim FLOPs per
+// query head on them, at 8 query heads 32 per byte: HBM-bound by a factor of 8 on the tensor cores, but not on the FMA pipe.
+//
+// Products: mma.m16n8k16 with the KEYS (the V columns) as the 16 rows and the query rows as the 8 columns, so that a
+// group of up to 8 rows wastes nothing on the operand that costs: the one converted from bytes.  (tcgen05 wants 128
+// rows of A, both operands in the same 8-bit or 16-bit type in shared memory: the bytes would have to be converted and
+// written back there, or the queries and weights rounded to 8 bits.)  A word of four stored bytes becomes two operand
+// registers in place: bytes 0, 2 and bytes 1, 3.  For K the order of the head dimension inside a product is free (the
+// queries are laid out the same way); for V the two registers are two columns of the head, whose weights are the same.
+//   S^T[token][row] = K q^T        ldmatrix: lane (g, c) of a quad layout holds d = 16 s + 4c .. 4c + 3 of token g
+//   O^T[d][row]    += V^T P^T      ldmatrix.trans: lane holds d = 16 m + 2g, 2g + 1 of tokens 2c, 2c + 1
+// P^T comes out of S^T's accumulators by two 8x8 transposes (movmatrix) per 16 tokens.
+//
+// Queries and weights are fp16 operands: a bf16 query is scaled by a power of two to the top of the fp16 range (exact
+// but for elements 2^-30 smaller than the row's largest), the weights are at most 2^14 with 11 bits each.  The scale of
+// a V block goes into its tokens' exponents (s + log2 of the scale), so that the running reference covers both;
+// the sum of the weights takes it back out.  Scores, sums and the output are 32-bit.
+//
+// Work: the 32-token tiles of all (sequence, key/value head, 8 or 16 query rows) in one order, cut evenly over the CTAs
+// (one per SM) whatever the lengths; the 8 warps of a CTA take its tiles in turn, each with a ring of tiles of its own
+// in flight that runs on over sequence boundaries, and add up at the end of each piece.  A piece that is not a whole
+// (sequence, head) goes to the workspace and a second kernel joins the pieces in order: results do not depend on timing.
+#include <atomic>
+
+#include "rswa_cache.cuh"
+
+namespace rswa {
+
+int make_rows_map(CUtensorMap* map, const void* base, long long rows, int row_bytes, int box_rows);
+int check_table(const rswa_block_table_t& t, const int32_t* lens, const int32_t* status, int block_size, const char* what);
+
+using namespace tc05;
+
+namespace {
+
+constexpr int kTok = 32;     // tokens of a tile
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kMinShare = 8; // tiles of a CTA at least: one per warp
+constexpr float kRoom = 14.f;  // a weight may grow to 2^14 before the reference is raised (fp16 ends at 2^16)
+constexpr float kLow = 4.f;    // and is raised to the maximum minus 4, so that not every new maximum raises it
+
+struct AttnKernelParams {
+  CUtensorMap map[2];
+  CacheView c;
+  const int* table;
+  long long table_stride;
+  int batch, max_blocks;
+  const int* lens;
+  const uint16_t* q;
+  long long q_sb, q_st, q_sh;
+  int q_len, hq, group, rows, row_tiles;  // rows = q_len * group, in tiles of 8 * kNT
+  int window, n_sink;                     // window < 0: all
+  float scale_log2;
+  int bf16;
+  uint16_t* out;
+  float* lse;        // or null
+  float* part_o;     // [CTAs][2][8 * kNT][head_dim]
+  float* part_ml;    // [CTAs][2][8 * kNT][2]
+  float* scores;     // [tiles][kTok][8 * kNT], or null: what the weights need
+  float* weights;
+  long long w_sb, w_sh;
+  int ctas;
+  int* status;
+  int* mirror;
+};
+
+// The tiles of one sequence: the ones its sink tokens lie in, then the ones from its oldest visible token on.
+struct SeqTiles {
+  int len, n_sink_tiles, first, n;
+};
+__device__ __forceinline__ SeqTiles seq_tiles(const AttnKernelParams& p, int b) {
+  SeqTiles s;
+  int len = p.lens[b];
+  const int cap = p.max_blocks * p.c.bs;
+  if (len < 0 || len > cap) {
+    raise_status(p.status, p.mirror, kErrSeqLen);
+    len = 0;
+  }
+  const int oldest = p.window < 0 ? 0 : max(0, max(0, len - p.q_len) - p.window);
+  s.len = len;
+  s.first = oldest / kTok;
+  s.n_sink_tiles = min((min(p.n_sink, len) + kTok - 1) / kTok, s.first);
+  s.n = s.n_sink_tiles + (len + kTok - 1) / kTok - s.first;
+  return s;
+}
+__device__ __forceinline__ int tile_slot(const SeqTiles& s, int i) { return (i < s.n_sink_tiles ? i : s.first + i - s.n_sink_tiles) * kTok; }
+
+// Where the work of a CTA begins and ends: equal shares of all tiles, none of fewer than kMinShare.
+__device__ __forceinline__ long long n_shares(long long total, int ctas) { return min(static_cast<long long>(ctas), max(1LL, total / kMinShare)); }
+__device__ __forceinline__ long long share_begin(long long total, long long shares, long long c) { return total * c / shares; }
+__device__ __forceinline__ long long share_of(long long total, long long shares, long long tile) { return ((tile + 1) * shares - 1) / total; }
+
+// Prefix sums of the sequences' tiles (per key/value head and row tile): thread i of kThreads holds `per` sequences.
+// s_prefix[i]: tiles in front of thread i's sequences; s_prefix[kThreads]: all.
+__device__ __forceinline__ void tile_prefix(const AttnKernelParams& p, long long* s_prefix, long long* s_warp) {
+  const int per = (p.batch + kThreads - 1) / kThreads;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long mine = 0;
+  for (int i = 0; i < per; ++i) {
+    const int b = threadIdx.x * per + i;
+    if (b < p.batch) mine += seq_tiles(p, b).n;
+  }
+  long long sum = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const long long o = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) sum += o;
+  }
+  if (lane == 31) s_warp[warp] = sum;
+  __syncthreads();
+  long long before = 0;
+  for (int w = 0; w < warp; ++w) before += s_warp[w];
+  s_prefix[threadIdx.x] = before + sum - mine;
+  if (threadIdx.x == kThreads - 1) s_prefix[kThreads] = before + sum;
+  __syncthreads();
+}
+
+// A place in the order of all tiles: sequence, then head, then row tile, then tile.
+struct Cursor {
+  int b, item, i;       // item = head * row_tiles + row tile
+  SeqTiles s;
+  long long at;         // index among all tiles
+  // moves forward by n tiles; false: behind the last
+  __device__ __forceinline__ void skip(const AttnKernelParams& p, long long n, long long end) {
+    at += n;
+    if (at >= end) return;
+    long long k = i + n;
+    const int items = p.c.hkv * p.row_tiles;
+    while (k >= s.n) {
+      k -= s.n;
+      if (++item == items) {
+        item = 0;
+        do s = seq_tiles(p, ++b); while (s.n == 0);
+      }
+    }
+    i = static_cast<int>(k);
+  }
+};
+__device__ __forceinline__ Cursor cursor_at(const AttnKernelParams& p, const long long* s_prefix, long long tile) {
+  const long long items = static_cast<long long>(p.c.hkv) * p.row_tiles;
+  const int per = (p.batch + kThreads - 1) / kThreads;
+  int lo = 0, hi = kThreads - 1;  // the last thread whose prefix is not behind the tile
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (s_prefix[mid] * items <= tile) lo = mid; else hi = mid - 1;
+  }
+  // (threads of no tiles share a prefix: the last of them holds the tile, or has no sequences and the walk starts
+  // at a sequence of its own)
+  Cursor c;
+  c.at = tile;
+  c.b = lo * per;
+  long long rest = tile - s_prefix[lo] * items;
+  c.s = seq_tiles(p, c.b);
+  while (rest >= c.s.n * items) {
+    rest -= c.s.n * items;
+    c.s = seq_tiles(p, ++c.b);
+  }
+  c.item = static_cast<int>(rest / c.s.n);
+  c.i = static_cast<int>(rest % c.s.n);
+  return c;
+}
+
+template <int kD>
+struct Ring {
+  static constexpr int kTileBytes = kTok * kD;      // of K, and of V
+  static constexpr int kStageBytes = 2 * kTileBytes;
+};
+
+template <int kNT, int kStages>
+struct Ctl {
+  uint64_t full[kWarps][kStages];
+  float scale[kWarps][kStages][4];  // K and V scale of the tile's first 16 tokens, and of its last 16
+  float ml[kWarps][8 * kNT][2];     // reference and sum of every warp's piece
+  int err;
+};
+
+// [rings][sums of the warps' pieces; at first the sequences' prefix sums][control]
+template <int kD, int kNT>
+struct Layout {
+  static constexpr int kStages = kD == 128 ? 3 : 6;
+  static constexpr int kRings = kWarps * kStages * Ring<kD>::kStageBytes;
+  static constexpr int kMerge = kWarps * 8 * kD * 4;
+  static constexpr int kBytes = kRings + kMerge + static_cast<int>(sizeof(Ctl<kNT, kStages>));
+  static_assert(kBytes <= 232448, "shared memory budget");
+};
+
+__device__ __forceinline__ void tma_load_rows(void* dst, const CUtensorMap* m, uint64_t* bar, int row) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(0), "r"(row)
+      : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 16-byte piece `chunk` of row `row` of a tile, as TMA's swizzle left it
+template <int kD>
+__device__ __forceinline__ uint32_t piece(uint32_t base, int row, int chunk) {
+  return base + row * kD + ((kD == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4);
+}
+
+// kNT: query rows in columns of 8.
+template <int kD, int kNT, bool kInt8>
+__global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_constant__ AttnKernelParams p) {
+  using L = Layout<kD, kNT>;
+  using R = Ring<kD>;
+  constexpr int kS = L::kStages, kKS = kD / 16;
+  constexpr int kRows = 8 * kNT;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  auto& ctl = *reinterpret_cast<Ctl<kNT, kS>*>(smem + L::kRings + L::kMerge);
+  float* const merge = reinterpret_cast<float*>(smem + L::kRings);
+  long long* const s_prefix = reinterpret_cast<long long*>(merge);
+  static_assert(L::kMerge >= (kThreads + 1 + kWarps) * 8, "the prefix sums lie where the pieces' sums come later");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  uint64_t* const full = ctl.full[warp];
+  uint8_t* const ring = smem + warp * kS * R::kStageBytes;
+
+  if (threadIdx.x == 0) ctl.err = 0;
+  if (lane == 0)
+    for (int i = 0; i < kS; ++i) mbar_init(full + i, 1 + 4);  // lane 0's announcement of the bytes, four lanes' scales
+  mbar_fence_init();
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&p.map[0]);
+    prefetch_tmap(&p.map[1]);
+  }
+  griddep_wait();
+  tile_prefix(p, s_prefix, s_prefix + kThreads + 1);
+  const long long total = s_prefix[kThreads] * p.c.hkv * p.row_tiles;
+  const long long shares = n_shares(total, p.ctas);
+  if (blockIdx.x >= shares || total == 0) return;
+  const long long begin = share_begin(total, shares, blockIdx.x), end = share_begin(total, shares, blockIdx.x + 1);
+
+  // The loads of this warp's tiles run kS ahead of the arithmetic.
+  const int bs = p.c.bs, box = min(bs, kTok);
+  Cursor lc = cursor_at(p, s_prefix, begin);
+  Cursor cc = lc;  // the arithmetic's: first tile of the current piece
+  __syncthreads();  // (the prefix sums make room)
+  lc.skip(p, warp, end);
+  uint32_t pending = 0;  // stages with a load that has not been waited for
+  auto issue = [&](int st) {
+    if (lc.at >= end) return;
+    const int slot = tile_slot(lc.s, lc.i), h = lc.item / p.row_tiles;
+    // (a tile is part of one block, or two blocks of 16; the second may lie behind the sequence's end: not looked at)
+    int pg[2];
+    const int j = slot / bs;
+    pg[0] = table_entry(p.table, p.table_stride, lc.b, j, p.c.num_blocks, p.status, p.mirror);
+    pg[1] = pg[0];
+    if (bs < kTok) pg[1] = slot + bs < lc.s.len ? table_entry(p.table, p.table_stride, lc.b, j + 1, p.c.num_blocks, p.status, p.mirror) : pg[0];
+    // (reported; any block will do then)
+    pg[0] = max(pg[0], 0);
+    pg[1] = max(pg[1], 0);
+    pending |= 1u << st;
+    uint8_t* const dst = ring + st * R::kStageBytes;
+    if (lane == 0) {
+      mbar_expect_tx(full + st, R::kStageBytes);
+      const int off = slot % bs;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv)
+        for (int half = 0; half < kTok / box; ++half)
+          tma_load_rows(dst + kv * R::kTileBytes + half * box * kD, &p.map[kv], full + st, (pg[half] * p.c.hkv + h) * bs + off);
+    }
+    if (lane < 4) {
+      const float* src = p.c.scale[lane & 1] + static_cast<long long>(pg[lane >> 1]) * p.c.hkv + h;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&ctl.scale[warp][st][lane])), "l"(src) : "memory");
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(full + st)) : "memory");
+    }
+    lc.skip(p, kWarps, end);
+  };
+#pragma unroll
+  for (int st = 0; st < kS; ++st) issue(st);
+
+  uint32_t phases = 0;
+  int st = 0;
+  bool dead = false;
+  while (cc.at < end) {
+    const long long piece_end = min(end, cc.at + cc.s.n - cc.i);
+    const int h = cc.item / p.row_tiles, row0 = (cc.item - h * p.row_tiles) * kRows;
+    // the queries of this piece as operands: row g of each column block, d = 16 s + 4c .. 4c + 3
+    uint32_t qf[kNT][kKS][2];
+    float rs[kNT][2];  // factor of the scores of rows 2c, 2c + 1, log2(e) in it
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+      const int row = row0 + nt * 8 + g;
+      float factor = 0.f;
+      if (row < p.rows) {
+        const int i = row / p.group, hd = h * p.group + row - i * p.group;
+        const uint16_t* src = p.q + cc.b * p.q_sb + i * p.q_st + hd * p.q_sh + c * 4;
+#pragma unroll
+        for (int s = 0; s < kKS; ++s) {
+          const uint2 x = *reinterpret_cast<const uint2*>(src + s * 16);
+          qf[nt][s][0] = __byte_perm(x.x, x.y, 0x5410);  // elements 0, 2
+          qf[nt][s][1] = __byte_perm(x.x, x.y, 0x7632);  // elements 1, 3
+        }
+        factor = 1.f;
+      } else {
+#pragma unroll
+        for (int s = 0; s < kKS; ++s) qf[nt][s][0] = qf[nt][s][1] = 0;
+      }
+      if (p.bf16) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int s = 0; s < kKS; ++s) most = __vmaxu2(most, __vmaxu2(qf[nt][s][0] & 0x7fff7fffu, qf[nt][s][1] & 0x7fff7fffu));
+        most = max(most & 0xffffu, most >> 16);
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        // largest element to [2^14, 2^15); exponents below 2^-100 are taken for it.  Not finite: the whole row NaN
+        const int e = max(static_cast<int>(most >> 7), 27);
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 + 127 - e) << 23);
+        const float mul = most >= 0x7f80u ? __uint_as_float(0x7fffffffu) : up;
+#pragma unroll
+        for (int s = 0; s < kKS; ++s)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t w = qf[nt][s][k];
+            qf[nt][s][k] = pack2<false>(__uint_as_float(w << 16) * mul, __uint_as_float(w & 0xffff0000u) * mul);
+          }
+        factor *= __uint_as_float(static_cast<uint32_t>(e - 14) << 23);
+      }
+      factor *= p.scale_log2 * kHalfFactor<kInt8>;
+      rs[nt][0] = __shfl_sync(0xffffffffu, factor, c * 8);
+      rs[nt][1] = __shfl_sync(0xffffffffu, factor, c * 8 + 4);
+    }
+    // what the rows of this lane's accumulators (2c, 2c + 1 of each column block) see: slots up to last, from first on
+    int last[kNT][2], first[kNT][2];
+    int last_min = 0x7fffffff, first_max = 0;
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int row = row0 + nt * 8 + 2 * c + k;
+        const int pos = cc.s.len - p.q_len + min(row, p.rows - 1) / p.group;  // (rows behind the last one are not stored)
+        last[nt][k] = pos;
+        first[nt][k] = p.window < 0 ? 0 : max(0, pos - p.window);
+        last_min = min(last_min, pos);
+        first_max = max(first_max, first[nt][k]);
+      }
+    last_min = __reduce_min_sync(0xffffffffu, last_min);
+    first_max = __reduce_max_sync(0xffffffffu, first_max);
+
+    float o[kNT][kKS][4], m[kNT][2], l[kNT][2];
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+#pragma unroll
+      for (int s = 0; s < kKS; ++s) o[nt][s][0] = o[nt][s][1] = o[nt][s][2] = o[nt][s][3] = 0.f;
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
+    // this warp's tiles of the piece: those whose index from `begin` is `warp` modulo kWarps
+    const int lag = static_cast<int>((cc.at - begin) % kWarps);
+    for (long long at = cc.at + (warp + kWarps - lag) % kWarps; at < piece_end; at += kWarps) {
+      if (!dead) dead = !mbar_wait_w(full + st, (phases >> st) & 1, &ctl.err, kErrWaitProducer);
+      if (!dead) {
+        phases ^= 1u << st;
+        pending &= ~(1u << st);
+      }
+      const int slot = tile_slot(cc.s, cc.i + static_cast<int>(at - cc.at));
+      const uint32_t k_base = smem_u32(ring + st * R::kStageBytes), v_base = k_base + R::kTileBytes;
+      float sk[2], lv[2], iv[2];  // of each 16 tokens: K's scale, log2 of V's and 1 / V's
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        // (tokens that no row sees, whose block may not even have a scale, take 1)
+        const int a = slot + 16 * t;
+        const bool some = a < cc.s.len;
+        sk[t] = some ? ctl.scale[warp][st][2 * t] : 1.f;
+        const float sv = some ? ctl.scale[warp][st][2 * t + 1] : 1.f;
+        lv[t] = __log2f(sv);
+        iv[t] = 1.f / sv;
+      }
+      // ---- scores
+      float acc[2][kNT][4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) acc[t][nt][0] = acc[t][nt][1] = acc[t][nt][2] = acc[t][nt][3] = 0.f;
+#pragma unroll
+      for (int s = 0; s < kKS; ++s) {
+        uint32_t w[4], lo[4], hi[4];
+        ldsm4(w, piece<kD>(k_base, lane, s));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) to_half2<kInt8>(w[k], lo[k], hi[k]);
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) {
+          mma16816(acc[0][nt], lo[0], lo[1], hi[0], hi[1], qf[nt][s][0], qf[nt][s][1]);
+          mma16816(acc[1][nt], lo[2], lo[3], hi[2], hi[3], qf[nt][s][0], qf[nt][s][1]);
+        }
+      }
+      // ---- to base 2, hidden ones to -inf
+      const bool plain = slot + kTok - 1 <= last_min && (slot >= first_max || slot + kTok <= p.n_sink);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[t][nt][k] *= rs[nt][k & 1] * sk[t];
+      if (!plain) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int tok = slot + 16 * t + g + 8 * (k >> 1);
+              if (!(tok <= last[nt][k & 1] && (tok >= first[nt][k & 1] || tok < p.n_sink))) acc[t][nt][k] = -INFINITY;
+            }
+      }
+      if (p.scores != nullptr) {
+        float* const to = p.scores + at * (kTok * kRows);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt) {
+            *reinterpret_cast<float2*>(to + (16 * t + g) * kRows + nt * 8 + 2 * c) = make_float2(acc[t][nt][0], acc[t][nt][1]);
+            *reinterpret_cast<float2*>(to + (16 * t + g + 8) * kRows + nt * 8 + 2 * c) = make_float2(acc[t][nt][2], acc[t][nt][3]);
+          }
+      }
+      // ---- running reference
+      float top[kNT][2];
+      bool raise = false;
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = k; e < 4; e += 2)  // (a hidden token stays hidden whatever its block's scale is)
+              acc[t][nt][e] = !plain && acc[t][nt][e] == -INFINITY ? -INFINITY : acc[t][nt][e] + lv[t];
+          top[nt][k] = fmaxf(fmaxf(acc[0][nt][k], acc[0][nt][k + 2]), fmaxf(acc[1][nt][k], acc[1][nt][k + 2]));
+          raise = raise || top[nt][k] > m[nt][k] + kRoom;
+        }
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float x = top[nt][k];
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            const float old = m[nt][k];
+            const float next = x - kLow > old ? x - kLow : old;
+            const float f = next > old ? ex2f(old - next) : 1.f;
+            m[nt][k] = next;
+            l[nt][k] *= f;
+#pragma unroll
+            for (int s = 0; s < kKS; ++s) o[nt][s][k] *= f, o[nt][s][k + 2] *= f;
+          }
+      }
+      // ---- weights, as the right operand of V^T P^T
+      uint32_t pf[2][kNT][2];
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
+        const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const float a = ex2f(acc[t][nt][0] - m0), b = ex2f(acc[t][nt][1] - m1);
+          const float d = ex2f(acc[t][nt][2] - m0), e = ex2f(acc[t][nt][3] - m1);
+          l[nt][0] += a + d == 0.f ? 0.f : (a + d) * iv[t];
+          l[nt][1] += b + e == 0.f ? 0.f : (b + e) * iv[t];
+          pf[t][nt][0] = transpose8(pack2<false>(a, b));
+          pf[t][nt][1] = transpose8(pack2<false>(d, e));
+        }
+      }
+      // ---- output
+#pragma unroll
+      for (int s = 0; s < kKS; ++s) {
+        uint32_t w[4], lo[4], hi[4];
+        ldsm4_t(w, piece<kD>(v_base, lane, s));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) to_half2<kInt8>(w[k], lo[k], hi[k]);
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) {
+          mma16816(o[nt][s], lo[0], hi[0], lo[1], hi[1], pf[0][nt][0], pf[0][nt][1]);
+          mma16816(o[nt][s], lo[2], hi[2], lo[3], hi[3], pf[1][nt][0], pf[1][nt][1]);
+        }
+      }
+      __syncwarp();  // every lane has read the stage
+      if (!dead) issue(st);
+      st = st + 1 == kS ? 0 : st + 1;
+    }
+
+    // ---- the warps' sums of this piece
+    const bool from_start = cc.i == 0, to_end = piece_end - cc.at == cc.s.n - cc.i;
+    const bool whole = from_start && to_end;
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float x = l[nt][k];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        if (g == 0) {
+          ctl.ml[warp][nt * 8 + 2 * c + k][0] = m[nt][k];
+          ctl.ml[warp][nt * 8 + 2 * c + k][1] = x;
+        }
+      }
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+      // (float d of row r lies at d ^ 8 * (r / 2): no bank twice in a half-warp's stores)
+      float* const mine = merge + warp * 8 * kD;
+#pragma unroll
+      for (int s = 0; s < kKS; ++s) {
+        *reinterpret_cast<float2*>(mine + (2 * c) * kD + ((s * 16 + 2 * g) ^ (8 * c))) = make_float2(o[nt][s][0], o[nt][s][2]);
+        *reinterpret_cast<float2*>(mine + (2 * c + 1) * kD + ((s * 16 + 2 * g) ^ (8 * c))) = make_float2(o[nt][s][1], o[nt][s][3]);
+      }
+      __syncthreads();
+      const int r = threadIdx.x / (kD / 4), d4 = threadIdx.x % (kD / 4);
+      if (r < 8) {
+        const int row = row0 + nt * 8 + r;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ctl.ml[w][nt * 8 + r][0]);
+        float sum = 0.f;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float lw = ctl.ml[w][nt * 8 + r][1];
+          if (lw == 0.f) continue;  // (no visible token)
+          const float f = ex2f(ctl.ml[w][nt * 8 + r][0] - top);
+          const float4 y = *reinterpret_cast<const float4*>(merge + (w * 8 + r) * kD + ((d4 * 4) ^ (r / 2 * 8)));
+          sum += lw * f;
+          x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
+        }
+        if (row < p.rows) {
+          if (whole) {
+            const int i = row / p.group, hd = h * p.group + row - i * p.group;
+            const float inv = sum == 0.f ? 0.f : kHalfFactor<kInt8> / sum;
+            uint16_t* const to = p.out + ((static_cast<long long>(cc.b) * p.q_len + i) * p.hq + hd) * kD + d4 * 4;
+            *reinterpret_cast<uint2*>(to) = p.bf16 ? make_uint2(pack2<true>(x.x * inv, x.y * inv), pack2<true>(x.z * inv, x.w * inv))
+                                                   : make_uint2(pack2<false>(x.x * inv, x.y * inv), pack2<false>(x.z * inv, x.w * inv));
+            if (p.lse != nullptr && d4 == 0)
+              p.lse[(static_cast<long long>(cc.b) * p.hq + hd) * p.q_len + i] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.6931471805599453f;
+          } else {
+            const long long to = (static_cast<long long>(blockIdx.x) * 2 + (from_start ? 1 : 0)) * kRows + nt * 8 + r;
+            *reinterpret_cast<float4*>(p.part_o + to * kD + d4 * 4) = x;
+            if (d4 == 0) *reinterpret_cast<float2*>(p.part_ml + to * 2) = make_float2(top, sum);
+          }
+        }
+      }
+      __syncthreads();
+    }
+    cc.skip(p, piece_end - cc.at, end);
+  }
+  if (dead) {
+    // the copies still on their way must not outlive the CTA's shared memory; each wait is limited
+    int own_err = 0;
+    for (int i = 0; i < kS; ++i)
+      if (pending >> i & 1) mbar_wait(full + i, (phases >> i) & 1, &own_err, kErrWaitProducer);
+    if (lane == 0) raise_status(p.status, p.mirror, kErrWaitProducer);
+  }
+}
+
+// Joins the pieces of every (sequence, head, row tile) that more than one CTA worked on, in the CTAs' order, and writes
+// the rows of sequences that have nothing to attend to.  One CTA per (sequence, head, row tile).
+template <int kD, int kNT, bool kInt8>
+__global__ void __launch_bounds__(kThreads) cache_join_kernel(const __grid_constant__ AttnKernelParams p) {
+  constexpr int kRows = 8 * kNT;
+  __shared__ long long s_prefix[kThreads + 1], s_warp[kWarps];
+  griddep_wait();
+  const int items = p.c.hkv * p.row_tiles;
+  const int b = blockIdx.x / items, item = blockIdx.x - b * items;
+  const int h = item / p.row_tiles, row0 = (item - h * p.row_tiles) * kRows;
+  const SeqTiles s = seq_tiles(p, b);
+  long long lo = 0, hi = 0;
+  long long total = 1, shares = 1;
+  if (s.n > 0) {
+    tile_prefix(p, s_prefix, s_warp);
+    total = s_prefix[kThreads] * items;
+    shares = n_shares(total, p.ctas);
+    const int per = (p.batch + kThreads - 1) / kThreads;
+    long long first = s_prefix[b / per];
+    for (int k = b / per * per; k < b; ++k) first += seq_tiles(p, k).n;
+    first = first * items + static_cast<long long>(item) * s.n;
+    lo = share_of(total, shares, first);
+    hi = share_of(total, shares, first + s.n - 1);
+    if (lo == hi) return;  // written already
+    // (the first piece is its CTA's last one, from the item's start on; the others are their CTAs' first ones)
+  }
+  for (int r = threadIdx.x / (kD / 4); r < kRows; r += kThreads / (kD / 4)) {
+    const int row = row0 + r, d4 = threadIdx.x % (kD / 4);
+    if (row >= p.rows) break;
+    float top = -INFINITY, sum = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (s.n > 0) {
+      for (long long c = lo; c <= hi; ++c) top = fmaxf(top, p.part_ml[((c * 2 + (c == lo ? 1 : 0)) * kRows + r) * 2]);
+#pragma unroll 4
+      for (long long c = lo; c <= hi; ++c) {
+        const long long at = (c * 2 + (c == lo ? 1 : 0)) * kRows + r;
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+        const float4 y = *reinterpret_cast<const float4*>(p.part_o + at * kD + d4 * 4);
+        if (ml.y == 0.f) continue;
+        const float f = ex2f(ml.x - top);
+        sum += ml.y * f;
+        x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
+      }
+    }
+    const int i = row / p.group, hd = h * p.group + row - i * p.group;
+    const float inv = sum == 0.f ? 0.f : kHalfFactor<kInt8> / sum;
+    uint16_t* const to = p.out + ((static_cast<long long>(b) * p.q_len + i) * p.hq + hd) * kD + d4 * 4;
+    *reinterpret_cast<uint2*>(to) = p.bf16 ? make_uint2(pack2<true>(x.x * inv, x.y * inv), pack2<true>(x.z * inv, x.w * inv))
+                                           : make_uint2(pack2<false>(x.x * inv, x.y * inv), pack2<false>(x.z * inv, x.w * inv));
+    if (p.lse != nullptr && d4 == 0)
+      p.lse[(static_cast<long long>(b) * p.hq + hd) * p.q_len + i] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.6931471805599453f;
+  }
+}
+
+// Adds every visible slot's softmax weights up, from the scores that the first kernel kept and the final log-sum-exp.
+// One CTA per (sequence, head) and kWeightTiles tiles.
+constexpr int kWeightTiles = 64;
+template <int kNT>
+__global__ void __launch_bounds__(kThreads) cache_weights_kernel(const __grid_constant__ AttnKernelParams p, int chunks) {
+  constexpr int kRows = 8 * kNT;
+  __shared__ long long s_prefix[kThreads + 1], s_warp[kWarps];
+  extern __shared__ float s_lse[];  // [row_tiles * kRows], base 2; +inf for rows that see nothing and rows behind the last
+  griddep_wait();
+  const int bh = blockIdx.x / chunks, b = bh / p.c.hkv, h = bh - b * p.c.hkv;
+  const SeqTiles s = seq_tiles(p, b);
+  const int t0 = (blockIdx.x - bh * chunks) * kWeightTiles;
+  if (t0 >= s.n) return;
+  for (int r = threadIdx.x; r < p.row_tiles * kRows; r += kThreads) {
+    float x = INFINITY;
+    if (r < p.rows) {
+      const int i = r / p.group;
+      x = p.lse[(static_cast<long long>(b) * p.hq + h * p.group + r - i * p.group) * p.q_len + i] * 1.4426950408889634f;
+      if (x == -INFINITY) x = INFINITY;
+    }
+    s_lse[r] = x;
+  }
+  tile_prefix(p, s_prefix, s_warp);
+  const int items = p.c.hkv * p.row_tiles, per = (p.batch + kThreads - 1) / kThreads;
+  long long first = s_prefix[b / per];
+  for (int k = b / per * per; k < b; ++k) first += seq_tiles(p, k).n;
+  first = first * items + static_cast<long long>(h) * p.row_tiles * s.n;
+  const int t1 = min(t0 + kWeightTiles, s.n);
+  for (int k = t0 * kTok + threadIdx.x; k < t1 * kTok; k += kThreads) {
+    const int tile = k / kTok, tok = tile_slot(s, tile) + k % kTok;
+    if (tok >= s.len) continue;
+    float sum = 0.f;
+    for (int rt = 0; rt < p.row_tiles; ++rt) {
+      const float4* from = reinterpret_cast<const float4*>(p.scores + ((first + static_cast<long long>(rt) * s.n + tile) * kTok + k % kTok) * kRows);
+#pragma unroll
+      for (int v = 0; v < kRows / 4; ++v) {
+        const float4 x = from[v];
+        const float* lse = s_lse + rt * kRows + v * 4;
+        sum += ex2f(x.x - lse[0]) + ex2f(x.y - lse[1]) + ex2f(x.z - lse[2]) + ex2f(x.w - lse[3]);
+      }
+    }
+    float* const to = p.weights + b * p.w_sb + h * p.w_sh + tok;
+    *to += sum;
+  }
+}
+
+struct Plan {
+  int nt, row_tiles, ctas;
+  long long most_tiles;  // of a sequence, per head and row tile
+  int64_t o_bytes, ml_bytes, score_bytes, lse_bytes;
+  int64_t total() const { return o_bytes + ml_bytes + score_bytes; }
+};
+
+// kNT = 1 up to 8 query rows per key/value head, else row tiles of 16.
+int make_plan(const rswa_cache_attn_params_t& a, Plan& plan) {
+  const long long rows = static_cast<long long>(a.q_len) * (a.n_q_heads / a.cache.n_kv_heads);
+  plan.nt = rows <= 8 ? 1 : 2;
+  const long long per_tile = 8 * plan.nt;
+  const long long row_tiles = (rows + per_tile - 1) / per_tile;
+  const long long cap = static_cast<long long>(a.table.max_blocks) * a.cache.block_size;
+  long long most = (cap + kTok - 1) / kTok;
+  if (a.window >= 0) {
+    const long long seen = (static_cast<long long>(a.window) + a.q_len + kTok - 1) / kTok + 1 + (static_cast<long long>(a.n_sink) + kTok - 1) / kTok;
+    most = most < seen ? most : seen;
+  }
+  plan.most_tiles = most;
+  const long long items = static_cast<long long>(a.table.batch) * a.cache.n_kv_heads * row_tiles;
+  // (a row tile's log-sum-exps lie in shared memory while the weights are added up)
+  if (row_tiles > 512 || items > 0x7fffffffLL || items * ((most + kWeightTiles - 1) / kWeightTiles) > 0x7fffffffLL) {
+    set_error("rswa_cache_attn: too many queries in one call");
+    return RSWA_E_UNSUPPORTED;
+  }
+  plan.row_tiles = static_cast<int>(row_tiles);
+  const long long share = items * most / kMinShare;
+  const int sms = sm_count();
+  plan.ctas = static_cast<int>(share < 1 ? 1 : share < sms ? share : sms);
+  plan.o_bytes = 2LL * plan.ctas * per_tile * a.cache.head_dim * 4;
+  plan.ml_bytes = (2LL * plan.ctas * per_tile * 2 * 4 + 255) / 256 * 256;
+  plan.score_bytes = a.weights != nullptr ? items * most * kTok * per_tile * 4 : 0;
+  return RSWA_OK;
+}
+
+int check_attn(const rswa_cache_attn_params_t* p) {
+  const char* what = "rswa_cache_attn";
+  if (p == nullptr) {
+    set_error("%s: null params", what);
+    return RSWA_E_ARG;
+  }
+  const rswa_cache_t& c = p->cache;
+  if ((c.head_dim != 64 && c.head_dim != 128) || (c.block_size != 16 && c.block_size != 32 && c.block_size != 64 && c.block_size != 128)) {
+    set_error("%s: head_dim must be 64 or 128 (got %d), block_size 16, 32, 64 or 128 (got %d)", what, c.head_dim, c.block_size);
+    return RSWA_E_UNSUPPORTED;
+  }
+  if (c.n_kv_heads <= 0 || c.n_kv_heads > 32767 || p->n_q_heads <= 0 || p->q_len < 0 || p->n_sink < 0 || p->table.batch < 0 || p->table.max_blocks < 0) {
+    set_error("%s: batch, lengths, sink tokens and head counts must not be negative", what);
+    return RSWA_E_ARG;
+  }
+  if (p->n_q_heads % c.n_kv_heads != 0) {
+    set_error("%s: Number of query heads must be divisible by number of key/value heads", what);
+    return RSWA_E_ARG;
+  }
+  return RSWA_OK;
+}
+
+template <int kD, int kNT, bool kInt8>
+cudaError_t launch_attn(const AttnKernelParams& kp, const Plan& plan, cudaStream_t s) {
+  const auto kern = cache_attn_kernel<kD, kNT, kInt8>;
+  constexpr int smem = Layout<kD, kNT>::kBytes;
+  static std::atomic<uint64_t> set{0};  // devices on which the kernel's shared memory has been allowed
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !(set.load(std::memory_order_relaxed) >> dev & 1)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) set.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  e = launch_kernel(kern, dim3(plan.ctas), kThreads, smem, s, true, kp);
+  if (e != cudaSuccess) return e;
+  const long long items = static_cast<long long>(kp.batch) * kp.c.hkv * plan.row_tiles;
+  e = launch_kernel(cache_join_kernel<kD, kNT, kInt8>, dim3(static_cast<unsigned>(items)), kThreads, 0, s, true, kp);
+  if (e != cudaSuccess) return e;
+  count_launches(2);
+  if (kp.weights != nullptr && plan.most_tiles > 0) {
+    const long long chunks = (plan.most_tiles + kWeightTiles - 1) / kWeightTiles;
+    const dim3 grid(static_cast<unsigned>(static_cast<long long>(kp.batch) * kp.c.hkv * chunks));
+    e = launch_kernel(cache_weights_kernel<kNT>, grid, kThreads, plan.row_tiles * 8 * kNT * 4, s, true, kp, static_cast<int>(chunks));
+    if (e != cudaSuccess) return e;
+    count_launches(1);
+  }
+  return cudaSuccess;
+}
+
+}  // namespace
+
+}  // namespace rswa
+
+using namespace rswa;
+
+extern "C" int64_t rswa_cache_attn_workspace_bytes(const rswa_cache_attn_params_t* p) {
+  int rc = check_attn(p);
+  if (rc != RSWA_OK) return rc;
+  Plan plan;
+  rc = make_plan(*p, plan);
+  return rc != RSWA_OK ? rc : plan.total();
+}
+
+extern "C" int rswa_cache_attn(const rswa_cache_attn_params_t* p, void* stream) {
+  const char* what = "rswa_cache_attn";
+  int rc = check_attn(p);
+  if (rc == RSWA_OK) rc = check_cache(p->cache, what);
+  if (rc == RSWA_OK) rc = check_table(p->table, p->lens, p->status, p->cache.block_size, what);
+  if (rc != RSWA_OK) return rc;
+  if (p->dtype != RSWA_DTYPE_BF16 && p->dtype != RSWA_DTYPE_FP16) {
+    set_error("%s: dtype must be bf16 (0) or fp16 (1), got %d", what, p->dtype);
+    return RSWA_E_UNSUPPORTED;
+  }
+  if (!(p->softmax_scale > 0.f)) {
+    set_error("%s: softmax_scale must be positive", what);
+    return RSWA_E_ARG;
+  }
+  if (p->table.batch == 0 || p->q_len == 0) return RSWA_OK;
+  const auto off = [](const void* x, uintptr_t n) { return x == nullptr || reinterpret_cast<uintptr_t>(x) % n != 0; };
+  if (off(p->q, 16) || off(p->out, 16) || p->q_stride_b % 8 || p->q_stride_t % 8 || p->q_stride_h % 8) {
+    set_error("%s: q and out must be 16-byte aligned, q with strides that are multiples of 8 elements", what);
+    return RSWA_E_ARG;
+  }
+  if (p->weights != nullptr && p->lse == nullptr) {
+    set_error("%s: weights need lse", what);
+    return RSWA_E_ARG;
+  }
+  Plan plan;
+  rc = make_plan(*p, plan);
+  if (rc != RSWA_OK) return rc;
+  if (p->workspace_bytes < plan.total() || off(p->workspace, 256)) {
+    set_error("%s: the workspace must be 256-byte aligned and hold %lld bytes", what, static_cast<long long>(plan.total()));
+    return RSWA_E_ARG;
+  }
+  const rswa_cache_t& c = p->cache;
+  if (c.num_blocks * c.n_kv_heads * c.block_size > 0x7fffffffLL) {
+    set_error("%s: a cache of more than 2^31 rows (blocks x heads x tokens)", what);
+    return RSWA_E_UNSUPPORTED;
+  }
+  AttnKernelParams kp;
+  const long long rows = c.num_blocks * c.n_kv_heads * c.block_size;
+  const int box = c.block_size < kTok ? c.block_size : kTok;
+  rc = make_rows_map(&kp.map[0], c.k, rows, c.head_dim, box);
+  if (rc == RSWA_OK) rc = make_rows_map(&kp.map[1], c.v, rows, c.head_dim, box);
+  if (rc != RSWA_OK) return rc;
+  kp.c = cache_view(c);
+  kp.table = p->table.entries, kp.table_stride = p->table.stride;
+  kp.batch = p->table.batch, kp.max_blocks = p->table.max_blocks;
+  kp.lens = p->lens;
+  kp.q = static_cast<const uint16_t*>(p->q);
+  kp.q_sb = p->q_stride_b, kp.q_st = p->q_stride_t, kp.q_sh = p->q_stride_h;
+  kp.q_len = p->q_len, kp.hq = p->n_q_heads, kp.group = p->n_q_heads / c.n_kv_heads;
+  kp.rows = kp.q_len * kp.group, kp.row_tiles = plan.row_tiles;
+  kp.window = p->window < 0 ? -1 : p->window, kp.n_sink = p->n_sink;
+  kp.scale_log2 = p->softmax_scale * 1.4426950408889634f;
+  kp.bf16 = p->dtype == RSWA_DTYPE_BF16;
+  kp.out = static_cast<uint16_t*>(p->out);
+  kp.lse = p->lse;
+  uint8_t* const ws = static_cast<uint8_t*>(p->workspace);
+  kp.part_o = reinterpret_cast<float*>(ws);
+  kp.part_ml = reinterpret_cast<float*>(ws + plan.o_bytes);
+  kp.scores = p->weights != nullptr ? reinterpret_cast<float*>(ws + plan.o_bytes + plan.ml_bytes) : nullptr;
+  kp.weights = p->weights;
+  kp.w_sb = p->w_stride_b, kp.w_sh = p->w_stride_h;
+  kp.ctas = plan.ctas;
+  kp.status = p->status;
+  kp.mirror = status_mirror(p->status);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool int8 = c.kind == RSWA_CACHE_INT8;
+  cudaError_t e;
+  if (c.head_dim == 64)
+    e = plan.nt == 1 ? (int8 ? launch_attn<64, 1, true>(kp, plan, s) : launch_attn<64, 1, false>(kp, plan, s))
+                     : (int8 ? launch_attn<64, 2, true>(kp, plan, s) : launch_attn<64, 2, false>(kp, plan, s));
+  else
+    e = plan.nt == 1 ? (int8 ? launch_attn<128, 1, true>(kp, plan, s) : launch_attn<128, 1, false>(kp, plan, s))
+                     : (int8 ? launch_attn<128, 2, true>(kp, plan, s) : launch_attn<128, 2, false>(kp, plan, s));
+  if (e != cudaSuccess) {
+    set_error("%s: launch failed: %s", what, cudaGetErrorString(e));
+    return RSWA_E_CUDA;
+  }
+  return RSWA_OK;
+}

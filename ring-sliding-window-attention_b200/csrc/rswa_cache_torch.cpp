@@ -1,0 +1,317 @@
+// Host side of the operators on the 8-bit key/value cache: checks of the tensors, the C ABI's structs, the launch.
+// In C++ for the same reason as the single-GPU calls (rswa_torch.cpp): a decoding step calls each of them once per layer,
+// and through ctypes the host would need longer than the GPU.
+//
+// Every function returns False instead of doing anything where the device has no status word yet or an error of an
+// earlier call has not been raised: Python sees to that and calls again.  Checks that need no device come first.
+#include "rswa_torch.h"
+
+#include <c10/core/GradMode.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
+
+#include <cmath>
+#include <cstring>
+
+#include "../../include/rswa.h"
+
+namespace rswa_host {
+
+namespace {
+
+constexpr int64_t kIntMax = 0x7fffffff;
+
+at::Tensor tensor_arg(PyObject* o, const char* what, const char* name) {
+  TORCH_CHECK_TYPE(THPVariable_Check(o) && THPVariable_CheckTypeExact(Py_TYPE(o)), what, ": ", name, " must be a torch.Tensor, got ", Py_TYPE(o)->tp_name);
+  return THPVariable_Unpack(o);
+}
+int64_t int_arg(PyObject* o, const char* what, const char* name) {
+  const int64_t v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) {
+    PyErr_Clear();
+    TORCH_CHECK_TYPE(false, what, ": ", name, " must be an integer");
+  }
+  return v;
+}
+
+// These operators have no derivative, and a trace or a transform would see only the allocation of their results.
+void check_plain(const at::Tensor& t, const char* what, const char* name) {
+  TORCH_CHECK(!(c10::GradMode::is_enabled() && t.requires_grad()), what, ": ", name,
+              " requires a gradient, which this operator has none of: call it under torch.no_grad() or with a detached tensor");
+  TORCH_CHECK(!t._fw_grad(0).defined(), what, ": no forward-mode derivative");
+}
+void check_mode(const char* what) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), what, ": cannot be traced");
+  TORCH_CHECK(!c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode), what, ": no torch.func transforms");
+}
+void check_16bit(const at::Tensor& t, const char* what, const char* name) {
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, what, ": ", name, " must be bfloat16 or float16, got ", t.scalar_type());
+}
+void check_device(const at::Tensor& t, const at::Tensor& like, const char* what, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.layout() == at::kStrided, what, ": ", name, " must be a CUDA tensor: ring_swa has no CPU path");
+  TORCH_CHECK_VALUE(t.device() == like.device(), what, ": ", name, " is on ", t.device(), ", the cache on ", like.device());
+}
+
+struct Cache {
+  at::Tensor k, v, ks, vs;
+};
+Cache cache_args(PyObject* const* args, const char* what) {
+  Cache c = {tensor_arg(args[0], what, "cache.k"), tensor_arg(args[1], what, "cache.v"), tensor_arg(args[2], what, "cache.k_scale"),
+             tensor_arg(args[3], what, "cache.v_scale")};
+  TORCH_CHECK_VALUE(c.k.dim() == 4 && c.v.sizes() == c.k.sizes() && c.ks.dim() == 2 && c.ks.size(0) == c.k.size(0) && c.ks.size(1) == c.k.size(1) &&
+                        c.vs.sizes() == c.ks.sizes(),
+                    what, ": cache.k and cache.v must be [num_blocks, num_kv_heads, block_size, head_dim], the scales [num_blocks, num_kv_heads]");
+  TORCH_CHECK_VALUE((c.k.scalar_type() == at::kChar || c.k.scalar_type() == at::kFloat8_e4m3fn) && c.v.scalar_type() == c.k.scalar_type() &&
+                        c.ks.scalar_type() == at::kFloat && c.vs.scalar_type() == at::kFloat,
+                    what, ": cache.k and cache.v must both be int8 or both float8_e4m3fn, the scales float32");
+  for (const at::Tensor* t : {&c.k, &c.v, &c.ks, &c.vs}) TORCH_CHECK_VALUE(t->is_contiguous(), what, ": the cache's tensors must be contiguous");
+  TORCH_CHECK_VALUE(c.k.numel() > 0 && c.k.size(0) <= kIntMax && c.k.size(1) <= kIntMax, what, ": the cache is empty or too large");
+  TORCH_CHECK_VALUE((c.k.size(3) == 64 || c.k.size(3) == 128) && (c.k.size(2) == 16 || c.k.size(2) == 32 || c.k.size(2) == 64 || c.k.size(2) == 128), what,
+                    ": head_dim must be 64 or 128 and block_size 16, 32, 64 or 128, got ", c.k.size(3), " and ", c.k.size(2));
+  return c;
+}
+void check_cache_device(const Cache& c, const char* what) {
+  for (const at::Tensor* t : {&c.k, &c.v, &c.ks, &c.vs}) check_device(*t, c.k, what, "the cache");
+}
+rswa_cache_t cache_struct(const Cache& c) {
+  rswa_cache_t r;
+  r.k = c.k.data_ptr(), r.v = c.v.data_ptr();
+  r.k_scale = static_cast<float*>(c.ks.data_ptr()), r.v_scale = static_cast<float*>(c.vs.data_ptr());
+  r.num_blocks = c.k.size(0);
+  r.n_kv_heads = static_cast<int32_t>(c.k.size(1)), r.block_size = static_cast<int32_t>(c.k.size(2)), r.head_dim = static_cast<int32_t>(c.k.size(3));
+  r.kind = c.k.scalar_type() == at::kChar ? RSWA_CACHE_INT8 : RSWA_CACHE_E4M3;
+  return r;
+}
+
+// block table [batch, max_blocks] and lengths [batch]
+void check_table(const at::Tensor& table, const at::Tensor& lens, int64_t block_size, const char* what, const char* name = "block_table") {
+  TORCH_CHECK_VALUE(table.dim() == 2 && lens.dim() == 1 && lens.size(0) == table.size(0), what, ": ", name, " must be [batch, max_blocks] and lens [batch]");
+  TORCH_CHECK_VALUE(table.scalar_type() == at::kInt && lens.scalar_type() == at::kInt, what, ": ", name, " and lens must be int32");
+  TORCH_CHECK_VALUE((table.size(1) <= 1 || table.stride(1) == 1) && (lens.size(0) <= 1 || lens.stride(0) == 1), what, ": rows of ", name,
+                    " and lens must be contiguous");
+  TORCH_CHECK_VALUE(table.size(0) <= kIntMax && table.size(1) <= kIntMax / block_size, what, ": ", name, " is too large");
+}
+rswa_block_table_t table_struct(const at::Tensor& table) {
+  rswa_block_table_t t;
+  t.entries = table.const_data_ptr<int32_t>();
+  // (rows of a table that is one row of another one, repeated, may lie on each other: it is only read)
+  t.stride = table.size(0) > 1 ? table.stride(0) : table.size(1);
+  t.batch = static_cast<int32_t>(table.size(0)), t.max_blocks = static_cast<int32_t>(table.size(1));
+  return t;
+}
+
+// The kernels load 16 bytes at a time along the head dimension.
+at::Tensor loadable(const at::Tensor& t) {
+  bool ok = (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0 && t.stride(-1) == 1;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+int64_t stride_of(const at::Tensor& t, int64_t dim) { return t.size(dim) <= 1 ? 0 : t.stride(dim); }
+
+int32_t dtype_code(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? RSWA_DTYPE_BF16 : RSWA_DTYPE_FP16; }
+
+bool ready(int dev) {
+  if (status_word(dev) == nullptr) return false;
+  if (!reported(dev)) return true;
+  // an error cannot be raised and cleared inside a stream capture
+  cudaStreamCaptureStatus st;
+  return cudaStreamIsCapturing(c10::cuda::getCurrentCUDAStream(dev).stream(), &st) == cudaSuccess && st != cudaStreamCaptureStatusNone;
+}
+void* stream_of(int dev) { return c10::cuda::getCurrentCUDAStream(dev).stream(); }
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// accumulated weights [batch, num_kv_heads, >= tokens]
+void check_weights(const at::Tensor& w, int64_t batch, int64_t heads, int64_t tokens, const char* what, const char* name) {
+  TORCH_CHECK_VALUE(w.scalar_type() == at::kFloat && w.dim() == 3 && w.size(0) == batch && w.size(1) == heads && w.size(2) >= tokens, what, ": ", name,
+                    " must be float32 [batch, num_kv_heads, at least max_blocks * block_size = ", tokens, "], got ", w.sizes());
+  TORCH_CHECK_VALUE((w.size(2) <= 1 || w.stride(2) == 1) && (w.size(1) <= 1 || w.stride(1) >= w.size(2)) &&
+                        (w.size(0) <= 1 || w.stride(0) >= (w.size(1) - 1) * w.stride(1) + w.size(2)),
+                    what, ": ", name, " must be contiguous along the tokens, without rows that overlap");
+}
+
+}  // namespace
+
+// cache_append(k_cache, v_cache, k_scale, v_scale, k, v, block_table, lens, cu_seqlens or None)
+PyObject* py_cache_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const char* what = "cache_append";
+  TORCH_CHECK_TYPE(n == 9, what, " takes 9 arguments");
+  const Cache c = cache_args(args, what);
+  at::Tensor k = tensor_arg(args[4], what, "k"), v = tensor_arg(args[5], what, "v");
+  const at::Tensor table = tensor_arg(args[6], what, "block_table"), lens = tensor_arg(args[7], what, "lens");
+  const at::Tensor cu = args[8] == Py_None ? at::Tensor() : tensor_arg(args[8], what, "cu_seqlens");
+  check_16bit(k, what, "k");
+  TORCH_CHECK_VALUE(k.dim() == (cu.defined() ? 3 : 4), what, ": k must be ", cu.defined() ? "[tokens, num_kv_heads, head_dim] with" : "[batch, tokens, num_kv_heads, head_dim] without",
+                    " cu_seqlens");
+  TORCH_CHECK_VALUE(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type(), what, ": k and v must have the same shape and type");
+  TORCH_CHECK_VALUE(k.size(-2) == c.k.size(1) && k.size(-1) == c.k.size(3), what, ": k has ", k.size(-2), " heads of ", k.size(-1), ", the cache ", c.k.size(1), " of ",
+                    c.k.size(3));
+  check_table(table, lens, c.k.size(2), what);
+  if (cu.defined()) {
+    TORCH_CHECK_VALUE(cu.scalar_type() == at::kInt && cu.dim() == 1 && cu.size(0) == table.size(0) + 1 && (cu.size(0) <= 1 || cu.stride(0) == 1), what,
+                      ": cu_seqlens must be contiguous int32 [batch + 1]");
+  } else {
+    TORCH_CHECK_VALUE(k.size(0) == table.size(0), what, ": k has ", k.size(0), " sequences, block_table ", table.size(0));
+  }
+  TORCH_CHECK_VALUE(k.numel() / (k.size(-1) * k.size(-2)) <= kIntMax, what, ": too many tokens");
+  check_plain(k, what, "k");
+  check_plain(v, what, "v");
+  check_mode(what);
+  check_cache_device(c, what);
+  check_device(k, c.k, what, "k"), check_device(v, c.k, what, "v"), check_device(table, c.k, what, "block_table"), check_device(lens, c.k, what, "lens");
+  if (cu.defined()) check_device(cu, c.k, what, "cu_seqlens");
+  const int dev = c.k.get_device();
+  if (!ready(dev)) Py_RETURN_FALSE;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::cuda::CUDAGuard guard(c.k.device());
+    k = loadable(k), v = loadable(v);
+    rswa_cache_append_params_t p;
+    std::memset(&p, 0, sizeof(p));
+    p.cache = cache_struct(c);
+    p.table = table_struct(table);
+    p.lens = lens.const_data_ptr<int32_t>();
+    p.dtype = dtype_code(k);
+    const int64_t t = k.dim() - 3;  // the token dimension
+    p.tokens = t == 0 ? k.size(0) : k.size(0) * k.size(1);
+    p.cu_seqlens = cu.defined() ? cu.const_data_ptr<int32_t>() : nullptr;
+    p.k = k.const_data_ptr(), p.v = v.const_data_ptr();
+    p.k_stride_b = t == 0 ? 0 : stride_of(k, 0), p.k_stride_t = stride_of(k, t), p.k_stride_h = stride_of(k, t + 1);
+    p.v_stride_b = t == 0 ? 0 : stride_of(v, 0), p.v_stride_t = stride_of(v, t), p.v_stride_h = stride_of(v, t + 1);
+    p.status = status_word(dev);
+    check(rswa_cache_append(&p, stream_of(dev)), what);
+    for (const at::Tensor* w : {&c.k, &c.v, &c.ks, &c.vs}) written(*w);
+  }
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_read(k_cache, v_cache, k_scale, v_scale, block_table, lens, rows, bf16) -> (k, v)
+PyObject* py_cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const char* what = "cache_read";
+  TORCH_CHECK_TYPE(n == 8, what, " takes 8 arguments");
+  const Cache c = cache_args(args, what);
+  const at::Tensor table = tensor_arg(args[4], what, "block_table"), lens = tensor_arg(args[5], what, "lens");
+  const int64_t rows = int_arg(args[6], what, "max_len");
+  const bool bf16 = PyObject_IsTrue(args[7]);
+  check_table(table, lens, c.k.size(2), what);
+  TORCH_CHECK_VALUE(rows >= 0 && rows <= kIntMax - 128, what, ": max_len must be non-negative, got ", rows);
+  check_mode(what);
+  check_cache_device(c, what);
+  check_device(table, c.k, what, "block_table"), check_device(lens, c.k, what, "lens");
+  const int dev = c.k.get_device();
+  if (!ready(dev)) Py_RETURN_FALSE;
+  at::Tensor k, v;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::cuda::CUDAGuard guard(c.k.device());
+    const auto options = c.k.options().dtype(bf16 ? at::kBFloat16 : at::kHalf);
+    k = at::empty({table.size(0), rows, c.k.size(1), c.k.size(3)}, options);
+    v = at::empty(k.sizes(), options);
+    rswa_cache_read_params_t p;
+    std::memset(&p, 0, sizeof(p));
+    p.cache = cache_struct(c);
+    p.table = table_struct(table);
+    p.lens = lens.const_data_ptr<int32_t>();
+    p.dtype = dtype_code(k);
+    p.rows = static_cast<int32_t>(rows);
+    p.k = k.data_ptr(), p.v = v.data_ptr();
+    p.status = status_word(dev);
+    check(rswa_cache_read(&p, stream_of(dev)), what);
+  }
+  return Py_BuildValue("(NN)", THPVariable_Wrap(k), THPVariable_Wrap(v));
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_attn(k_cache, v_cache, k_scale, v_scale, q, block_table, lens, window or None, n_sink, scale or None, weights or None, want_lse)
+//   -> out or (out, lse)
+PyObject* py_cache_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const char* what = "cache_attn";
+  TORCH_CHECK_TYPE(n == 12, what, " takes 12 arguments");
+  const Cache c = cache_args(args, what);
+  at::Tensor q = tensor_arg(args[4], what, "q");
+  const at::Tensor table = tensor_arg(args[5], what, "block_table"), lens = tensor_arg(args[6], what, "lens");
+  int64_t window = -1;
+  if (args[7] != Py_None) {
+    window = int_arg(args[7], what, "window_size");
+    TORCH_CHECK_VALUE(window >= 0, what, ": window_size must be non-negative, or None for every earlier token; got ", window);
+  }
+  const int64_t n_sink = int_arg(args[8], what, "num_sink_tokens");
+  TORCH_CHECK_VALUE(n_sink >= 0, what, ": num_sink_tokens must be non-negative, got ", n_sink);
+  const at::Tensor weights = args[10] == Py_None ? at::Tensor() : tensor_arg(args[10], what, "weights");
+  const bool want_lse = PyObject_IsTrue(args[11]);
+  check_16bit(q, what, "q");
+  TORCH_CHECK_VALUE(q.dim() == 4 && q.size(3) == c.k.size(3), what, ": q must be [batch, queries, num_q_heads, ", c.k.size(3), "], got ", q.sizes());
+  TORCH_CHECK_VALUE(q.size(2) > 0 && q.size(2) % c.k.size(1) == 0, what, ": Number of query heads must be divisible by number of key/value heads, got ", q.size(2),
+                    " and ", c.k.size(1));
+  double scale = 1. / std::sqrt(static_cast<double>(q.size(3)));
+  if (args[9] != Py_None) {
+    scale = PyFloat_AsDouble(args[9]);
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      TORCH_CHECK_TYPE(false, what, ": softmax_scale must be a number");
+    }
+  }
+  TORCH_CHECK_VALUE(static_cast<float>(scale) > 0.f && std::isfinite(static_cast<float>(scale)), what, ": softmax_scale must be positive, got ", scale);
+  check_table(table, lens, c.k.size(2), what);
+  TORCH_CHECK_VALUE(q.size(0) == table.size(0), what, ": q has ", q.size(0), " sequences, block_table ", table.size(0));
+  TORCH_CHECK_VALUE(q.size(1) <= 65536 && q.size(2) <= 65536, what, ": too many queries or heads");
+  if (weights.defined()) check_weights(weights, table.size(0), c.k.size(1), table.size(1) * c.k.size(2), what, "weights");
+  check_plain(q, what, "q");
+  if (weights.defined()) check_plain(weights, what, "weights");
+  check_mode(what);
+  check_cache_device(c, what);
+  check_device(q, c.k, what, "q"), check_device(table, c.k, what, "block_table"), check_device(lens, c.k, what, "lens");
+  if (weights.defined()) check_device(weights, c.k, what, "weights");
+  const int dev = c.k.get_device();
+  if (!ready(dev)) Py_RETURN_FALSE;
+  at::Tensor out, lse;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::cuda::CUDAGuard guard(c.k.device());
+    q = loadable(q);
+    out = at::empty(q.sizes(), q.options());
+    if (want_lse || weights.defined()) lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+    rswa_cache_attn_params_t p;
+    std::memset(&p, 0, sizeof(p));
+    p.cache = cache_struct(c);
+    p.table = table_struct(table);
+    p.lens = lens.const_data_ptr<int32_t>();
+    p.dtype = dtype_code(q);
+    p.q_len = static_cast<int32_t>(q.size(1)), p.n_q_heads = static_cast<int32_t>(q.size(2));
+    p.window = window < 0 ? -1 : static_cast<int32_t>(std::min(window, kIntMax));
+    p.n_sink = static_cast<int32_t>(std::min(n_sink, kIntMax));
+    p.softmax_scale = static_cast<float>(scale);
+    p.q = q.const_data_ptr();
+    p.q_stride_b = stride_of(q, 0), p.q_stride_t = stride_of(q, 1), p.q_stride_h = stride_of(q, 2);
+    p.out = out.data_ptr();
+    p.lse = lse.defined() ? lse.data_ptr<float>() : nullptr;
+    if (weights.defined()) {
+      p.weights = weights.data_ptr<float>();
+      p.w_stride_b = stride_of(weights, 0), p.w_stride_h = stride_of(weights, 1);
+    }
+    p.status = status_word(dev);
+    const int64_t bytes = rswa_cache_attn_workspace_bytes(&p);
+    if (bytes < 0) check(static_cast<int>(bytes), what);
+    // (from the allocator of the current stream: a graph that captures the call keeps it, two calls never share it)
+    const at::Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+    p.workspace = ws.data_ptr();
+    p.workspace_bytes = bytes;
+    check(rswa_cache_attn(&p, stream_of(dev)), what);
+    if (weights.defined()) written(weights);
+  }
+  if (!want_lse) return THPVariable_Wrap(out);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(out), THPVariable_Wrap(lse));
+  END_HANDLE_TH_ERRORS
+}
+
+}  // namespace rswa_host

@@ -27,6 +27,7 @@
 #include <cstring>
 
 #include "../../include/rswa.h"
+#include "rswa_torch.h"
 
 namespace {
 
@@ -102,11 +103,7 @@ void fill_geom(rswa_geom_t& g, const at::Tensor& q, const at::Tensor& k, const a
   s.len = static_cast<int32_t>(dk.tokens);
 }
 
-void check(int rc, const char* what) {
-  if (rc == RSWA_OK) return;
-  if (rc == RSWA_E_ARG || rc == RSWA_E_UNSUPPORTED) TORCH_CHECK_VALUE(false, what, ": ", rswa_last_error());
-  TORCH_CHECK(false, what, ": ", rswa_last_error(), " (code ", rc, ")");
-}
+using rswa_host::check;
 
 // q, k, v (and cu_seqlens) are what the kernels take and fit together.
 bool fits(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu) {
@@ -310,9 +307,29 @@ PyMethodDef g_methods[] = {
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_attention)), METH_FASTCALL,
      "attention(q, k, v, window, n_sink, scale, cu_seqlens) -> out or None (the call is not for this path)"},
     {"new_status", py_new_status, METH_O, "new_status(device_index) -> (status word, host mirror)"},
+    {"cache_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rswa_host::py_cache_append)), METH_FASTCALL,
+     "cache_append(k_cache, v_cache, k_scale, v_scale, k, v, block_table, lens, cu_seqlens) -> None, or False (call again after "
+     "raise_if_reported)"},
+    {"cache_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rswa_host::py_cache_read)), METH_FASTCALL,
+     "cache_read(k_cache, v_cache, k_scale, v_scale, block_table, lens, rows, bf16) -> (k, v), or False"},
+    {"cache_attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rswa_host::py_cache_attn)), METH_FASTCALL,
+     "cache_attn(k_cache, v_cache, k_scale, v_scale, q, block_table, lens, window, n_sink, scale, weights, want_lse) -> out or (out, lse), "
+     "or False"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", "Single-GPU host path of ring_swa", -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
+
+namespace rswa_host {
+
+int32_t* status_word(int device) { return device >= 0 && device < kMaxDevices ? g_status[device] : nullptr; }
+bool reported(int device) { return device >= 0 && device < kMaxDevices && g_mirror[device] != nullptr && *g_mirror[device] != 0; }
+void check(int rc, const char* what) {
+  if (rc == RSWA_OK) return;
+  if (rc == RSWA_E_ARG || rc == RSWA_E_UNSUPPORTED) TORCH_CHECK_VALUE(false, what, ": ", rswa_last_error());
+  TORCH_CHECK(false, what, ": ", rswa_last_error(), " (code ", rc, ")");
+}
+
+}  // namespace rswa_host
 
 PyMODINIT_FUNC PyInit__native(void) { return PyModule_Create(&g_module); }

@@ -88,6 +88,47 @@ class MergeAccParams(C.Structure):
     ]
 
 
+class Cache(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("num_blocks", C.c_int64),
+        ("n_kv_heads", C.c_int32), ("block_size", C.c_int32), ("head_dim", C.c_int32), ("kind", C.c_int32),
+    ]
+
+
+class BlockTable(C.Structure):
+    _fields_ = [("entries", C.c_void_p), ("stride", C.c_int64), ("batch", C.c_int32), ("max_blocks", C.c_int32)]
+
+
+class CacheAppendParams(C.Structure):
+    _fields_ = [
+        ("cache", Cache), ("table", BlockTable), ("lens", C.c_void_p),
+        ("dtype", C.c_int32), ("reserved", C.c_int32), ("tokens", C.c_int64), ("cu_seqlens", C.c_void_p),
+        ("k", C.c_void_p), ("k_stride_b", C.c_int64), ("k_stride_t", C.c_int64), ("k_stride_h", C.c_int64),
+        ("v", C.c_void_p), ("v_stride_b", C.c_int64), ("v_stride_t", C.c_int64), ("v_stride_h", C.c_int64),
+        ("status", C.c_void_p),
+    ]
+
+
+class CacheReadParams(C.Structure):
+    _fields_ = [
+        ("cache", Cache), ("table", BlockTable), ("lens", C.c_void_p),
+        ("dtype", C.c_int32), ("rows", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p), ("status", C.c_void_p),
+    ]
+
+
+class CacheAttnParams(C.Structure):
+    _fields_ = [
+        ("cache", Cache), ("table", BlockTable), ("lens", C.c_void_p),
+        ("dtype", C.c_int32), ("q_len", C.c_int32), ("n_q_heads", C.c_int32), ("window", C.c_int32), ("n_sink", C.c_int32),
+        ("softmax_scale", C.c_float),
+        ("q", C.c_void_p), ("q_stride_b", C.c_int64), ("q_stride_t", C.c_int64), ("q_stride_h", C.c_int64),
+        ("out", C.c_void_p), ("lse", C.c_void_p),
+        ("weights", C.c_void_p), ("w_stride_b", C.c_int64), ("w_stride_h", C.c_int64),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("status", C.c_void_p),
+    ]
+
+
 # every symbol include/rswa.h declares, with its signature
 SYMBOLS = {
     "rswa_launch_count": (C.c_int64, []),
@@ -119,6 +160,10 @@ SYMBOLS = {
     "rswa_event_record": (C.c_int, [C.c_void_p, C.c_void_p]),
     "rswa_event_wait": (C.c_int, [C.c_void_p, C.c_void_p]),
     "rswa_event_elapsed_ms": (C.c_float, [C.c_void_p, C.c_void_p]),
+    "rswa_cache_append": (C.c_int, [C.POINTER(CacheAppendParams), C.c_void_p]),
+    "rswa_cache_read": (C.c_int, [C.POINTER(CacheReadParams), C.c_void_p]),
+    "rswa_cache_attn_workspace_bytes": (C.c_int64, [C.POINTER(CacheAttnParams)]),
+    "rswa_cache_attn": (C.c_int, [C.POINTER(CacheAttnParams), C.c_void_p]),
     "rswa_selftest_mma": (C.c_int, [C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
 }
 

@@ -98,14 +98,25 @@ def _clear_status(device: torch.device) -> None:
     _mirrors[_dev_key(device)].zero_()
 
 
+# errors that are not a wait that ran out (csrc/rswa_cache.cuh)
+_ERROR_TEXT = {
+    110: "a block table entry that is no block of the cache",
+    111: "a length or an offset that is negative or too large for the block table or the tokens given",
+}
+
+
+def _error_text(code: int) -> str:
+    return _ERROR_TEXT.get(code, "a bounded wait ran out")
+
+
 def check_device_status(device: Optional[torch.device] = None) -> None:
-    """Synchronises and raises if any kernel reported a device-side time-out since the last check."""
+    """Synchronises and raises if any kernel reported a device-side time-out or a bad length or block table since the last check."""
     if device is None:
         device = torch.device("cuda", torch.cuda.current_device())
     code = int(status_word(device).item())
     if code != 0:
         _clear_status(device)
-        raise RuntimeError(f"ring_swa kernel reported device-side error code {code} (a bounded wait ran out)")
+        raise RuntimeError(f"ring_swa kernel reported device-side error code {code} ({_error_text(code)})")
 
 
 def raise_if_reported(device: torch.device) -> None:
@@ -117,7 +128,8 @@ def raise_if_reported(device: torch.device) -> None:
     code = int(mirror[0])
     if code != 0 and not torch.cuda.is_current_stream_capturing():
         _clear_status(device)
-        raise RuntimeError(f"ring_swa: a kernel of an earlier call gave up on a bounded device-side wait "
+        what = "gave up on a bounded device-side wait" if code not in _ERROR_TEXT else f"found {_ERROR_TEXT[code]}"
+        raise RuntimeError(f"ring_swa: a kernel of an earlier call {what} "
                            f"(code {code}); the results of that call are invalid. The status word has been "
                            f"cleared, later calls run normally.")
 

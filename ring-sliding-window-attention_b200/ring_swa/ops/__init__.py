@@ -1,6 +1,7 @@
 """Operator-level names of the reference's ring_swa.ops (ring_swa/ops/__init__.py:1-38), all backed by
 librswa.so: the communication helpers, the four attention operators that stand where the
-reference calls flash-attn, the attention-plus-merge steps built on them, and the merge itself."""
+reference calls flash-attn, the attention-plus-merge steps built on them, and the merge itself; and, not in the
+reference, the operators that decode from a key/value cache in 8 bits."""
 from .comm import (
     ring_attn_p2p_communicate,
     broadcast_tensor_to_group,
@@ -21,6 +22,12 @@ from .attn import (
     flash_attn_varlen_bwd_func,
 )
 from .merge import merge_attn_out
+from .kv_cache import (
+    KVCache,
+    cache_append,
+    cache_read,
+    cache_attn,
+)
 
 __all__ = [
     "ring_attn_p2p_communicate",
@@ -37,4 +44,8 @@ __all__ = [
     "flash_attn_varlen_bwd_func",
     "merge_attn_out",
     "get_group_local_to_global_rank_map",
+    "KVCache",
+    "cache_append",
+    "cache_read",
+    "cache_attn",
 ]

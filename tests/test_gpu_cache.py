@@ -1,0 +1,341 @@
+"""The 8-bit key/value cache on the GPU against its definition in 64 bits (tests/cache_ref.py).
+
+Tolerances.  Stored values and scales are exact: scales are powers of two, so that bringing a 16-bit value (or a stored one)
+to a scale is exact in 32 bits and only the rounding to 8 bits, which is the definition's, is left; reading back is exact
+where the target type can hold the value and one rounding otherwise.
+
+Attention: (a) the output's rounding, half a step: eps / 2 * |out|; (b) the weights are rounded to fp16, at most 2^-11 of
+each (2^-25 of the largest for the smallest ones): 2^-11 * sum p|v|; (c) an error e of a score changes each weight by a
+factor within e^(+-e) before and after the division by their sum: 2 e * sum p|v|, where a 32-bit sum of d products
+is off by at most (d + 8) * 2^-24 * sum|q||k| * scale; (d) 32-bit exponentials, sums and scalings, 2^-18 in all.
+The log-sum-exp is off by e, and by the sums' and the logarithm's rounding, 2^-20 relative to 1 and to itself.
+"""
+import math
+import random
+
+import pytest
+import torch
+
+import cache_ref as R
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def _ops():
+    from ring_swa import ops
+    return ops
+
+
+def make(kind, num_blocks, heads, bs, d, seed, garbage=True):
+    """A cache on the GPU whose unused blocks hold what must not matter: arbitrary bytes, NaN scales."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(seed)
+    cache = ops.KVCache.empty(num_blocks, heads, bs, d, dtype=R.TORCH[kind])
+    if garbage:
+        for x in (cache.k, cache.v):
+            x.view(torch.uint8).copy_(torch.randint(0, 256, x.shape, generator=g, dtype=torch.uint8))
+        cache.k_scale.fill_(math.nan)
+        cache.v_scale.fill_(math.nan)
+    return cache
+
+
+def host(cache):
+    return {"k": cache.k.cpu().float().double(), "v": cache.v.cpu().float().double(),
+            "k_scale": cache.k_scale.cpu().double(), "v_scale": cache.v_scale.cpu().double()}
+
+
+def tables(lens, bs, max_blocks, num_blocks, seed):
+    r = random.Random(seed)
+    pages = r.sample(range(num_blocks), num_blocks)
+    table = torch.full((len(lens), max_blocks), -1, dtype=torch.int32)
+    for i, n in enumerate(lens):
+        for j in range((n + bs - 1) // bs):
+            table[i, j] = pages.pop()
+    return table
+
+
+def normal(*shape, seed, dt):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(DT[dt])
+
+
+def filled(kind, dt, lens, heads, bs, d, seed, v_spread=False, spare=3):
+    """A cache with `lens` tokens per sequence, written by cache_append in one packed call, and its table."""
+    ops = _ops()
+    blocks = [(n + bs - 1) // bs for n in lens]
+    total = sum(blocks) + spare
+    table = tables(lens, bs, max(blocks + [1]) + 1, total, seed)
+    cache = make(kind, total, heads, bs, d, seed)
+    t = sum(lens)
+    k, v = normal(t, heads, d, seed=seed + 1, dt=dt), normal(t, heads, d, seed=seed + 2, dt=dt)
+    if v_spread:  # blocks of very different magnitudes
+        v = (v.float() * torch.exp2(torch.arange(t)[:, None, None] % 40 / 4.0 - 5)).to(DT[dt])
+    cu = torch.tensor([0] + list(torch.tensor(lens).cumsum(0)), dtype=torch.int32)
+    ops.cache_append(cache, k.cuda(), v.cuda(), table.cuda(), torch.zeros(len(lens), dtype=torch.int32, device="cuda"), cu_seqlens=cu.cuda())
+    return cache, table, k, v, cu
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dt,bs,d,heads", [("bf16", 16, 64, 1), ("bf16", 64, 128, 3), ("fp16", 128, 128, 2), ("fp16", 32, 64, 8), ("bf16", 128, 64, 2),
+                                           ("bf16", 16, 128, 4)])
+def test_append_and_read_are_exact(kind, dt, bs, d, heads):
+    ops = _ops()
+    first, more, last = [0, 1, bs, 3 * bs - 1, 5, 2 * bs], [bs + 3, 1, 0, 2, 2 * bs, 1], [1, 1, 1, 1, 1, 1]
+    lens = [0] * 6
+    room = [(a + b + 1 + bs - 1) // bs for a, b in zip(first, more)]
+    table = tables([n * bs for n in room], bs, max(room) + 1, sum(room) + 2, seed=5)
+    cache = make(kind, sum(room) + 2, heads, bs, d, seed=6)
+    ref = host(cache)
+    for step, counts in enumerate((first, more, last)):
+        t = sum(counts)
+        # every step's values are larger in some sequences: scales of blocks in use have to grow
+        grow = torch.repeat_interleave(torch.tensor([1.0, 3.0, 0.1, 9.0, 1.0, 40.0]) ** step, torch.tensor(counts))[:, None, None]
+        k, v = ((normal(t, heads, d, seed=10 * step + i, dt=dt).float() * grow).to(DT[dt]) for i in (0, 1))
+        cu = torch.tensor([0] + torch.tensor(counts).cumsum(0).tolist(), dtype=torch.int32)
+        R.append(ref, kind, table.tolist(), lens, [x.double() for x in k.split(counts)], [x.double() for x in v.split(counts)], counts)
+        at = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        if step < 2:
+            ops.cache_append(cache, k.cuda(), v.cuda(), table.cuda(), at, cu_seqlens=cu.cuda())
+        else:
+            ops.cache_append(cache, k.view(6, 1, heads, d).cuda(), v.view(6, 1, heads, d).cuda(), table.cuda(), at)
+        lens = [a + b for a, b in zip(lens, counts)]
+        got = host(cache)
+        for name in ("k", "v", "k_scale", "v_scale"):  # (unused blocks and slots included: left as they were)
+            torch.testing.assert_close(got[name], ref[name], rtol=0, atol=0, equal_nan=True)
+    for most in (1, max(lens) - 1, max(lens), max(lens) + bs):
+        for out in ("bf16", "fp16"):
+            got = ops.cache_read(cache, table.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"), most, dtype=DT[out])
+            for x, name in zip(got, ("k", "v")):
+                want = torch.zeros(6, most, heads, d, dtype=torch.float64)
+                for i, n in enumerate(lens):
+                    y = R.rows(ref, name, table[i], n)[:most]
+                    want[i, :y.shape[0]] = y
+                assert torch.equal(x.cpu(), want.float().to(DT[out]))
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_append_edges(kind):
+    """Zeros, the smallest and the largest values, infinities and NaN; exact ends of the range; a slice of a fused projection."""
+    ops = _ops()
+    heads, bs, d = 2, 16, 64
+    top = R.TOP[kind]
+    x = torch.randn(6 * bs, 3 * heads, d, generator=torch.Generator().manual_seed(0)).bfloat16()
+    k = x[:, heads:2 * heads]
+    k[0:bs] = 0
+    k[bs:2 * bs] = 1e-38
+    k[2 * bs:3 * bs] = 3e38
+    k[3 * bs, 0, 0], k[3 * bs, 1, 0] = math.inf, math.nan
+    k[4 * bs:5 * bs].clamp_(-1, 1)[0, 0, 0] = torch.tensor(top * 2 ** 3).bfloat16()
+    k[5 * bs:].clamp_(-1, 1)
+    k[5 * bs, 0, 0] = torch.nextafter(torch.tensor(top).bfloat16(), torch.tensor(1e9).bfloat16())
+    cache = make(kind, 8, heads, bs, d, seed=1)
+    ref = host(cache)
+    table = torch.tensor([[7, 0, 3, 5, 2, 1, 4]], dtype=torch.int32)
+    xs = x.cuda()
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    R.append(ref, kind, table.tolist(), [0], [x[:, heads:2 * heads].double()], [x[:, 2 * heads:].double()], [6 * bs])
+    ops.cache_append(cache, xs[None, :, heads:2 * heads], xs[None, :, 2 * heads:], table.cuda(), zero)
+    got = host(cache)
+    bad = torch.isnan(ref["k_scale"])
+    assert torch.equal(torch.isnan(got["k_scale"]), bad) and bad[5].all() and not bad[[7, 0, 3, 2, 1]].any()
+    torch.testing.assert_close(got["k_scale"], ref["k_scale"], rtol=0, atol=0, equal_nan=True)
+    for page in (7, 0, 3, 2, 1):
+        assert torch.equal(got["k"][page], ref["k"][page])
+    torch.testing.assert_close(got["v"], ref["v"], rtol=0, atol=0, equal_nan=True)
+    # a token behind a poisoned block's: the block stays NaN, its neighbours do not care
+    k2, v2 = ops.cache_read(cache, table.cuda(), torch.tensor([6 * bs], dtype=torch.int32, device="cuda"), 6 * bs)
+    assert torch.isnan(k2[0, 3 * bs:4 * bs]).all() and torch.isfinite(k2[0, :2 * bs]).all() and torch.isfinite(k2[0, 4 * bs:]).all()
+    assert torch.isfinite(v2).all()
+
+
+def check_attn(cache, table, lens, q, window, sink, scale=None, weights=None):
+    ops = _ops()
+    dt = q.dtype
+    ref = host(cache)
+    dev = [t.cuda() for t in (q, table, torch.tensor(lens, dtype=torch.int32))]
+    acc = None if weights is None else weights.cuda().clone()
+    out, lse = ops.cache_attn(dev[0], cache, dev[1], dev[2], window_size=window, num_sink_tokens=sink, softmax_scale=scale, weights=acc,
+                              return_lse=True)
+    want, want_lse, w, size, most = R.attn(ref, table, lens, q.double(), window, sink, scale)
+    e = (q.shape[-1] + 8) * 2.0 ** -24 * most
+    eps = torch.finfo(dt).eps / 2
+    tol = eps * want.abs() + (1 + eps) * (2.0 ** -11 + 2 * e + 2.0 ** -18) * size + 1e-30
+    err = (out.cpu().double() - want).abs()
+    assert torch.isfinite(out).all()
+    assert (err <= tol).all(), f"out: {(err / tol).max().item():.3g} of the tolerance"
+    none = torch.isinf(want_lse)
+    got_lse = lse.cpu().double()
+    assert torch.equal(torch.isinf(got_lse), none)
+    assert ((got_lse - want_lse).abs()[~none] <= e + 2.0 ** -20 * (1 + want_lse[~none].abs())).all()
+    if weights is not None:
+        n = w.shape[-1]
+        got = acc.cpu().double()
+        assert torch.equal(got[..., n:], weights[..., n:].double()), "weights behind the last slot were written"
+        d = (got[..., :n] - weights[..., :n].double() - w).abs()
+        rows = q.shape[1] * q.shape[2]
+        assert (d <= (2 * e + 2.0 ** -18 + rows * 2.0 ** -24) * w + 2.0 ** -24 * (weights[..., :n].double() + w)).all()
+    return out
+
+
+CASES = [
+    # lens, (hq, hkv), d, bs, queries, window, sink
+    ([1], (1, 1), 64, 16, 1, None, 0),
+    ([33, 1, 0, 17, 16], (4, 4), 64, 16, 1, None, 0),
+    ([513], (4, 4), 64, 16, 1, None, 0),
+    ([100, 31, 32, 64, 65, 0, 2], (8, 2), 128, 32, 1, None, 0),
+    ([300, 1000, 7], (32, 8), 128, 64, 1, None, 0),
+    ([2500, 130], (64, 8), 128, 128, 1, None, 0),
+    ([777, 40], (16, 1), 128, 16, 1, None, 0),        # 16 rows: two columns of 8
+    ([1029, 3, 250], (32, 4), 128, 64, 4, None, 0),   # 32 rows: two row tiles; queries before the start
+    ([260, 8], (12, 4), 64, 32, 5, 100, 0),
+    ([2000, 50, 700], (32, 8), 128, 128, 1, 256, 4),
+    ([2000, 50, 700], (8, 2), 64, 16, 3, 33, 1),
+    ([1500, 1499], (16, 16), 128, 16, 2, 31, 40),
+    ([4000], (4, 1), 128, 32, 1, 0, 0),               # itself alone
+    ([900], (4, 2), 128, 64, 1, 0, 1),
+    ([600, 599], (40, 1), 64, 64, 7, 1 << 30, 1 << 30),
+]
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_attn(case, kind):
+    lens, (hq, hkv), d, bs, n, window, sink = CASES[case]
+    dt = "fp16" if case % 3 == 1 else "bf16"
+    cache, table, _, _, _ = filled(kind, dt, lens, hkv, bs, d, seed=case, v_spread=case % 2 == 0)
+    q = normal(len(lens), n, hq, d, seed=100 + case, dt=dt)
+    w = torch.rand(len(lens), hkv, table.shape[1] * bs + 5, generator=torch.Generator().manual_seed(case)) if case % 4 != 3 else None
+    check_attn(cache, table, lens, q, window, sink, scale=0.3 if case % 5 == 2 else None, weights=w)
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_attn_far_apart_scores_and_query_sizes(kind):
+    """Scores of +-300 and queries from 2^-60 to 2^60: the running reference and the queries' scaling."""
+    lens, bs, d = [700, 345], 32, 128
+    cache, table, _, _, _ = filled(kind, "bf16", lens, 2, bs, d, seed=3)
+    for mul in (40.0, 2.0 ** -60, 1.0):
+        q = (normal(2, 1, 8, d, seed=9, dt="bf16").float() * mul).bfloat16()
+        check_attn(cache, table, lens, q, None, 0)
+    q = (normal(2, 1, 8, d, seed=9, dt="bf16").float() * 2.0 ** 60).bfloat16()
+    check_attn(cache, table, lens, q, None, 0, scale=d ** -0.5 * 2.0 ** -60)
+
+
+def test_attn_of_a_poisoned_block():
+    """NaN reaches the rows and heads that see the block, and no others."""
+    lens, bs, d = [200], 16, 64
+    cache, table, _, _, _ = filled("int8", "bf16", lens, 2, bs, d, seed=4)
+    cache.v_scale[table[0, 3].item(), 1] = math.nan       # slots 48..63 of head 1
+    cache.k_scale[table[0, 12].item(), 0] = math.nan      # slots 192..199 of head 0: the newest
+    q = normal(1, 12, 4, d, seed=5, dt="bf16")
+    args = (q.cuda(), cache, table.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    out = _ops().cache_attn(*args)
+    # head 0 (rows of q heads 0, 1): queries from slot 192 on, the last 8; head 1: every query
+    assert torch.isnan(out[0, 4:, :2]).all() and torch.isfinite(out[0, :4, :2]).all() and torch.isnan(out[0, :, 2:]).all()
+    out = _ops().cache_attn(*args, window_size=100)
+    assert torch.isfinite(out[0, :, 2:]).all()
+    out = _ops().cache_attn(*args, window_size=128)
+    # query i at slot 188 + i sees from 60 + i on
+    assert torch.isnan(out[0, :4, 2:]).all() and torch.isfinite(out[0, 4:, 2:]).all()
+
+
+def test_attn_strided_queries_scales_and_results_do_not_depend_on_the_run():
+    lens, bs, d = [5000, 3, 1234, 2048], 64, 128
+    cache, table, _, _, _ = filled("int8", "bf16", lens, 4, bs, d, seed=8)
+    fused = normal(4, 2, 24, d, seed=1, dt="bf16")
+    q = fused[:, :, :16]
+    a = check_attn(cache, table, lens, q, 3000, 2)
+    b = check_attn(cache, table, lens, q.contiguous(), 3000, 2)
+    assert torch.equal(a, b)
+    # scales that are no powers of two
+    cache.k_scale.mul_(1.37)
+    cache.v_scale.mul_(0.71)
+    check_attn(cache, table, lens, q, None, 0)
+    # unaligned and otherwise strided queries
+    odd = torch.empty(4 * 2 * 16 * d + 1, dtype=torch.bfloat16)[1:].view(4, 2, 16, d).copy_(q)
+    check_attn(cache, table, lens, odd, None, 0)
+    check_attn(cache, table, lens, q[:1].expand(4, 2, 16, d), None, 0)
+
+
+def test_many_sequences_of_all_lengths():
+    r = random.Random(0)
+    lens = [r.choice((0, 1, 15, 16, 17, 31, 33, 64, 100, 200)) for _ in range(300)]
+    cache, table, _, _, _ = filled("e4m3", "bf16", lens, 1, 16, 64, seed=2)
+    q = normal(300, 1, 2, 64, seed=3, dt="bf16")
+    w = torch.zeros(300, 1, table.shape[1] * 16)
+    check_attn(cache, table, lens, q, None, 0, weights=w)
+    check_attn(cache, table, lens, q, 20, 3)
+
+
+def test_bad_tables_and_lengths_are_reported():
+    from ring_swa import _kernels as K
+    ops = _ops()
+    lens, bs, d = [100, 50], 16, 64
+    cache, table, _, _, _ = filled("int8", "bf16", lens, 2, bs, d, seed=4)
+    before = host(cache)
+    q = normal(2, 1, 4, d, seed=5, dt="bf16").cuda()
+    new = normal(2, 1, 2, d, seed=5, dt="bf16").cuda()
+    good = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    for bad, n, code in (([[0, 2, -1], [0, 2, 1 << 30]], None, 110), (None, [[100, -1], [100, 10000]], 111)):
+        for i in range(2):
+            t, l = table.clone(), good.clone()
+            if bad is not None:
+                t[bad[i][0], bad[i][1]] = bad[i][2]
+            if n is not None:
+                l = torch.tensor(n[i], dtype=torch.int32, device="cuda")
+            calls = [lambda: ops.cache_attn(q, cache, t.cuda(), l), lambda: ops.cache_read(cache, t.cuda(), l, 112)]
+            if n is not None:
+                calls.append(lambda: ops.cache_append(cache, new[1:], new[1:], t[1:].cuda(), l[1:]))
+            for call in calls:
+                call()
+                torch.cuda.synchronize()
+                with pytest.raises(RuntimeError, match=f"code {code}"):
+                    ops.cache_read(cache, table.cuda(), good, 1)
+                K.check_device_status()  # (cleared)
+    after = host(cache)
+    for name in before:
+        torch.testing.assert_close(after[name], before[name], rtol=0, atol=0, equal_nan=True)
+    check_attn(cache, table, lens, q.cpu(), None, 0)
+
+
+def test_a_captured_step_is_replayed_with_other_lengths_and_on_another_stream():
+    """append + attention captured once and replayed for five tokens; two such graphs run at the same time on two streams."""
+    ops = _ops()
+    bs, d, hkv, hq = 16, 128, 2, 8
+    runs = []
+    for seed in (0, 1):
+        lens = [30 + 700 * seed, 100, 15]
+        cache, table, _, _, _ = filled("int8", "bf16", [n + 8 for n in lens], hkv, bs, d, seed=seed, spare=0)
+        table = table.cuda()
+        runs.append(dict(cache=cache, table=table, lens=torch.tensor(lens, dtype=torch.int32, device="cuda"), host=lens,
+                         q=torch.zeros(3, 1, hq, d, dtype=torch.bfloat16, device="cuda"), k=torch.zeros(3, 1, hkv, d, dtype=torch.bfloat16, device="cuda"),
+                         v=torch.zeros(3, 1, hkv, d, dtype=torch.bfloat16, device="cuda"), w=torch.zeros(3, hkv, table.shape[1] * bs, device="cuda"),
+                         stream=torch.cuda.Stream()))
+    for r in runs:
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            ops.cache_append(r["cache"], r["k"], r["v"], r["table"], r["lens"])
+            r["lens"].add_(1)
+            r["out"] = ops.cache_attn(r["q"], r["cache"], r["table"], r["lens"], window_size=600, num_sink_tokens=2, weights=r["w"])
+        r["graph"] = g
+        r["eager"] = ops.KVCache(*(t.clone() for t in (r["cache"].k, r["cache"].v, r["cache"].k_scale, r["cache"].v_scale)))
+        r["eager_w"] = r["w"].clone()
+    for step in range(5):
+        for i, r in enumerate(runs):
+            for j, name in enumerate(("q", "k", "v")):
+                r[name].copy_(normal(*r[name].shape, seed=100 * step + 10 * i + j, dt="bf16"))
+        torch.cuda.synchronize()
+        for r in runs:
+            with torch.cuda.stream(r["stream"]):
+                r["graph"].replay()
+        torch.cuda.synchronize()
+        for r in runs:
+            at = torch.tensor([n + step for n in r["host"]], dtype=torch.int32, device="cuda")
+            ops.cache_append(r["eager"], r["k"], r["v"], r["table"], at)
+            want = ops.cache_attn(r["q"], r["eager"], r["table"], at + 1, window_size=600, num_sink_tokens=2, weights=r["eager_w"])
+            assert torch.equal(r["out"], want) and torch.equal(r["w"], r["eager_w"])
+            assert torch.equal(r["lens"], at + 1)
+            for name in ("k", "v"):
+                assert torch.equal(getattr(r["cache"], name).view(torch.uint8), getattr(r["eager"], name).view(torch.uint8))
