@@ -383,6 +383,60 @@ typedef struct rswa_cache_attn_params {
 int64_t rswa_cache_attn_workspace_bytes(const rswa_cache_attn_params_t* p);
 int rswa_cache_attn(const rswa_cache_attn_params_t* p, void* stream);
 
+/* The softmax weights that the queries of a prompt gave to each of its keys, summed over the query heads of a
+ * key/value head: out [batch, n_kv_heads, len] float, contiguous,
+ *   out[b, h, t] = sum over heads of the group and queries i that see t of exp(softmax_scale * q_i.k_t - lse_i)
+ * with the mask of rswa_fwd for one span that starts at position 0 (packed sequences with cu_seqlens and batch 1), and
+ * lse [batch, n_q_heads, len] (natural log, tokens contiguous) as rswa_fwd wrote it.  A query with lse -inf gives
+ * nothing.  q and k 16-bit, strides in elements as in rswa_fwd.  `workspace`: rswa_weight_sums_workspace_bytes() of
+ * device memory for the time of the call. */
+typedef struct rswa_weight_sums_params {
+  int32_t dtype;
+  int32_t batch, len, n_q_heads, n_kv_heads, head_dim; /* head_dim 64 or 128 */
+  int32_t window, n_sink;
+  float softmax_scale;
+  int32_t n_seqs;
+  const int32_t* cu_seqlens;
+  const void* q;
+  int64_t q_stride_b, q_stride_t, q_stride_h;
+  const void* k;
+  int64_t k_stride_b, k_stride_t, k_stride_h;
+  const float* lse;
+  int64_t lse_stride_b, lse_stride_h;
+  float* out;
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t* status;
+} rswa_weight_sums_params_t;
+
+int64_t rswa_weight_sums_workspace_bytes(const rswa_weight_sums_params_t* p);
+int rswa_weight_sums(const rswa_weight_sums_params_t* p, void* stream);
+
+/* Thins every sequence out to at most `budget` tokens: the first n_sink, the last n_recent, and as many as there is
+ * room for of those in between with the largest weights[b, h, slot] (of equal ones the ones in the lowest slots; NaN counts
+ * as the largest), chosen per key/value head.  They keep their order and are packed into the blocks that new_table names, which must be no
+ * blocks of the old table's (and belong to one sequence each), with the least scales that hold them.
+ *   new_lens [batch] = min(lens, budget)
+ *   new_weights [batch, n_kv_heads, new_w_len]: the kept tokens' weights, 0 behind them; new_w_len >= the tokens of new_table
+ *   kept [batch, n_kv_heads, budget]: the kept tokens' old slots, -1 behind them
+ * (both contiguous).  n_sink + n_recent <= budget; new_table must hold min(budget, the tokens of the old table). */
+typedef struct rswa_cache_evict_params {
+  rswa_cache_t cache;
+  rswa_block_table_t table;
+  const int32_t* lens;
+  const float* weights; /* [batch, n_kv_heads, >= max_blocks * block_size], slots contiguous */
+  int64_t w_stride_b, w_stride_h;
+  int32_t budget, n_sink, n_recent;
+  int32_t new_w_len;
+  rswa_block_table_t new_table;
+  int32_t* new_lens;
+  float* new_weights;
+  int32_t* kept;
+  int32_t* status;
+} rswa_cache_evict_params_t;
+
+int rswa_cache_evict(const rswa_cache_evict_params_t* p, void* stream);
+
 /* Kernels of this library launched by the process so far. */
 int64_t rswa_launch_count(void);
 

@@ -21,7 +21,7 @@ NATIVE_STAMP = NATIVE_OUT + ".stamp"
 NATIVE_SOURCES = [os.path.join(CSRC, s) for s in ("rswa_torch.cpp", "rswa_cache_torch.cpp")]
 NATIVE_HEADERS = [os.path.join(CSRC, "rswa_torch.h"), os.path.join(CSRC, "..", "..", "include", "rswa.h")]
 SOURCES = ["rswa_api.cu", "rswa_fwd.cu", "rswa_bwd.cu", "rswa_dq.cu", "rswa_aux.cu", "rswa_selftest.cu", "rswa_noalloc.cu", "rswa_peer.cu", "rswa_cache.cu",
-           "rswa_cache_attn.cu"]
+           "rswa_cache_attn.cu", "rswa_sums.cu", "rswa_evict.cu"]
 HEADERS = ["tc05.cuh", "rswa_common.cuh", "rswa_tiles.cuh", "rswa_cache.cuh", os.path.join("..", "..", "include", "rswa.h")]
 
 

@@ -105,10 +105,10 @@ rswa_block_table_t table_struct(const at::Tensor& table) {
   return t;
 }
 
-// The kernels load 16 bytes at a time along the head dimension.
-at::Tensor loadable(const at::Tensor& t) {
+// The kernels load 16 bytes at a time along the head dimension; through tensor maps they want positive strides besides.
+at::Tensor loadable(const at::Tensor& t, bool map = false) {
   bool ok = (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0 && t.stride(-1) == 1;
-  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.size(i) <= 1 || (t.stride(i) % 8 == 0 && (!map || t.stride(i) > 0)));
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 int64_t stride_of(const at::Tensor& t, int64_t dim) { return t.size(dim) <= 1 ? 0 : t.stride(dim); }
@@ -311,6 +311,142 @@ PyObject* py_cache_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   if (!want_lse) return THPVariable_Wrap(out);
   return Py_BuildValue("(NN)", THPVariable_Wrap(out), THPVariable_Wrap(lse));
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_evict(k_cache, v_cache, k_scale, v_scale, block_table, lens, weights, budget, new_block_table, n_sink, n_recent)
+//   -> (new_lens, new_weights, kept)
+PyObject* py_cache_evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const char* what = "cache_evict";
+  TORCH_CHECK_TYPE(n == 11, what, " takes 11 arguments");
+  const Cache c = cache_args(args, what);
+  const at::Tensor table = tensor_arg(args[4], what, "block_table"), lens = tensor_arg(args[5], what, "lens");
+  const at::Tensor weights = tensor_arg(args[6], what, "weights"), new_table = tensor_arg(args[8], what, "new_block_table");
+  const int64_t budget = int_arg(args[7], what, "budget"), n_sink = int_arg(args[9], what, "num_sink_tokens"), n_recent = int_arg(args[10], what, "num_recent_tokens");
+  const int64_t bs = c.k.size(2);
+  check_table(table, lens, bs, what);
+  check_table(new_table, lens, bs, what, "new_block_table");
+  check_weights(weights, table.size(0), c.k.size(1), table.size(1) * bs, what, "weights");
+  TORCH_CHECK_VALUE(budget > 0 && budget <= kIntMax, what, ": budget must be positive, got ", budget);
+  TORCH_CHECK_VALUE(n_sink >= 0 && n_recent >= 0 && n_sink <= budget && n_recent <= budget - n_sink, what, ": num_sink_tokens (", n_sink, ") and num_recent_tokens (", n_recent,
+                    ") must not be negative and fit into the budget of ", budget);
+  TORCH_CHECK_VALUE(new_table.size(1) * bs >= std::min(budget, table.size(1) * bs), what, ": new_block_table holds ", new_table.size(1) * bs,
+                    " tokens per sequence, but ", std::min(budget, table.size(1) * bs), " may stay");
+  check_plain(weights, what, "weights");
+  check_mode(what);
+  check_cache_device(c, what);
+  check_device(table, c.k, what, "block_table"), check_device(lens, c.k, what, "lens"), check_device(weights, c.k, what, "weights");
+  check_device(new_table, c.k, what, "new_block_table");
+  const int dev = c.k.get_device();
+  if (!ready(dev)) Py_RETURN_FALSE;
+  at::Tensor new_lens, new_weights, kept;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::cuda::CUDAGuard guard(c.k.device());
+    new_lens = at::empty({table.size(0)}, lens.options());
+    new_weights = at::empty({table.size(0), c.k.size(1), new_table.size(1) * bs}, weights.options());
+    kept = at::empty({table.size(0), c.k.size(1), budget}, lens.options());
+    rswa_cache_evict_params_t p;
+    std::memset(&p, 0, sizeof(p));
+    p.cache = cache_struct(c);
+    p.table = table_struct(table);
+    p.new_table = table_struct(new_table);
+    p.lens = lens.const_data_ptr<int32_t>();
+    p.weights = weights.const_data_ptr<float>();
+    p.w_stride_b = stride_of(weights, 0), p.w_stride_h = stride_of(weights, 1);
+    p.budget = static_cast<int32_t>(budget), p.n_sink = static_cast<int32_t>(n_sink), p.n_recent = static_cast<int32_t>(n_recent);
+    p.new_w_len = static_cast<int32_t>(new_weights.size(2));
+    p.new_lens = new_lens.data_ptr<int32_t>();
+    p.new_weights = new_weights.data_ptr<float>();
+    p.kept = kept.data_ptr<int32_t>();
+    p.status = status_word(dev);
+    check(rswa_cache_evict(&p, stream_of(dev)), what);
+    for (const at::Tensor* w : {&c.k, &c.v, &c.ks, &c.vs}) written(*w);
+  }
+  return Py_BuildValue("(NNN)", THPVariable_Wrap(new_lens), THPVariable_Wrap(new_weights), THPVariable_Wrap(kept));
+  END_HANDLE_TH_ERRORS
+}
+
+// weight_sums(q, k, lse, window or None, n_sink, scale or None, cu_seqlens or None) -> sums
+PyObject* py_weight_sums(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const char* what = "attn_weight_sums";
+  TORCH_CHECK_TYPE(n == 7, what, " takes 7 arguments");
+  at::Tensor q = tensor_arg(args[0], what, "q"), k = tensor_arg(args[1], what, "k"), lse = tensor_arg(args[2], what, "softmax_lse");
+  const at::Tensor cu = args[6] == Py_None ? at::Tensor() : tensor_arg(args[6], what, "cu_seqlens");
+  int64_t window = kIntMax;
+  if (args[3] != Py_None) {
+    window = int_arg(args[3], what, "window_size");
+    TORCH_CHECK_VALUE(window >= 0, what, ": window_size must be non-negative, or None for every earlier token; got ", window);
+  }
+  const int64_t n_sink = int_arg(args[4], what, "num_sink_tokens");
+  TORCH_CHECK_VALUE(n_sink >= 0, what, ": num_sink_tokens must be non-negative, got ", n_sink);
+  check_16bit(q, what, "q");
+  const int64_t dims = cu.defined() ? 3 : 4, t = dims - 3;  // the token dimension
+  TORCH_CHECK_VALUE(q.dim() == dims && k.dim() == dims, what, ": q and k must be ", cu.defined() ? "[tokens, heads, head_dim] with" : "[batch, tokens, heads, head_dim] without", " cu_seqlens");
+  TORCH_CHECK_VALUE(k.scalar_type() == q.scalar_type() && k.size(-1) == q.size(-1) && k.size(t) == q.size(t) && (t == 0 || k.size(0) == q.size(0)), what,
+                    ": q and k must have the same type, head dimension and number of tokens");
+  TORCH_CHECK_VALUE(q.size(-1) == 64 || q.size(-1) == 128, what, ": head_dim must be 64 or 128, got ", q.size(-1));
+  TORCH_CHECK_VALUE(k.size(-2) > 0 && q.size(-2) > 0 && q.size(-2) % k.size(-2) == 0, what, ": Number of query heads must be divisible by number of key/value heads, got ",
+                    q.size(-2), " and ", k.size(-2));
+  const int64_t batch = t == 0 ? 1 : q.size(0), len = q.size(t), hq = q.size(-2), hkv = k.size(-2);
+  TORCH_CHECK_VALUE(batch <= kIntMax && len <= kIntMax && hq <= kIntMax, what, ": too large");
+  TORCH_CHECK_VALUE(lse.scalar_type() == at::kFloat && lse.dim() == dims - 1 && lse.size(-1) == len && lse.size(-2) == hq && (t == 0 || lse.size(0) == batch), what,
+                    ": softmax_lse must be float32 ", cu.defined() ? "[num_q_heads, tokens]" : "[batch, num_q_heads, tokens]", ", got ", lse.sizes());
+  if (cu.defined())
+    TORCH_CHECK_VALUE(cu.scalar_type() == at::kInt && cu.dim() == 1 && cu.size(0) >= 2 && cu.stride(0) == 1, what, ": cu_seqlens must be contiguous int32 [sequences + 1]");
+  double scale = 1. / std::sqrt(static_cast<double>(q.size(-1)));
+  if (args[5] != Py_None) {
+    scale = PyFloat_AsDouble(args[5]);
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      TORCH_CHECK_TYPE(false, what, ": softmax_scale must be a number");
+    }
+  }
+  TORCH_CHECK_VALUE(static_cast<float>(scale) > 0.f && std::isfinite(static_cast<float>(scale)), what, ": softmax_scale must be positive, got ", scale);
+  check_plain(q, what, "q"), check_plain(k, what, "k"), check_plain(lse, what, "softmax_lse");
+  check_mode(what);
+  TORCH_CHECK(q.is_cuda() && q.layout() == at::kStrided, what, ": q must be a CUDA tensor: ring_swa has no CPU path");
+  for (const at::Tensor* x : std::initializer_list<const at::Tensor*>{&k, &lse, &cu})
+    if (x->defined()) TORCH_CHECK_VALUE(x->device() == q.device() && x->layout() == at::kStrided, what, ": all tensors must be on one device");
+  const int dev = q.get_device();
+  if (!ready(dev)) Py_RETURN_FALSE;
+  at::Tensor out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::cuda::CUDAGuard guard(q.device());
+    out = at::empty(t == 0 ? at::IntArrayRef({hkv, len}) : at::IntArrayRef({batch, hkv, len}), lse.options());
+    if (out.numel() > 0) {
+      q = loadable(q, true), k = loadable(k, true);
+      if (lse.stride(-1) != 1) lse = lse.contiguous();
+      rswa_weight_sums_params_t p;
+      std::memset(&p, 0, sizeof(p));
+      p.dtype = dtype_code(q);
+      p.batch = static_cast<int32_t>(batch), p.len = static_cast<int32_t>(len), p.n_q_heads = static_cast<int32_t>(hq), p.n_kv_heads = static_cast<int32_t>(hkv);
+      p.head_dim = static_cast<int32_t>(q.size(-1));
+      p.window = static_cast<int32_t>(std::min(window, kIntMax)), p.n_sink = static_cast<int32_t>(std::min(n_sink, kIntMax));
+      p.softmax_scale = static_cast<float>(scale);
+      p.cu_seqlens = cu.defined() ? cu.const_data_ptr<int32_t>() : nullptr;
+      p.n_seqs = cu.defined() ? static_cast<int32_t>(cu.size(0) - 1) : 0;
+      // (strides of dimensions of size 1 mean nothing: any that the tensor maps take)
+      const auto stride = [](const at::Tensor& x, int64_t dim) { return x.size(dim) <= 1 ? x.size(-1) * x.size(-2) : x.stride(dim); };
+      p.q = q.const_data_ptr(), p.k = k.const_data_ptr();
+      p.q_stride_b = t == 0 ? 0 : stride(q, 0), p.q_stride_t = stride(q, t), p.q_stride_h = stride(q, t + 1);
+      p.k_stride_b = t == 0 ? 0 : stride(k, 0), p.k_stride_t = stride(k, t), p.k_stride_h = stride(k, t + 1);
+      p.lse = lse.const_data_ptr<float>();
+      p.lse_stride_b = t == 0 ? 0 : stride_of(lse, 0), p.lse_stride_h = stride_of(lse, t);
+      p.out = out.data_ptr<float>();
+      p.status = status_word(dev);
+      const int64_t bytes = rswa_weight_sums_workspace_bytes(&p);
+      if (bytes < 0) check(static_cast<int>(bytes), what);
+      const at::Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+      p.workspace = ws.data_ptr();
+      p.workspace_bytes = bytes;
+      check(rswa_weight_sums(&p, stream_of(dev)), what);
+    }
+  }
+  return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }
 

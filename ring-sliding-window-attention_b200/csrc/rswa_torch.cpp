@@ -315,6 +315,11 @@ PyMethodDef g_methods[] = {
     {"cache_attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rswa_host::py_cache_attn)), METH_FASTCALL,
      "cache_attn(k_cache, v_cache, k_scale, v_scale, q, block_table, lens, window, n_sink, scale, weights, want_lse) -> out or (out, lse), "
      "or False"},
+    {"cache_evict", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rswa_host::py_cache_evict)), METH_FASTCALL,
+     "cache_evict(k_cache, v_cache, k_scale, v_scale, block_table, lens, weights, budget, new_block_table, n_sink, n_recent) -> (new_lens, "
+     "new_weights, kept), or False"},
+    {"weight_sums", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rswa_host::py_weight_sums)), METH_FASTCALL,
+     "weight_sums(q, k, lse, window, n_sink, scale, cu_seqlens) -> sums, or False"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", "Single-GPU host path of ring_swa", -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -18,5 +18,7 @@ void check(int rc, const char* what);
 PyObject* py_cache_append(PyObject*, PyObject* const* args, Py_ssize_t n);
 PyObject* py_cache_read(PyObject*, PyObject* const* args, Py_ssize_t n);
 PyObject* py_cache_attn(PyObject*, PyObject* const* args, Py_ssize_t n);
+PyObject* py_cache_evict(PyObject*, PyObject* const* args, Py_ssize_t n);
+PyObject* py_weight_sums(PyObject*, PyObject* const* args, Py_ssize_t n);
 
 }  // namespace rswa_host

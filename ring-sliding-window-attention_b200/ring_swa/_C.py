@@ -129,6 +129,29 @@ class CacheAttnParams(C.Structure):
     ]
 
 
+class WeightSumsParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("batch", C.c_int32), ("len", C.c_int32), ("n_q_heads", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("window", C.c_int32), ("n_sink", C.c_int32), ("softmax_scale", C.c_float), ("n_seqs", C.c_int32),
+        ("cu_seqlens", C.c_void_p),
+        ("q", C.c_void_p), ("q_stride_b", C.c_int64), ("q_stride_t", C.c_int64), ("q_stride_h", C.c_int64),
+        ("k", C.c_void_p), ("k_stride_b", C.c_int64), ("k_stride_t", C.c_int64), ("k_stride_h", C.c_int64),
+        ("lse", C.c_void_p), ("lse_stride_b", C.c_int64), ("lse_stride_h", C.c_int64),
+        ("out", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("status", C.c_void_p),
+    ]
+
+
+class CacheEvictParams(C.Structure):
+    _fields_ = [
+        ("cache", Cache), ("table", BlockTable), ("lens", C.c_void_p),
+        ("weights", C.c_void_p), ("w_stride_b", C.c_int64), ("w_stride_h", C.c_int64),
+        ("budget", C.c_int32), ("n_sink", C.c_int32), ("n_recent", C.c_int32), ("new_w_len", C.c_int32),
+        ("new_table", BlockTable), ("new_lens", C.c_void_p), ("new_weights", C.c_void_p), ("kept", C.c_void_p),
+        ("status", C.c_void_p),
+    ]
+
+
 # every symbol include/rswa.h declares, with its signature
 SYMBOLS = {
     "rswa_launch_count": (C.c_int64, []),
@@ -164,6 +187,9 @@ SYMBOLS = {
     "rswa_cache_read": (C.c_int, [C.POINTER(CacheReadParams), C.c_void_p]),
     "rswa_cache_attn_workspace_bytes": (C.c_int64, [C.POINTER(CacheAttnParams)]),
     "rswa_cache_attn": (C.c_int, [C.POINTER(CacheAttnParams), C.c_void_p]),
+    "rswa_weight_sums_workspace_bytes": (C.c_int64, [C.POINTER(WeightSumsParams)]),
+    "rswa_weight_sums": (C.c_int, [C.POINTER(WeightSumsParams), C.c_void_p]),
+    "rswa_cache_evict": (C.c_int, [C.POINTER(CacheEvictParams), C.c_void_p]),
     "rswa_selftest_mma": (C.c_int, [C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
 }
 

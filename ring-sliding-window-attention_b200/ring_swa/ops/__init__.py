@@ -27,6 +27,8 @@ from .kv_cache import (
     cache_append,
     cache_read,
     cache_attn,
+    cache_evict,
+    attn_weight_sums,
 )
 
 __all__ = [
@@ -48,4 +50,6 @@ __all__ = [
     "cache_append",
     "cache_read",
     "cache_attn",
+    "cache_evict",
+    "attn_weight_sums",
 ]

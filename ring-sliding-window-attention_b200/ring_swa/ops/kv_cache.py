@@ -12,6 +12,12 @@ scale per head (KVCache), addressed through a block table as serving programs ke
     lens += 1
     out = cache_attn(q, cache, block_table, lens, window_size=4096, num_sink_tokens=4)
 
+and, for a cache that is kept to a number of tokens by what the model has attended to:
+
+    weights[b, :, :n] = attn_weight_sums(q, k, softmax_lse, window)    # of a prompt
+    out = cache_attn(q, cache, block_table, lens, weights=weights)     # every step adds its own
+    lens, weights, kept = cache_evict(cache, block_table, lens, weights, budget, new_block_table, 4, 512)
+
 block_table [batch, max_blocks] and lens [batch] are int32 tensors of the caller's on the cache's device: slot t of
 sequence b is token t % block_size of block block_table[b, t // block_size].  Nothing here changes lens, copies it to the
 host or waits for the device, so that a step can be captured into a CUDA graph and replayed with other lengths.  Positions
@@ -32,17 +38,21 @@ from .. import _kernels as K
 _native = None
 
 
-def _call(name: str, cache: "KVCache", *args):
+def _call(name: str, device: torch.device, *args):
     global _native
     if _native is None:
         _native = K.native_module()
     fn = getattr(_native, name)
-    result = fn(cache.k, cache.v, cache.k_scale, cache.v_scale, *args)
+    result = fn(*args)
     if result is False:  # no status word yet, or an error of an earlier call to raise
-        K.status_word(cache.k.device)
-        K.raise_if_reported(cache.k.device)
-        result = fn(cache.k, cache.v, cache.k_scale, cache.v_scale, *args)
+        K.status_word(device)
+        K.raise_if_reported(device)
+        result = fn(*args)
     return result
+
+
+def _call_cache(name: str, cache: "KVCache", *args):
+    return _call(name, cache.k.device, cache.k, cache.v, cache.k_scale, cache.v_scale, *args)
 
 
 class KVCache:
@@ -91,7 +101,7 @@ def cache_append(cache: KVCache, k: torch.Tensor, v: torch.Tensor, block_table: 
     NaN.  The blocks written to must belong to one sequence each; blocks that are only read (a shared prefix that ends
     with a full block) may be shared.
     """
-    _call("cache_append", cache, k, v, block_table, lens, cu_seqlens)
+    _call_cache("cache_append", cache, k, v, block_table, lens, cu_seqlens)
 
 
 def cache_read(cache: KVCache, block_table: torch.Tensor, lens: torch.Tensor, max_len: int,
@@ -100,7 +110,7 @@ def cache_read(cache: KVCache, block_table: torch.Tensor, lens: torch.Tensor, ma
     continues a cached prefix: k, v [batch, max_len, num_kv_heads, head_dim], zero behind a sequence's end."""
     if dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"cache_read: dtype must be torch.bfloat16 or torch.float16, got {dtype}")
-    return _call("cache_read", cache, block_table, lens, max_len, dtype == torch.bfloat16)
+    return _call_cache("cache_read", cache, block_table, lens, max_len, dtype == torch.bfloat16)
 
 
 def cache_attn(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, lens: torch.Tensor,
@@ -120,4 +130,35 @@ def cache_attn(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, lens:
     every slot got from the queries and heads of its key/value head (what cache_evict goes by; start it with
     attn_weight_sums of the prompt, or zeros).
     """
-    return _call("cache_attn", cache, q, block_table, lens, window_size, num_sink_tokens, softmax_scale, weights, return_lse)
+    return _call_cache("cache_attn", cache, q, block_table, lens, window_size, num_sink_tokens, softmax_scale, weights, return_lse)
+
+
+def attn_weight_sums(q: torch.Tensor, k: torch.Tensor, softmax_lse: torch.Tensor, window_size: Optional[int] = None,
+                     num_sink_tokens: int = 0, softmax_scale: Optional[float] = None,
+                     cu_seqlens: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The softmax weight that every key of a prompt got, summed over the queries that see it and the query heads of
+    its key/value head: float32 [batch, num_kv_heads, tokens], packed [num_kv_heads, tokens].
+
+    q [batch, tokens, num_q_heads, head_dim], k [batch, tokens, num_kv_heads, head_dim], bf16 or fp16, head_dim 64 or 128;
+    packed [tokens, heads, head_dim] with cu_seqlens (int32, on the device).  The mask is that of cache_attn (and of
+    ring_streaming_llm_attn on one GPU); softmax_lse [batch, num_q_heads, tokens] (packed [num_q_heads, tokens]) float32 is
+    the log-sum-exp of the same attention, as wrapped_flash_attn_fwd and torch.ops.ring_swa.swa_fwd return it.
+    """
+    return _call("weight_sums", q.device, q, k, softmax_lse, window_size, num_sink_tokens, softmax_scale, cu_seqlens)
+
+
+def cache_evict(cache: KVCache, block_table: torch.Tensor, lens: torch.Tensor, weights: torch.Tensor, budget: int,
+                new_block_table: torch.Tensor, num_sink_tokens: int = 0, num_recent_tokens: int = 0
+                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Cuts every sequence to at most `budget` tokens: its first num_sink_tokens, its last num_recent_tokens, and those in
+    between with the largest weights, chosen for each key/value head (equal weights: the earlier token; NaN counts as the
+    largest).  The tokens keep their order.
+
+    weights float32 [batch, num_kv_heads, at least max_blocks * block_size], as cache_attn adds them up.  The kept keys and
+    values go to the blocks named by new_block_table ([batch, blocks for min(budget, tokens of block_table)], int32), which
+    must be other blocks than those of block_table and belong to one sequence each; the old ones are only read, so that a
+    prefix may be shared, and are free afterwards.  A sequence within the budget is moved as it is.
+    Returns (new_lens [batch] int32, new_weights [batch, num_kv_heads, tokens of new_block_table], kept [batch,
+    num_kv_heads, budget] int32: the old slots of the kept tokens, -1 behind them).
+    """
+    return _call_cache("cache_evict", cache, block_table, lens, weights, budget, new_block_table, num_sink_tokens, num_recent_tokens)

@@ -95,3 +95,51 @@ def attn(cache, table, lens, q, window, sink, scale=None):
             size[i, j] = torch.einsum("hgt,thd->hgd", pr, v[seen].abs()).reshape(hq, d)
             w[i][:, :lens[i]][:, seen] += pr.sum(1)
     return out, lse, w, size, most
+
+
+def weight_sums(q, k, lse, window, sink, scale, lens):
+    """Packed: q [t, hq, d], k [t, hkv, d], lse [hq, t].  Returns sums [hkv, t], the largest sum of |q||k| * scale, the number of terms [t]."""
+    t, hq, d = q.shape
+    hkv = k.shape[1]
+    grp = hq // hkv
+    scale = d ** -0.5 if scale is None else scale
+    out, terms, most, at = torch.zeros(hkv, t, dtype=torch.float64), torch.zeros(t), 0.0, 0
+    for n in lens:
+        seq = slice(at, at + n)
+        i, j = torch.arange(n)[:, None], torch.arange(n)[None]
+        seen = j <= i if window is None else (j <= i) & ((i - j <= window) | (j < sink))
+        terms[seq] = seen.sum(0).float() * grp
+        for h in range(hq):
+            s = q[seq, h] @ k[seq, h // grp].T * scale
+            most = max(most, (q[seq, h].abs() @ k[seq, h // grp].abs().T * scale).nan_to_num(0).max().item() if n else 0.0)
+            w = (s - lse[h, seq].double()[:, None]).exp()
+            w = torch.where(torch.isneginf(lse[h, seq])[:, None], torch.zeros_like(w), w)
+            out[h // grp, seq] += torch.where(seen, w, torch.zeros_like(w)).sum(0)
+        at += n
+    return out, most, terms
+
+
+def keep(w, n, budget, sink, recent):
+    """The slots of one sequence and head that stay, in order: by sorting."""
+    if n <= budget:
+        return list(range(n))
+    key = lambda t: -math.inf if math.isnan(w[t]) else -w[t]  # noqa: E731
+    nan_first = sorted(range(sink, n - recent), key=lambda t: (not math.isnan(w[t]), key(t), t))
+    return sorted([*range(sink), *nan_first[:budget - sink - recent], *range(n - recent, n)])
+
+
+def evict(cache, kind, table, lens, weights, budget, new_table, sink, recent):
+    """Changes the cache in place; returns new_lens, new weights as lists, kept as lists."""
+    bs = cache["k"].shape[2]
+    kept = [[keep(weights[b, h].tolist(), n, budget, sink, recent) for h in range(weights.shape[1])] for b, n in enumerate(lens)]
+    for name in ("k", "v"):
+        for b, n in enumerate(lens):
+            x = rows(cache, name, table[b], n)
+            for h, slots in enumerate(kept[b]):
+                for at in range(0, len(slots), bs):
+                    y = x[slots[at:at + bs], h]
+                    page = int(new_table[b][at // bs])
+                    s = scale_for(y.abs().max().item() if not torch.isnan(y).any() else math.nan, kind)
+                    cache[name][page, h, :y.shape[0]] = to_stored(y / s, kind)
+                    cache[name + "_scale"][page, h] = s
+    return [min(n, budget) for n in lens], kept

@@ -79,6 +79,38 @@ def test_read_refuses():
         ops.cache_read(cpu_cache(), TABLE, LENS, 1.5)
 
 
+W = torch.zeros(3, 2, 32)
+
+
+@pytest.mark.parametrize("change", [
+    dict(budget=0), dict(budget=-3), dict(num_sink_tokens=-1), dict(num_recent_tokens=-1), dict(budget=8, num_sink_tokens=4, num_recent_tokens=5),
+    dict(budget=1 << 40), dict(weights=W[:, :, :31]), dict(weights=W.double()), dict(weights=W[:2]), dict(weights=W[:1].expand(3, 2, 32)),
+    dict(new_block_table=TABLE[:2]), dict(new_block_table=TABLE.long()), dict(budget=17, new_block_table=TABLE[:, :1].contiguous()),
+    dict(block_table=TABLE[0]), dict(lens=LENS.long()),
+])
+def test_evict_refuses(change):
+    args = dict(cache=cpu_cache(), block_table=TABLE, lens=LENS, weights=W, budget=16, new_block_table=TABLE)
+    args.update(change)
+    with pytest.raises(ValueError):
+        ops.cache_evict(**args)
+
+
+SQ, SK, SL = torch.zeros(2, 10, 4, 64, dtype=torch.bfloat16), torch.zeros(2, 10, 2, 64, dtype=torch.bfloat16), torch.zeros(2, 4, 10)
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=SQ.float()), dict(k=SK.half()), dict(q=SQ[0], k=SK[0], softmax_lse=SL[0]), dict(k=SK[:, :9]), dict(k=SK[:1]), dict(q=SQ[:, :, :3]),
+    dict(q=SQ[..., :32], k=SK[..., :32]), dict(softmax_lse=SL[:, :3]), dict(softmax_lse=SL[..., :9]), dict(softmax_lse=SL.double()), dict(softmax_lse=SL[:1]),
+    dict(window_size=-1), dict(num_sink_tokens=-1), dict(softmax_scale=0.0), dict(cu_seqlens=torch.tensor([0, 10], dtype=torch.int32)),
+    dict(q=SQ[0], k=SK[0], softmax_lse=SL[0], cu_seqlens=torch.tensor([0, 10])), dict(q=SQ[0], k=SK[0], softmax_lse=SL[0], cu_seqlens=torch.tensor([0], dtype=torch.int32)),
+])
+def test_weight_sums_refuse(change):
+    args = dict(q=SQ, k=SK, softmax_lse=SL, window_size=4)
+    args.update(change)
+    with pytest.raises(ValueError):
+        ops.attn_weight_sums(**args)
+
+
 def test_no_cpu_path_no_gradient_no_other_tensors():
     with pytest.raises(RuntimeError, match="no CPU path"):
         ops.cache_attn(Q, cpu_cache(), TABLE, LENS)
@@ -88,6 +120,12 @@ def test_no_cpu_path_no_gradient_no_other_tensors():
         ops.cache_attn(Q.clone().requires_grad_(True), cpu_cache(), TABLE, LENS)
     with pytest.raises(RuntimeError, match="gradient"):
         ops.cache_append(cpu_cache(), KV, KV.clone().requires_grad_(True), TABLE, LENS)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.cache_evict(cpu_cache(), TABLE, LENS, W, 16, TABLE)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.attn_weight_sums(SQ, SK, SL, 4)
+    with pytest.raises(RuntimeError, match="gradient"):
+        ops.attn_weight_sums(SQ, SK.clone().requires_grad_(True), SL, 4)
     with pytest.raises(TypeError):
         ops.cache_attn(Q.float().numpy(), cpu_cache(), TABLE, LENS)
 
@@ -103,8 +141,10 @@ def test_no_cpu_path_no_gradient_no_other_tensors():
 def test_the_c_entries_refuse():
     from ring_swa import _C
     lib = _C.lib()
-    for name in ("append", "read", "attn"):
-        assert getattr(lib, f"rswa_cache_{name}")(None, None) == -1
+    for name in ("cache_append", "cache_read", "cache_attn", "cache_evict", "weight_sums"):
+        assert getattr(lib, "rswa_" + name)(None, None) == -1
+    for name in ("cache_attn", "weight_sums"):
+        assert getattr(lib, f"rswa_{name}_workspace_bytes")(None) == -1
     p = _C.CacheAttnParams()
     p.cache.head_dim, p.cache.block_size, p.cache.n_kv_heads = 128, 64, 8
     p.table.batch, p.table.max_blocks, p.q_len, p.n_q_heads, p.window = 32, 128, 1, 32, -1
@@ -127,7 +167,8 @@ def test_struct_sizes_match_the_header():
     import tempfile
     from ring_swa import _C
     names = [("rswa_cache_t", _C.Cache), ("rswa_block_table_t", _C.BlockTable), ("rswa_cache_append_params_t", _C.CacheAppendParams),
-             ("rswa_cache_read_params_t", _C.CacheReadParams), ("rswa_cache_attn_params_t", _C.CacheAttnParams)]
+             ("rswa_cache_read_params_t", _C.CacheReadParams), ("rswa_cache_attn_params_t", _C.CacheAttnParams),
+             ("rswa_weight_sums_params_t", _C.WeightSumsParams), ("rswa_cache_evict_params_t", _C.CacheEvictParams)]
     src = '#include <stdio.h>\n#include "rswa.h"\nint main(void) {\n' + "".join(f'  printf("%zu\\n", sizeof({n}));\n' for n, _ in names) + "  return 0;\n}\n"
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     with tempfile.TemporaryDirectory() as tmp:

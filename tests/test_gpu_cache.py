@@ -9,6 +9,10 @@ each (2^-25 of the largest for the smallest ones): 2^-11 * sum p|v|; (c) an erro
 factor within e^(+-e) before and after the division by their sum: 2 e * sum p|v|, where a 32-bit sum of d products
 is off by at most (d + 8) * 2^-24 * sum|q||k| * scale; (d) 32-bit exponentials, sums and scalings, 2^-18 in all.
 The log-sum-exp is off by e, and by the sums' and the logarithm's rounding, 2^-20 relative to 1 and to itself.
+
+Sums of weights: each term is off by the factor of (c), by the rounding of s * scale * log2(e) - lse * log2(e), half a step
+of its larger part (2^-24 * (|s| + |lse|) * log2(e), taken with the largest |lse|, times ln 2), and by the exponential's
+2^-20; the 128 terms of a tile are added in 32 bits (at most 128 * 2^-24), the tiles with compensation (2^-23).
 """
 import math
 import random
@@ -339,3 +343,229 @@ def test_a_captured_step_is_replayed_with_other_lengths_and_on_another_stream():
             assert torch.equal(r["lens"], at + 1)
             for name in ("k", "v"):
                 assert torch.equal(getattr(r["cache"], name).view(torch.uint8), getattr(r["eager"], name).view(torch.uint8))
+
+
+SUMS = [
+    # lens, (hq, hkv), d, window, sink, packed
+    ([1], (1, 1), 64, 0, 0, False),
+    ([5], (4, 2), 128, None, 0, True),
+    ([128], (4, 4), 64, 128, 0, False),
+    ([129], (2, 1), 128, 0, 0, False),
+    ([300], (8, 2), 128, 100, 0, False),
+    ([777], (4, 4), 64, 1 << 30, 1 << 30, False),
+    ([1000], (6, 2), 128, 129, 1, True),
+    ([1, 255, 1, 256, 2, 500, 3], (4, 2), 64, 64, 4, True),
+    ([700, 30, 900], (4, 1), 128, 250, 2, True),
+    ([1, 1, 1, 1, 40, 128, 128], (2, 2), 64, 20, 0, True),
+    ([2100], (16, 2), 128, 500, 300, False),
+    ([513] * 3, (4, 4), 128, 33, 1, False),   # a batch
+    ([260] * 2, (2, 1), 64, None, 0, False),
+]
+
+
+@pytest.mark.parametrize("case", range(len(SUMS)))
+def test_weight_sums(case):
+    ops = _ops()
+    lens, (hq, hkv), d, window, sink, packed = SUMS[case]
+    dt = "fp16" if case % 2 else "bf16"
+    t = sum(lens)
+    qk = normal(t, hq + hkv, d, seed=case, dt=dt)
+    q, k = qk[:, :hq], qk[:, hq:]
+    scale = None if case % 3 else 0.2
+    # the log-sum-exp of the attention itself
+    cu = [0] + torch.tensor(lens).cumsum(0).tolist()
+    lse = torch.full((hq, t), -math.inf, dtype=torch.float64)
+    for a, z in zip(cu, cu[1:]):
+        i, j = torch.arange(z - a)[:, None], torch.arange(z - a)[None]
+        seen = j <= i if window is None else (j <= i) & ((i - j <= window) | (j < sink))
+        for h in range(hq):
+            s = q[a:z, h].double() @ k[a:z, h // (hq // hkv)].double().T * (d ** -0.5 if scale is None else scale)
+            lse[h, a:z] = s.masked_fill(~seen, -math.inf).logsumexp(1)
+    lse = lse.float()
+    if case == 8:
+        lse[1, 3], lse[0, 900] = -math.inf, -math.inf   # queries that are said to have seen nothing
+    want, most, terms = R.weight_sums(q.double(), k.double(), lse, window, sink, scale, lens)
+    if packed:
+        got = ops.attn_weight_sums(q.cuda(), k.cuda(), lse.cuda(), window, sink, softmax_scale=scale, cu_seqlens=torch.tensor(cu, dtype=torch.int32).cuda())
+    else:
+        b = len(lens)
+        qb, kb = (x.contiguous().cuda().view(b, t // b, -1, d) for x in (q, k))
+        got = ops.attn_weight_sums(qb, kb, lse.view(hq, b, t // b).transpose(0, 1).cuda(), window, sink, softmax_scale=scale)
+        got = got.transpose(0, 1).reshape(hkv, t)
+    e = (d + 8) * 2.0 ** -24 * most
+    big = lse[torch.isfinite(lse)].abs().max().item()
+    rel = e + 2.0 ** -24 * (most + big) + 2.0 ** -20 + 128 * 2.0 ** -24 + 2.0 ** -23
+    err = (got.cpu().double() - want).abs()
+    assert (err <= rel * want + 1e-30).all(), f"{(err / (rel * want + 1e-30)).max().item():.3g} of the tolerance"
+    if case != 8:  # (every query's weights add up to one; the log-sum-exps' own rounding is 2^-24 * |lse|)
+        assert abs(want.sum().item() / (t * hq) - 1) < 2.0 ** -23 * (1 + big)
+
+
+def test_weight_sums_of_the_forward_kernels_and_run_to_run():
+    """With the log-sum-exp that the attention operator returns; the same bits every time."""
+    import ring_swa.compiled  # noqa: F401  (registers the operator)
+    ops = _ops()
+    b, s, hq, hkv, d, window, sink = 2, 3000, 8, 2, 128, 700, 4
+    q, k, v = (normal(b, s, h, d, seed=i, dt="bf16").cuda() for i, h in enumerate((hq, hkv, hkv)))
+    _, lse = torch.ops.ring_swa.swa_fwd(q, k, v, window, sink, d ** -0.5, None)
+    got = ops.attn_weight_sums(q, k, lse, window, sink)
+    assert abs(got.double().sum().item() / (b * s * hq) - 1) < 2e-3  # (16-bit weights in the forward kernel's sum)
+    for i in range(b):
+        want, _, _ = R.weight_sums(q[i].cpu().double(), k[i].cpu().double(), lse[i].cpu(), window, sink, None, [s])
+        assert ((got[i].cpu().double() - want).abs() <= 1e-4 * want).all()
+    assert torch.equal(got, ops.attn_weight_sums(q, k, lse, window, sink))
+
+
+EVICT = [
+    # lens, heads, d, bs, budget, sink, recent
+    ([100], 1, 64, 16, 40, 0, 0),
+    ([1500, 40, 1], 2, 64, 16, 512, 4, 128),
+    ([300, 513, 64, 0], 3, 128, 64, 200, 1, 50),
+    ([2000, 1999], 2, 128, 128, 1000, 0, 1000),      # the newest alone
+    ([700], 4, 64, 32, 4, 4, 0),                      # the sinks alone
+    ([700], 2, 128, 16, 699, 2, 3),
+    ([100, 90], 2, 64, 32, 500, 4, 100),              # nothing to do
+    ([5000, 33], 1, 64, 16, 1, 0, 0),
+    ([70000], 1, 64, 128, 20000, 4, 1000),
+]
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("case", range(len(EVICT)))
+def test_evict(case, kind):
+    ops = _ops()
+    lens, heads, d, bs, budget, sink, recent = EVICT[case]
+    cap = max(1, max((n + bs - 1) // bs for n in lens))
+    new_cap = (min(budget, cap * bs) + bs - 1) // bs
+    total = sum((n + bs - 1) // bs for n in lens)
+    new_total = sum((min(n, budget) + bs - 1) // bs for n in lens)
+    cache, table, _, _, _ = filled(kind, "bf16", lens, heads, bs, d, seed=case, v_spread=True, spare=new_total + 2)
+    table = table[:, :cap]
+    free = sorted(set(range(total + new_total + 2)) - set(table.flatten().tolist()))
+    random.Random(case).shuffle(free)
+    new_table = torch.full((len(lens), new_cap), -1, dtype=torch.int32)
+    for i, n in enumerate(lens):
+        for j in range((min(n, budget) + bs - 1) // bs):
+            new_table[i, j] = free.pop()
+    g = torch.Generator().manual_seed(case)
+    w = (torch.randn(len(lens), heads, cap * bs + 3, generator=g) * 2).exp()
+    # all kinds of ties: a few values for most, zeros of both signs, infinities, NaN, negative ones
+    w = torch.where(torch.rand(w.shape, generator=g) < 0.7, w.round().clamp(0, 3), w)
+    w = torch.where(torch.rand(w.shape, generator=g) < 0.05, -w, w)
+    if case % 2:
+        w[..., 7::97], w[..., 11::131] = math.nan, math.inf
+    ref = host(cache)
+    want_lens, want_kept = R.evict(ref, kind, table, lens, w, budget, new_table, sink, recent)
+    dev = torch.tensor(lens, dtype=torch.int32).cuda()
+    new_lens, new_w, kept = ops.cache_evict(cache, table.cuda(), dev, w.cuda(), budget, new_table.cuda(), sink, recent)
+    assert new_lens.tolist() == want_lens and new_lens.dtype == torch.int32
+    assert new_w.shape == (len(lens), heads, new_cap * bs) and kept.shape == (len(lens), heads, budget)
+    for b in range(len(lens)):
+        for h in range(heads):
+            slots = want_kept[b][h]
+            assert kept[b, h].tolist() == slots + [-1] * (budget - len(slots))
+            want = torch.zeros(new_cap * bs)
+            want[:len(slots)] = w[b, h][slots]
+            torch.testing.assert_close(new_w[b, h].cpu(), want, rtol=0, atol=0, equal_nan=True)
+    got = host(cache)
+    for name in ("k", "v", "k_scale", "v_scale"):  # (the old blocks and the unused ones as they were)
+        torch.testing.assert_close(got[name], ref[name], rtol=0, atol=0, equal_nan=True)
+    # evicting again what is within the budget now: the same values, bit for bit
+    if case in (1, 2):
+        room = ops.KVCache(*(torch.cat([x, torch.zeros_like(x)]) for x in (cache.k, cache.v, cache.k_scale, cache.v_scale)))
+        third = torch.where(new_table >= 0, new_table + cache.k.shape[0], new_table)
+        args = (new_lens, new_cap * bs)
+        ops.cache_evict(room, new_table.cuda(), new_lens, new_w, budget, third.cuda())
+        for x, y in zip(ops.cache_read(room, new_table.cuda(), *args), ops.cache_read(room, third.cuda(), *args)):
+            assert torch.equal(x, y)
+
+
+def test_evict_keeps_poison_and_reports_bad_tables():
+    ops = _ops()
+    cache, table, _, _, _ = filled("int8", "bf16", [64], 2, 16, 64, seed=1, spare=4)
+    free = sorted(set(range(8)) - set(table.flatten().tolist()))
+    new_table = torch.tensor([free[:2]], dtype=torch.int32)
+    w = torch.arange(128.0).view(1, 2, 64) % 64
+    w = torch.nn.functional.pad(w, (0, table.shape[1] * 16 - 64))
+    cache.v_scale[table[0, 1].item(), 0] = math.nan     # slots 16..31
+    lens = torch.tensor([64], dtype=torch.int32).cuda()
+    w[0, 0, 16:18] = 100.0
+    _, _, kept = ops.cache_evict(cache, table.cuda(), lens, w.cuda(), 32, new_table.cuda())
+    assert kept[0, 0].tolist() == [16, 17, *range(34, 64)] and kept[0, 1].tolist() == list(range(32, 64))
+    k, v = ops.cache_read(cache, new_table.cuda(), torch.tensor([32], dtype=torch.int32).cuda(), 32)
+    assert torch.isnan(v[0, :16, 0]).all() and torch.isfinite(v[0, 16:, 0]).all() and torch.isfinite(v[0, :, 1]).all() and torch.isfinite(k).all()
+    before = host(cache)
+    for bad in (-1, 8, 1 << 30):
+        ops.cache_evict(cache, table.cuda(), lens, w.cuda(), 32, torch.tensor([[new_table[0, 0].item(), bad]], dtype=torch.int32).cuda())
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="code 110"):
+            ops.cache_read(cache, table.cuda(), lens, 1)
+    ops.cache_evict(cache, table.cuda(), lens - 100, w.cuda(), 32, new_table.cuda())
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="code 111"):
+        ops.cache_read(cache, table.cuda(), lens, 1)
+    after = host(cache)
+    for name in before:
+        torch.testing.assert_close(after[name], before[name], rtol=0, atol=0, equal_nan=True)
+
+
+def test_prompt_then_steps_then_eviction_then_steps():
+    """The operators together: a packed batch of prompts through StreamingLLM attention, its weights and its keys and values into
+    the cache, steps that add their weights, an eviction, further steps, and the cut prefix read back for a next turn."""
+    import ring_swa
+    import ring_swa.compiled  # noqa: F401
+    ops = _ops()
+    hq, hkv, d, bs, window, sink, budget = 8, 2, 128, 32, 400, 4, 256
+    lens, steps = [600, 90, 333], 6
+    t = sum(lens)
+    cu = torch.tensor([0, 600, 690, 1023], dtype=torch.int32)
+    q, k, v = (normal(t, h, d, seed=20 + i, dt="bf16") for i, h in enumerate((hq, hkv, hkv)))
+    dev = [x.cuda() for x in (q, k, v, cu)]
+    out = ring_swa.ring_streaming_llm_attn_varlen(*dev[:3], window, dev[3], cp_size=1, num_sink_tokens=sink)
+    out2, lse = torch.ops.ring_swa.swa_fwd(dev[0][None], dev[1][None], dev[2][None], window, sink, d ** -0.5, dev[3])
+    assert torch.equal(out, out2[0])
+    cap = (max(lens) + 2 * steps + bs - 1) // bs
+    table = tables([n + 2 * steps for n in lens], bs, cap, 60, seed=2)
+    cache = make("int8", 60 + 30, hkv, bs, d, seed=3)
+    lens_dev = torch.zeros(3, dtype=torch.int32, device="cuda")
+    w = torch.zeros(3, hkv, cap * bs, device="cuda")
+    ops.cache_append(cache, dev[1], dev[2], table.cuda(), lens_dev, cu_seqlens=dev[3])
+    sums = ops.attn_weight_sums(dev[0], dev[1], lse[0], window, sink, cu_seqlens=dev[3])
+    for i in range(3):
+        w[i, :, :lens[i]] = sums[:, cu[i]:cu[i + 1]]
+    lens_dev += dev[3][1:] - dev[3][:-1]
+    ref, ref_w, ref_lens = host(cache), w.cpu().double(), list(lens)
+    kind = "int8"
+
+    def step(n, table, seed, cap):
+        nonlocal ref_w
+        x = [normal(3, 1, h, d, seed=seed + i, dt="bf16") for i, h in enumerate((hq, hkv, hkv))]
+        ops.cache_append(cache, x[1].cuda(), x[2].cuda(), table.cuda(), lens_dev)
+        lens_dev.add_(1)
+        R.append(ref, kind, table.tolist(), ref_lens, [y.double() for y in x[1]], [y.double() for y in x[2]], [1, 1, 1])
+        for i in range(3):
+            ref_lens[i] += 1
+        got = ops.cache_attn(x[0].cuda(), cache, table.cuda(), lens_dev, window_size=window, num_sink_tokens=sink, weights=w)
+        want, _, dw, size, most = R.attn(ref, table, ref_lens, x[0].double(), window, sink)
+        ref_w[..., :dw.shape[-1]] += dw
+        e = (d + 8) * 2.0 ** -24 * most
+        assert ((got.cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 1.01 * (2.0 ** -11 + 2 * e + 2.0 ** -18) * size).all()
+
+    for n in range(steps):
+        step(n, table, 100 + 10 * n, cap)
+    new_cap = (budget + steps + bs - 1) // bs
+    new_table = torch.arange(60, 60 + 3 * new_cap, dtype=torch.int32).view(3, new_cap)
+    exact_w = w.cpu()
+    assert ((exact_w.double() - ref_w).abs() <= 2.0 ** -17 * ref_w).all()
+    ref_lens, kept = R.evict(ref, kind, table, ref_lens, exact_w, budget, new_table, sink, 64)
+    new_lens, w, got_kept = ops.cache_evict(cache, table.cuda(), lens_dev, w, budget, new_table.cuda(), sink, 64)
+    assert [[x[:n].tolist() for x in y] for y, n in zip(got_kept, ref_lens)] == kept and new_lens.tolist() == ref_lens
+    lens_dev.copy_(new_lens)
+    ref_w = w.cpu().double()
+    for n in range(steps):
+        step(n, new_table, 500 + 10 * n, new_cap)
+    got = ops.cache_read(cache, new_table.cuda(), lens_dev, new_cap * bs)
+    for x, name in zip(got, ("k", "v")):
+        for i, n in enumerate(ref_lens):
+            assert torch.equal(x[i, :n].cpu(), R.rows(ref, name, new_table[i], n).bfloat16())
+            assert not x[i, n:].any()
