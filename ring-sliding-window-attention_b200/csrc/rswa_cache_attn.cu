@@ -23,9 +23,10 @@
 // the sum of the weights takes it back out.  Scores, sums and the output are 32-bit.
 //
 // Work: the 32-token tiles of all (sequence, key/value head, 8 or 16 query rows) in one order, cut evenly over the CTAs
-// (one per SM) whatever the lengths; the 8 warps of a CTA take its tiles in turn, each with a ring of tiles of its own
-// in flight that runs on over sequence boundaries, and add up at the end of each piece.  A piece that is not a whole
-// (sequence, head) goes to the workspace and a second kernel joins the pieces in order: results do not depend on timing.
+// (one per SM) whatever the lengths.  In a CTA one warp keeps a ring of tiles filled (its lanes look the blocks of 32
+// tiles up at a time: the table's latency is paid once for all of them), the others take the tiles in turn and add up at the
+// end of each piece; the ring runs on over sequence boundaries.  A piece that is not a whole (sequence, head) goes to the
+// workspace and a second kernel joins the pieces in order: results do not depend on timing.
 #include <atomic>
 
 #include "rswa_cache.cuh"
@@ -40,9 +41,9 @@ using namespace tc05;
 namespace {
 
 constexpr int kTok = 32;     // tokens of a tile
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
-constexpr int kMinShare = 8; // tiles of a CTA at least: one per warp
+constexpr int kScan = 256;   // threads of the prefix sums over sequences
+constexpr int kMinShare = 8; // tiles of a CTA at least
+constexpr int kJoin = 256;   // threads of the kernels behind the first one
 constexpr float kRoom = 14.f;  // a weight may grow to 2^14 before the reference is raised (fp16 ends at 2^16)
 constexpr float kLow = 4.f;    // and is raised to the maximum minus 4, so that not every new maximum raises it
 
@@ -63,7 +64,9 @@ struct AttnKernelParams {
   float* lse;        // or null
   float* part_o;     // [CTAs][2][8 * kNT][head_dim]
   float* part_ml;    // [CTAs][2][8 * kNT][2]
+  int4* cut;         // [CTAs]: an item whose first piece is the CTA's last one: sequence, head * row tiles + row tile, pieces (or 0)
   float* scores;     // [tiles][kTok][8 * kNT], or null: what the weights need
+  long long* first;  // [batch]: index of a sequence's first tile, with scores
   float* weights;
   long long w_sb, w_sh;
   int ctas;
@@ -97,28 +100,42 @@ __device__ __forceinline__ long long n_shares(long long total, int ctas) { retur
 __device__ __forceinline__ long long share_begin(long long total, long long shares, long long c) { return total * c / shares; }
 __device__ __forceinline__ long long share_of(long long total, long long shares, long long tile) { return ((tile + 1) * shares - 1) / total; }
 
-// Prefix sums of the sequences' tiles (per key/value head and row tile): thread i of kThreads holds `per` sequences.
-// s_prefix[i]: tiles in front of thread i's sequences; s_prefix[kThreads]: all.
+// Prefix sums of the sequences' tiles (per key/value head and row tile): thread i of the first kScan holds `per`
+// sequences.  s_prefix[i]: tiles in front of thread i's sequences; s_prefix[kScan]: all.
 __device__ __forceinline__ void tile_prefix(const AttnKernelParams& p, long long* s_prefix, long long* s_warp) {
-  const int per = (p.batch + kThreads - 1) / kThreads;
+  const int per = (p.batch + kScan - 1) / kScan;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long mine = 0;
-  for (int i = 0; i < per; ++i) {
-    const int b = threadIdx.x * per + i;
-    if (b < p.batch) mine += seq_tiles(p, b).n;
-  }
-  long long sum = mine;
+  long long mine = 0, sum = 0;
+  if (threadIdx.x < kScan) {
+    for (int i = 0; i < per; ++i) {
+      const int b = threadIdx.x * per + i;
+      if (b < p.batch) mine += seq_tiles(p, b).n;
+    }
+    sum = mine;
 #pragma unroll
-  for (int d = 1; d < 32; d *= 2) {
-    const long long o = __shfl_up_sync(0xffffffffu, sum, d);
-    if (lane >= d) sum += o;
+    for (int d = 1; d < 32; d *= 2) {
+      const long long o = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += o;
+    }
+    if (lane == 31) s_warp[warp] = sum;
   }
-  if (lane == 31) s_warp[warp] = sum;
   __syncthreads();
-  long long before = 0;
-  for (int w = 0; w < warp; ++w) before += s_warp[w];
-  s_prefix[threadIdx.x] = before + sum - mine;
-  if (threadIdx.x == kThreads - 1) s_prefix[kThreads] = before + sum;
+  if (threadIdx.x < kScan) {
+    long long before = 0;
+    for (int w = 0; w < warp; ++w) before += s_warp[w];
+    before += sum - mine;
+    s_prefix[threadIdx.x] = before;
+    if (threadIdx.x == kScan - 1) s_prefix[kScan] = before + mine;
+    if (p.first != nullptr && blockIdx.x == 0) {
+      const long long items = static_cast<long long>(p.c.hkv) * p.row_tiles;
+      for (int i = 0; i < per; ++i) {
+        const int b = threadIdx.x * per + i;
+        if (b >= p.batch) break;
+        p.first[b] = before * items;
+        before += seq_tiles(p, b).n;
+      }
+    }
+  }
   __syncthreads();
 }
 
@@ -145,8 +162,8 @@ struct Cursor {
 };
 __device__ __forceinline__ Cursor cursor_at(const AttnKernelParams& p, const long long* s_prefix, long long tile) {
   const long long items = static_cast<long long>(p.c.hkv) * p.row_tiles;
-  const int per = (p.batch + kThreads - 1) / kThreads;
-  int lo = 0, hi = kThreads - 1;  // the last thread whose prefix is not behind the tile
+  const int per = (p.batch + kScan - 1) / kScan;
+  int lo = 0, hi = kScan - 1;  // the last thread whose prefix is not behind the tile
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (s_prefix[mid] * items <= tile) lo = mid; else hi = mid - 1;
@@ -173,22 +190,26 @@ struct Ring {
   static constexpr int kStageBytes = 2 * kTileBytes;
 };
 
-template <int kNT, int kStages>
-struct Ctl {
-  uint64_t full[kWarps][kStages];
-  float scale[kWarps][kStages][4];  // K and V scale of the tile's first 16 tokens, and of its last 16
-  float ml[kWarps][8 * kNT][2];     // reference and sum of every warp's piece
-  int err;
-};
-
-// [rings][sums of the warps' pieces; at first the sequences' prefix sums][control]
+// kWarps that compute (with the loading one 16 warps of 128 registers a thread, or for 16 query rows 12 of 168),
+// kStages tiles in flight: 160 KB or more, where the latency of a load asks for about 50.
 template <int kD, int kNT>
 struct Layout {
-  static constexpr int kStages = kD == 128 ? 3 : 6;
-  static constexpr int kRings = kWarps * kStages * Ring<kD>::kStageBytes;
+  static constexpr int kWarps = kNT == 1 ? 15 : 11;
+  static constexpr int kThreads = (kWarps + 1) * 32;
+  static constexpr int kStages = (kNT == 1 ? 20 : 22) * (128 / kD);
+  struct Ctl {
+    uint64_t full[kStages], free[kStages];
+    float4 scale[kStages][2];           // of the tile's first 16 tokens and its last 16: K's scale, log2 of V's, 1 / V's
+    float ml[kWarps][8 * kNT][2];       // reference and sum of every warp's piece
+    int err;
+  };
+  static constexpr int kRings = kStages * Ring<kD>::kStageBytes;
   static constexpr int kMerge = kWarps * 8 * kD * 4;
-  static constexpr int kBytes = kRings + kMerge + static_cast<int>(sizeof(Ctl<kNT, kStages>));
+  // [ring][sums of the warps' pieces; at first the sequences' prefix sums][control]
+  static constexpr int kBytes = kRings + kMerge + static_cast<int>(sizeof(Ctl));
   static_assert(kBytes <= 232448, "shared memory budget");
+  static_assert(kMerge >= (kScan + 1 + kScan / 32) * 8, "the prefix sums lie where the pieces' sums come later");
+  static_assert(kStages >= kWarps, "a warp's next tile is at most one turn of the ring away");
 };
 
 __device__ __forceinline__ void tma_load_rows(void* dst, const CUtensorMap* m, uint64_t* bar, int row) {
@@ -219,78 +240,117 @@ __device__ __forceinline__ uint32_t piece(uint32_t base, int row, int chunk) {
   return base + row * kD + ((kD == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4);
 }
 
+template <int kWarps>
+__device__ __forceinline__ void sync_warps() {
+  asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
+}
+// four elements of a finished row, and its log-sum-exp
+template <int kD, bool kInt8>
+__device__ __forceinline__ void store_row(const AttnKernelParams& p, int b, int h, int row, int d4, float4 x, float top, float sum) {
+  const int i = row / p.group, hd = h * p.group + row - i * p.group;
+  const float inv = sum == 0.f ? 0.f : kHalfFactor<kInt8> / sum;
+  uint16_t* const to = p.out + ((static_cast<long long>(b) * p.q_len + i) * p.hq + hd) * kD + d4 * 4;
+  *reinterpret_cast<uint2*>(to) = p.bf16 ? make_uint2(pack2<true>(x.x * inv, x.y * inv), pack2<true>(x.z * inv, x.w * inv))
+                                         : make_uint2(pack2<false>(x.x * inv, x.y * inv), pack2<false>(x.z * inv, x.w * inv));
+  if (p.lse != nullptr && d4 == 0)
+    p.lse[(static_cast<long long>(b) * p.hq + hd) * p.q_len + i] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.6931471805599453f;
+}
+
 // kNT: query rows in columns of 8.
 template <int kD, int kNT, bool kInt8>
-__global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_constant__ AttnKernelParams p) {
+__global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_kernel(const __grid_constant__ AttnKernelParams p) {
   using L = Layout<kD, kNT>;
   using R = Ring<kD>;
-  constexpr int kS = L::kStages, kKS = kD / 16;
+  constexpr int kS = L::kStages, kKS = kD / 16, kWarps = L::kWarps;
   constexpr int kRows = 8 * kNT;
   extern __shared__ __align__(1024) uint8_t smem[];
-  auto& ctl = *reinterpret_cast<Ctl<kNT, kS>*>(smem + L::kRings + L::kMerge);
+  auto& ctl = *reinterpret_cast<typename L::Ctl*>(smem + L::kRings + L::kMerge);
   float* const merge = reinterpret_cast<float*>(smem + L::kRings);
   long long* const s_prefix = reinterpret_cast<long long*>(merge);
-  static_assert(L::kMerge >= (kThreads + 1 + kWarps) * 8, "the prefix sums lie where the pieces' sums come later");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  uint64_t* const full = ctl.full[warp];
-  uint8_t* const ring = smem + warp * kS * R::kStageBytes;
 
-  if (threadIdx.x == 0) ctl.err = 0;
-  if (lane == 0)
-    for (int i = 0; i < kS; ++i) mbar_init(full + i, 1 + 4);  // lane 0's announcement of the bytes, four lanes' scales
-  mbar_fence_init();
+  griddep_launch();
   if (threadIdx.x == 0) {
+    ctl.err = 0;
     prefetch_tmap(&p.map[0]);
     prefetch_tmap(&p.map[1]);
   }
+  if (threadIdx.x < kS) {
+    mbar_init(&ctl.full[threadIdx.x], 1);
+    mbar_init(&ctl.free[threadIdx.x], 1);
+  }
+  mbar_fence_init();
   griddep_wait();
-  tile_prefix(p, s_prefix, s_prefix + kThreads + 1);
-  const long long total = s_prefix[kThreads] * p.c.hkv * p.row_tiles;
+  tile_prefix(p, s_prefix, s_prefix + kScan + 1);
+  const long long total = s_prefix[kScan] * p.c.hkv * p.row_tiles;
   const long long shares = n_shares(total, p.ctas);
-  if (blockIdx.x >= shares || total == 0) return;
+  if (blockIdx.x >= shares || total == 0) {
+    if (threadIdx.x == 0) p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
+    return;
+  }
   const long long begin = share_begin(total, shares, blockIdx.x), end = share_begin(total, shares, blockIdx.x + 1);
-
-  // The loads of this warp's tiles run kS ahead of the arithmetic.
-  const int bs = p.c.bs, box = min(bs, kTok);
-  Cursor lc = cursor_at(p, s_prefix, begin);
-  Cursor cc = lc;  // the arithmetic's: first tile of the current piece
+  Cursor cc = cursor_at(p, s_prefix, begin);
   __syncthreads();  // (the prefix sums make room)
-  lc.skip(p, warp, end);
-  uint32_t pending = 0;  // stages with a load that has not been waited for
-  auto issue = [&](int st) {
-    if (lc.at >= end) return;
-    const int slot = tile_slot(lc.s, lc.i), h = lc.item / p.row_tiles;
-    // (a tile is part of one block, or two blocks of 16; the second may lie behind the sequence's end: not looked at)
-    int pg[2];
-    const int j = slot / bs;
-    pg[0] = table_entry(p.table, p.table_stride, lc.b, j, p.c.num_blocks, p.status, p.mirror);
-    pg[1] = pg[0];
-    if (bs < kTok) pg[1] = slot + bs < lc.s.len ? table_entry(p.table, p.table_stride, lc.b, j + 1, p.c.num_blocks, p.status, p.mirror) : pg[0];
-    // (reported; any block will do then)
-    pg[0] = max(pg[0], 0);
-    pg[1] = max(pg[1], 0);
-    pending |= 1u << st;
-    uint8_t* const dst = ring + st * R::kStageBytes;
-    if (lane == 0) {
-      mbar_expect_tx(full + st, R::kStageBytes);
-      const int off = slot % bs;
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv)
-        for (int half = 0; half < kTok / box; ++half)
-          tma_load_rows(dst + kv * R::kTileBytes + half * box * kD, &p.map[kv], full + st, (pg[half] * p.c.hkv + h) * bs + off);
-    }
-    if (lane < 4) {
-      const float* src = p.c.scale[lane & 1] + static_cast<long long>(pg[lane >> 1]) * p.c.hkv + h;
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(&ctl.scale[warp][st][lane])), "l"(src) : "memory");
-      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(full + st)) : "memory");
-    }
-    lc.skip(p, kWarps, end);
-  };
-#pragma unroll
-  for (int st = 0; st < kS; ++st) issue(st);
 
-  uint32_t phases = 0;
-  int st = 0;
+  if (warp == kWarps) {
+    // ---------------------------------------------------------------- loads: every lane looks up a tile of the next 32
+    const int bs = p.c.bs, box = min(bs, kTok);
+    Cursor lc = cc;
+    lc.skip(p, lane, end);
+    bool ok = true;
+    int at = 0;  // index of the tile within the share
+    int st = 0, round = 0;
+    const int n = static_cast<int>(end - begin);
+    while (at < n && ok) {
+      int row[2] = {0, 0};
+      float4 sc[2] = {make_float4(1.f, 0.f, 1.f, 0.f), make_float4(1.f, 0.f, 1.f, 0.f)};
+      if (lc.at < end) {
+        const int slot = tile_slot(lc.s, lc.i), h = lc.item / p.row_tiles, j = slot / bs;
+        // a tile is part of one block, or two blocks of 16; the second may lie behind the sequence's end: not looked at
+        int pg[2];
+        pg[0] = table_entry(p.table, p.table_stride, lc.b, j, p.c.num_blocks, p.status, p.mirror);
+        pg[1] = pg[0];
+        if (bs < kTok) pg[1] = slot + bs < lc.s.len ? table_entry(p.table, p.table_stride, lc.b, j + 1, p.c.num_blocks, p.status, p.mirror) : pg[0];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int page = max(pg[t], 0);  // (reported; any block will do then)
+          const long long ph = static_cast<long long>(page) * p.c.hkv + h;
+          row[t] = (page * p.c.hkv + h) * bs + slot % bs;
+          if (slot + 16 * t < lc.s.len) {  // (tokens behind the end: their block may not even have a scale)
+            const float sv = p.c.scale[1][ph];
+            sc[t] = make_float4(p.c.scale[0][ph], __log2f(sv), 1.f / sv, 0.f);
+          }
+        }
+      }
+      lc.skip(p, 32, end);
+      __syncwarp();
+#pragma unroll 1
+      for (int k = 0; k < 32 && at < n && ok; ++k, ++at) {
+        if (round > 0) ok = mbar_wait_w<20>(&ctl.free[st], (round - 1) & 1, &ctl.err, kErrWaitProducer);
+        if (ok && lane == k) {
+          ctl.scale[st][0] = sc[0];
+          ctl.scale[st][1] = sc[1];
+          mbar_expect_tx(&ctl.full[st], R::kStageBytes);
+          uint8_t* const dst = smem + st * R::kStageBytes;
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            tma_load_rows(dst + kv * R::kTileBytes, &p.map[kv], &ctl.full[st], row[0]);
+            if (box < kTok) tma_load_rows(dst + kv * R::kTileBytes + box * kD, &p.map[kv], &ctl.full[st], row[1]);
+          }
+        }
+        if (++st == kS) st = 0, ++round;
+      }
+    }
+    if (!ok) {
+      // the copies still on their way must not outlive the CTA's shared memory; each wait is limited
+      int own_err = 0;
+      for (int i = max(0, at - 1 - kS); i < at - 1; ++i) mbar_wait(&ctl.full[i % kS], (i / kS) & 1, &own_err, kErrWaitProducer);
+      if (lane == 0) raise_status(p.status, p.mirror, kErrWaitProducer);
+    }
+    return;
+  }
+
+  int st = warp, phase = 0;  // of this warp's next tile
   bool dead = false;
   while (cc.at < end) {
     const long long piece_end = min(end, cc.at + cc.s.n - cc.i);
@@ -368,24 +428,11 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
     // this warp's tiles of the piece: those whose index from `begin` is `warp` modulo kWarps
     const int lag = static_cast<int>((cc.at - begin) % kWarps);
     for (long long at = cc.at + (warp + kWarps - lag) % kWarps; at < piece_end; at += kWarps) {
-      if (!dead) dead = !mbar_wait_w(full + st, (phases >> st) & 1, &ctl.err, kErrWaitProducer);
-      if (!dead) {
-        phases ^= 1u << st;
-        pending &= ~(1u << st);
-      }
+      if (!dead) dead = !mbar_wait_w(&ctl.full[st], phase, &ctl.err, kErrWaitProducer);
       const int slot = tile_slot(cc.s, cc.i + static_cast<int>(at - cc.at));
-      const uint32_t k_base = smem_u32(ring + st * R::kStageBytes), v_base = k_base + R::kTileBytes;
-      float sk[2], lv[2], iv[2];  // of each 16 tokens: K's scale, log2 of V's and 1 / V's
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        // (tokens that no row sees, whose block may not even have a scale, take 1)
-        const int a = slot + 16 * t;
-        const bool some = a < cc.s.len;
-        sk[t] = some ? ctl.scale[warp][st][2 * t] : 1.f;
-        const float sv = some ? ctl.scale[warp][st][2 * t + 1] : 1.f;
-        lv[t] = __log2f(sv);
-        iv[t] = 1.f / sv;
-      }
+      const uint32_t k_base = smem_u32(smem + st * R::kStageBytes), v_base = k_base + R::kTileBytes;
+      const float4 sc0 = ctl.scale[st][0], sc1 = ctl.scale[st][1];
+      const float sk[2] = {sc0.x, sc1.x}, lv[2] = {sc0.y, sc1.y}, iv[2] = {sc0.z, sc1.z};
       // ---- scores
       float acc[2][kNT][4];
 #pragma unroll
@@ -495,8 +542,9 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
         }
       }
       __syncwarp();  // every lane has read the stage
-      if (!dead) issue(st);
-      st = st + 1 == kS ? 0 : st + 1;
+      if (lane == 0) mbar_arrive(&ctl.free[st]);
+      st += kWarps;
+      if (st >= kS) st -= kS, phase ^= 1;
     }
 
     // ---- the warps' sums of this piece
@@ -524,10 +572,9 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
         *reinterpret_cast<float2*>(mine + (2 * c) * kD + ((s * 16 + 2 * g) ^ (8 * c))) = make_float2(o[nt][s][0], o[nt][s][2]);
         *reinterpret_cast<float2*>(mine + (2 * c + 1) * kD + ((s * 16 + 2 * g) ^ (8 * c))) = make_float2(o[nt][s][1], o[nt][s][3]);
       }
-      __syncthreads();
-      const int r = threadIdx.x / (kD / 4), d4 = threadIdx.x % (kD / 4);
-      if (r < 8) {
-        const int row = row0 + nt * 8 + r;
+      sync_warps<kWarps>();
+      for (int r = threadIdx.x / (kD / 4); r < 8; r += kWarps * 32 / (kD / 4)) {
+        const int row = row0 + nt * 8 + r, d4 = threadIdx.x % (kD / 4);
         float top = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ctl.ml[w][nt * 8 + r][0]);
@@ -544,13 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
         }
         if (row < p.rows) {
           if (whole) {
-            const int i = row / p.group, hd = h * p.group + row - i * p.group;
-            const float inv = sum == 0.f ? 0.f : kHalfFactor<kInt8> / sum;
-            uint16_t* const to = p.out + ((static_cast<long long>(cc.b) * p.q_len + i) * p.hq + hd) * kD + d4 * 4;
-            *reinterpret_cast<uint2*>(to) = p.bf16 ? make_uint2(pack2<true>(x.x * inv, x.y * inv), pack2<true>(x.z * inv, x.w * inv))
-                                                   : make_uint2(pack2<false>(x.x * inv, x.y * inv), pack2<false>(x.z * inv, x.w * inv));
-            if (p.lse != nullptr && d4 == 0)
-              p.lse[(static_cast<long long>(cc.b) * p.hq + hd) * p.q_len + i] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.6931471805599453f;
+            store_row<kD, kInt8>(p, cc.b, h, row, d4, x, top, sum);
           } else {
             const long long to = (static_cast<long long>(blockIdx.x) * 2 + (from_start ? 1 : 0)) * kRows + nt * 8 + r;
             *reinterpret_cast<float4*>(p.part_o + to * kD + d4 * 4) = x;
@@ -558,87 +599,87 @@ __global__ void __launch_bounds__(kThreads, 1) cache_attn_kernel(const __grid_co
           }
         }
       }
-      __syncthreads();
+      sync_warps<kWarps>();
+    }
+    if (piece_end == end && threadIdx.x == 0) {
+      // (an item whose first piece this is and that goes on behind the share)
+      const long long first = cc.at - cc.i;
+      const int pieces = from_start && !to_end ? static_cast<int>(share_of(total, shares, first + cc.s.n - 1) - blockIdx.x + 1) : 0;
+      p.cut[blockIdx.x] = make_int4(cc.b, cc.item, pieces, 0);
     }
     cc.skip(p, piece_end - cc.at, end);
   }
-  if (dead) {
-    // the copies still on their way must not outlive the CTA's shared memory; each wait is limited
-    int own_err = 0;
-    for (int i = 0; i < kS; ++i)
-      if (pending >> i & 1) mbar_wait(full + i, (phases >> i) & 1, &own_err, kErrWaitProducer);
-    if (lane == 0) raise_status(p.status, p.mirror, kErrWaitProducer);
-  }
+  if (dead && lane == 0) raise_status(p.status, p.mirror, kErrWaitProducer);
 }
 
-// Joins the pieces of every (sequence, head, row tile) that more than one CTA worked on, in the CTAs' order, and writes
-// the rows of sequences that have nothing to attend to.  One CTA per (sequence, head, row tile).
+// Joins the pieces of every item that more than one CTA worked on, in the CTAs' order: block (c, r) row r of the item that the
+// first kernel's CTA c began and did not finish.  The pieces are dealt out to the warps, whose sums are added in order.
+// And writes the rows of sequences that have nothing to attend to.
 template <int kD, int kNT, bool kInt8>
-__global__ void __launch_bounds__(kThreads) cache_join_kernel(const __grid_constant__ AttnKernelParams p) {
-  constexpr int kRows = 8 * kNT;
-  __shared__ long long s_prefix[kThreads + 1], s_warp[kWarps];
+__global__ void __launch_bounds__(kJoin) cache_join_kernel(const __grid_constant__ AttnKernelParams p) {
+  constexpr int kRows = 8 * kNT, kParts = kJoin / (kD / 4);
+  __shared__ float4 s_x[kParts][kD / 4];
+  __shared__ float2 s_ml[kParts];
+  griddep_launch();
   griddep_wait();
-  const int items = p.c.hkv * p.row_tiles;
-  const int b = blockIdx.x / items, item = blockIdx.x - b * items;
-  const int h = item / p.row_tiles, row0 = (item - h * p.row_tiles) * kRows;
-  const SeqTiles s = seq_tiles(p, b);
-  long long lo = 0, hi = 0;
-  long long total = 1, shares = 1;
-  if (s.n > 0) {
-    tile_prefix(p, s_prefix, s_warp);
-    total = s_prefix[kThreads] * items;
-    shares = n_shares(total, p.ctas);
-    const int per = (p.batch + kThreads - 1) / kThreads;
-    long long first = s_prefix[b / per];
-    for (int k = b / per * per; k < b; ++k) first += seq_tiles(p, k).n;
-    first = first * items + static_cast<long long>(item) * s.n;
-    lo = share_of(total, shares, first);
-    hi = share_of(total, shares, first + s.n - 1);
-    if (lo == hi) return;  // written already
-    // (the first piece is its CTA's last one, from the item's start on; the others are their CTAs' first ones)
-  }
-  for (int r = threadIdx.x / (kD / 4); r < kRows; r += kThreads / (kD / 4)) {
-    const int row = row0 + r, d4 = threadIdx.x % (kD / 4);
-    if (row >= p.rows) break;
-    float top = -INFINITY, sum = 0.f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (s.n > 0) {
-      for (long long c = lo; c <= hi; ++c) top = fmaxf(top, p.part_ml[((c * 2 + (c == lo ? 1 : 0)) * kRows + r) * 2]);
-#pragma unroll 4
-      for (long long c = lo; c <= hi; ++c) {
-        const long long at = (c * 2 + (c == lo ? 1 : 0)) * kRows + r;
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-        const float4 y = *reinterpret_cast<const float4*>(p.part_o + at * kD + d4 * 4);
+  const int r = blockIdx.y, d4 = threadIdx.x % (kD / 4), part = threadIdx.x / (kD / 4);
+  if (blockIdx.x < p.ctas) {
+    const int4 cut = p.cut[blockIdx.x];
+    const int h = cut.y / p.row_tiles, row = (cut.y - h * p.row_tiles) * kRows + r;
+    if (cut.z > 0 && row < p.rows) {
+      const auto place = [&](int k) { return (static_cast<long long>(blockIdx.x + k) * 2 + (k == 0 ? 1 : 0)) * kRows + r; };
+      float top = -INFINITY, sum = 0.f;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = part; k < cut.z; k += kParts) top = fmaxf(top, p.part_ml[place(k) * 2]);
+      for (int k = part; k < cut.z; k += kParts) {
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + place(k) * 2);
+        const float4 y = *reinterpret_cast<const float4*>(p.part_o + place(k) * kD + d4 * 4);
         if (ml.y == 0.f) continue;
         const float f = ex2f(ml.x - top);
         sum += ml.y * f;
         x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
       }
+      s_x[part][d4] = x;
+      if (d4 == 0) s_ml[part] = make_float2(top, sum);
+      __syncthreads();
+      if (part == 0) {
+        top = -INFINITY, sum = 0.f;
+        x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) top = fmaxf(top, s_ml[k].x);
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) {
+          if (s_ml[k].y == 0.f) continue;
+          const float f = ex2f(s_ml[k].x - top);
+          const float4 y = s_x[k][d4];
+          sum += s_ml[k].y * f;
+          x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
+        }
+        store_row<kD, kInt8>(p, cut.x, h, row, d4, x, top, sum);
+      }
     }
-    const int i = row / p.group, hd = h * p.group + row - i * p.group;
-    const float inv = sum == 0.f ? 0.f : kHalfFactor<kInt8> / sum;
-    uint16_t* const to = p.out + ((static_cast<long long>(b) * p.q_len + i) * p.hq + hd) * kD + d4 * 4;
-    *reinterpret_cast<uint2*>(to) = p.bf16 ? make_uint2(pack2<true>(x.x * inv, x.y * inv), pack2<true>(x.z * inv, x.w * inv))
-                                           : make_uint2(pack2<false>(x.x * inv, x.y * inv), pack2<false>(x.z * inv, x.w * inv));
-    if (p.lse != nullptr && d4 == 0)
-      p.lse[(static_cast<long long>(b) * p.hq + hd) * p.q_len + i] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.6931471805599453f;
   }
+  if (blockIdx.y == 0)
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+      if (seq_tiles(p, b).n > 0) continue;
+      for (int row = part; row < p.rows * p.c.hkv; row += kParts)
+        store_row<kD, kInt8>(p, b, row / p.rows, row % p.rows, d4, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
+    }
 }
 
 // Adds every visible slot's softmax weights up, from the scores that the first kernel kept and the final log-sum-exp.
 // One CTA per (sequence, head) and kWeightTiles tiles.
-constexpr int kWeightTiles = 64;
+constexpr int kWeightTiles = 16;
 template <int kNT>
-__global__ void __launch_bounds__(kThreads) cache_weights_kernel(const __grid_constant__ AttnKernelParams p, int chunks) {
+__global__ void __launch_bounds__(kJoin) cache_weights_kernel(const __grid_constant__ AttnKernelParams p, int chunks) {
   constexpr int kRows = 8 * kNT;
-  __shared__ long long s_prefix[kThreads + 1], s_warp[kWarps];
   extern __shared__ float s_lse[];  // [row_tiles * kRows], base 2; +inf for rows that see nothing and rows behind the last
   griddep_wait();
   const int bh = blockIdx.x / chunks, b = bh / p.c.hkv, h = bh - b * p.c.hkv;
   const SeqTiles s = seq_tiles(p, b);
   const int t0 = (blockIdx.x - bh * chunks) * kWeightTiles;
   if (t0 >= s.n) return;
-  for (int r = threadIdx.x; r < p.row_tiles * kRows; r += kThreads) {
+  for (int r = threadIdx.x; r < p.row_tiles * kRows; r += kJoin) {
     float x = INFINITY;
     if (r < p.rows) {
       const int i = r / p.group;
@@ -647,13 +688,10 @@ __global__ void __launch_bounds__(kThreads) cache_weights_kernel(const __grid_co
     }
     s_lse[r] = x;
   }
-  tile_prefix(p, s_prefix, s_warp);
-  const int items = p.c.hkv * p.row_tiles, per = (p.batch + kThreads - 1) / kThreads;
-  long long first = s_prefix[b / per];
-  for (int k = b / per * per; k < b; ++k) first += seq_tiles(p, k).n;
-  first = first * items + static_cast<long long>(h) * p.row_tiles * s.n;
+  __syncthreads();
+  const long long first = p.first[b] + static_cast<long long>(h) * p.row_tiles * s.n;
   const int t1 = min(t0 + kWeightTiles, s.n);
-  for (int k = t0 * kTok + threadIdx.x; k < t1 * kTok; k += kThreads) {
+  for (int k = t0 * kTok + threadIdx.x; k < t1 * kTok; k += kJoin) {
     const int tile = k / kTok, tok = tile_slot(s, tile) + k % kTok;
     if (tok >= s.len) continue;
     float sum = 0.f;
@@ -674,8 +712,8 @@ __global__ void __launch_bounds__(kThreads) cache_weights_kernel(const __grid_co
 struct Plan {
   int nt, row_tiles, ctas;
   long long most_tiles;  // of a sequence, per head and row tile
-  int64_t o_bytes, ml_bytes, score_bytes, lse_bytes;
-  int64_t total() const { return o_bytes + ml_bytes + score_bytes; }
+  int64_t o_bytes, ml_bytes, cut_bytes, first_bytes, score_bytes;
+  int64_t total() const { return o_bytes + ml_bytes + cut_bytes + first_bytes + score_bytes; }
 };
 
 // kNT = 1 up to 8 query rows per key/value head, else row tiles of 16.
@@ -703,6 +741,8 @@ int make_plan(const rswa_cache_attn_params_t& a, Plan& plan) {
   plan.ctas = static_cast<int>(share < 1 ? 1 : share < sms ? share : sms);
   plan.o_bytes = 2LL * plan.ctas * per_tile * a.cache.head_dim * 4;
   plan.ml_bytes = (2LL * plan.ctas * per_tile * 2 * 4 + 255) / 256 * 256;
+  plan.cut_bytes = (plan.ctas * 16LL + 255) / 256 * 256;
+  plan.first_bytes = a.weights != nullptr ? (a.table.batch * 8LL + 255) / 256 * 256 : 0;
   plan.score_bytes = a.weights != nullptr ? items * most * kTok * per_tile * 4 : 0;
   return RSWA_OK;
 }
@@ -742,16 +782,17 @@ cudaError_t launch_attn(const AttnKernelParams& kp, const Plan& plan, cudaStream
     if (e != cudaSuccess) return e;
     if (dev < 64) set.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  e = launch_kernel(kern, dim3(plan.ctas), kThreads, smem, s, true, kp);
+  e = launch_kernel(kern, dim3(plan.ctas), Layout<kD, kNT>::kThreads, smem, s, true, kp);
   if (e != cudaSuccess) return e;
-  const long long items = static_cast<long long>(kp.batch) * kp.c.hkv * plan.row_tiles;
-  e = launch_kernel(cache_join_kernel<kD, kNT, kInt8>, dim3(static_cast<unsigned>(items)), kThreads, 0, s, true, kp);
+  const int blocks = plan.ctas > kp.batch ? plan.ctas : kp.batch < sm_count() ? kp.batch : sm_count();
+  const int most_rows = plan.row_tiles > 1 ? 8 * kNT : kp.rows;
+  e = launch_kernel(cache_join_kernel<kD, kNT, kInt8>, dim3(blocks, most_rows), kJoin, 0, s, true, kp);
   if (e != cudaSuccess) return e;
   count_launches(2);
   if (kp.weights != nullptr && plan.most_tiles > 0) {
     const long long chunks = (plan.most_tiles + kWeightTiles - 1) / kWeightTiles;
     const dim3 grid(static_cast<unsigned>(static_cast<long long>(kp.batch) * kp.c.hkv * chunks));
-    e = launch_kernel(cache_weights_kernel<kNT>, grid, kThreads, plan.row_tiles * 8 * kNT * 4, s, true, kp, static_cast<int>(chunks));
+    e = launch_kernel(cache_weights_kernel<kNT>, grid, kJoin, plan.row_tiles * 8 * kNT * 4, s, true, kp, static_cast<int>(chunks));
     if (e != cudaSuccess) return e;
     count_launches(1);
   }
@@ -827,10 +868,13 @@ extern "C" int rswa_cache_attn(const rswa_cache_attn_params_t* p, void* stream) 
   kp.bf16 = p->dtype == RSWA_DTYPE_BF16;
   kp.out = static_cast<uint16_t*>(p->out);
   kp.lse = p->lse;
-  uint8_t* const ws = static_cast<uint8_t*>(p->workspace);
+  uint8_t* ws = static_cast<uint8_t*>(p->workspace);
   kp.part_o = reinterpret_cast<float*>(ws);
-  kp.part_ml = reinterpret_cast<float*>(ws + plan.o_bytes);
-  kp.scores = p->weights != nullptr ? reinterpret_cast<float*>(ws + plan.o_bytes + plan.ml_bytes) : nullptr;
+  kp.part_ml = reinterpret_cast<float*>(ws += plan.o_bytes);
+  kp.cut = reinterpret_cast<int4*>(ws += plan.ml_bytes);
+  ws += plan.cut_bytes;
+  kp.first = p->weights != nullptr ? reinterpret_cast<long long*>(ws) : nullptr;
+  kp.scores = p->weights != nullptr ? reinterpret_cast<float*>(ws + plan.first_bytes) : nullptr;
   kp.weights = p->weights;
   kp.w_sb = p->w_stride_b, kp.w_sh = p->w_stride_h;
   kp.ctas = plan.ctas;
