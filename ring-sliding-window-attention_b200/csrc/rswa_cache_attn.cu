@@ -22,11 +22,13 @@
 // a V block goes into its tokens' exponents (s + log2 of the scale), so that the running reference covers both;
 // the sum of the weights takes it back out.  Scores, sums and the output are 32-bit.
 //
-// Work: the 32-token tiles of all (sequence, key/value head, 8 or 16 query rows) in one order, cut evenly over the CTAs
-// (one per SM) whatever the lengths.  In a CTA one warp keeps a ring of tiles filled (its lanes look the blocks of 32
-// tiles up at a time: the table's latency is paid once for all of them), the others take the tiles in turn and add up at the
-// end of each piece; the ring runs on over sequence boundaries.  A piece that is not a whole (sequence, head) goes to the
-// workspace and a second kernel joins the pieces in order: results do not depend on timing.
+// Work: the 32-token tiles of all (sequence, key/value head, 8 or 16 query rows) in one order, cut evenly whatever the
+// lengths over groups of four warps (one CTA of three or four groups per SM).  The warps of a group take its tiles in turn and
+// add up at the end of each piece; groups rather than CTAs because the end of a piece and the next one's queries cost every
+// warp that takes part as much as several tiles.  Every warp loads for itself: K of its next tile as soon as the scores are
+// formed, V as soon as the output is, on over sequence boundaries; its lanes look 32 tiles up in the block table at a
+// time, so that the table's latency is paid once for all of them.  A piece that is not a whole (sequence, head) goes to
+// the workspace and a second kernel joins the pieces in order: results do not depend on timing.
 #include <atomic>
 
 #include "rswa_cache.cuh"
@@ -42,8 +44,9 @@ namespace {
 
 constexpr int kTok = 32;     // tokens of a tile
 constexpr int kScan = 256;   // threads of the prefix sums over sequences
-constexpr int kMinShare = 8; // tiles of a CTA at least
-constexpr int kJoin = 256;   // threads of the kernels behind the first one
+constexpr int kGroup = 4;    // warps that share the work of a piece
+constexpr int kMinShare = 4; // tiles of a group at least
+constexpr int kJoin = 1024, kAdd = 256;  // threads of the kernels behind the first one
 constexpr float kRoom = 14.f;  // a weight may grow to 2^14 before the reference is raised (fp16 ends at 2^16)
 constexpr float kLow = 4.f;    // and is raised to the maximum minus 4, so that not every new maximum raises it
 
@@ -62,14 +65,14 @@ struct AttnKernelParams {
   int bf16;
   uint16_t* out;
   float* lse;        // or null
-  float* part_o;     // [CTAs][2][8 * kNT][head_dim]
-  float* part_ml;    // [CTAs][2][8 * kNT][2]
-  int4* cut;         // [CTAs]: an item whose first piece is the CTA's last one: sequence, head * row tiles + row tile, pieces (or 0)
+  float* part_o;     // [groups][2][8 * kNT][head_dim]
+  float* part_ml;    // [groups][2][8 * kNT][2]
+  int4* cut;         // [groups]: an item whose first piece is the group's last one: sequence, head * row tiles + row tile, pieces (or 0)
   float* scores;     // [tiles][kTok][8 * kNT], or null: what the weights need
   long long* first;  // [batch]: index of a sequence's first tile, with scores
   float* weights;
   long long w_sb, w_sh;
-  int ctas;
+  int groups;
   int* status;
   int* mirror;
 };
@@ -95,8 +98,8 @@ __device__ __forceinline__ SeqTiles seq_tiles(const AttnKernelParams& p, int b) 
 }
 __device__ __forceinline__ int tile_slot(const SeqTiles& s, int i) { return (i < s.n_sink_tiles ? i : s.first + i - s.n_sink_tiles) * kTok; }
 
-// Where the work of a CTA begins and ends: equal shares of all tiles, none of fewer than kMinShare.
-__device__ __forceinline__ long long n_shares(long long total, int ctas) { return min(static_cast<long long>(ctas), max(1LL, total / kMinShare)); }
+// Where the work of a group begins and ends: equal shares of all tiles, none of fewer than kMinShare.
+__device__ __forceinline__ long long n_shares(long long total, int groups) { return min(static_cast<long long>(groups), max(1LL, total / kMinShare)); }
 __device__ __forceinline__ long long share_begin(long long total, long long shares, long long c) { return total * c / shares; }
 __device__ __forceinline__ long long share_of(long long total, long long shares, long long tile) { return ((tile + 1) * shares - 1) / total; }
 
@@ -190,26 +193,25 @@ struct Ring {
   static constexpr int kStageBytes = 2 * kTileBytes;
 };
 
-// kWarps that compute (with the loading one 16 warps of 128 registers a thread, or for 16 query rows 12 of 168),
-// kStages tiles in flight: 160 KB or more, where the latency of a load asks for about 50.
+// 16 warps of 128 registers a thread, or for 16 query rows 12 of 168.  A tile in flight per warp is 96 KB or more, where
+// the latency of a load asks for about 50.
 template <int kD, int kNT>
 struct Layout {
-  static constexpr int kWarps = kNT == 1 ? 15 : 11;
-  static constexpr int kThreads = (kWarps + 1) * 32;
-  static constexpr int kStages = (kNT == 1 ? 20 : 22) * (128 / kD);
+  static constexpr int kWarps = kNT == 1 ? 16 : 12;
+  static constexpr int kThreads = kWarps * 32, kGroups = kWarps / kGroup;
   struct Ctl {
-    uint64_t full[kStages], free[kStages];
-    float4 scale[kStages][2];           // of the tile's first 16 tokens and its last 16: K's scale, log2 of V's, 1 / V's
+    uint64_t full[kWarps][2];           // K, V
+    float4 scale[kWarps][32][2];        // the looked-up tiles: of the first 16 tokens and the last 16 K's scale, log2 of V's, 1 / V's
+    int2 row[kWarps][32];               // and where their K and V lie
     float ml[kWarps][8 * kNT][2];       // reference and sum of every warp's piece
+    long long prefix[kScan + 1 + kScan / 32];
     int err;
   };
-  static constexpr int kRings = kStages * Ring<kD>::kStageBytes;
+  static constexpr int kRings = kWarps * Ring<kD>::kStageBytes;
   static constexpr int kMerge = kWarps * 8 * kD * 4;
-  // [ring][sums of the warps' pieces; at first the sequences' prefix sums][control]
+  // [tiles][sums of the warps' pieces][control]
   static constexpr int kBytes = kRings + kMerge + static_cast<int>(sizeof(Ctl));
   static_assert(kBytes <= 232448, "shared memory budget");
-  static_assert(kMerge >= (kScan + 1 + kScan / 32) * 8, "the prefix sums lie where the pieces' sums come later");
-  static_assert(kStages >= kWarps, "a warp's next tile is at most one turn of the ring away");
 };
 
 __device__ __forceinline__ void tma_load_rows(void* dst, const CUtensorMap* m, uint64_t* bar, int row) {
@@ -240,10 +242,7 @@ __device__ __forceinline__ uint32_t piece(uint32_t base, int row, int chunk) {
   return base + row * kD + ((kD == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4);
 }
 
-template <int kWarps>
-__device__ __forceinline__ void sync_warps() {
-  asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
-}
+__device__ __forceinline__ void sync_group(int group) { asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(kGroup * 32) : "memory"); }
 // four elements of a finished row, and its log-sum-exp
 template <int kD, bool kInt8>
 __device__ __forceinline__ void store_row(const AttnKernelParams& p, int b, int h, int row, int d4, float4 x, float top, float sum) {
@@ -261,13 +260,18 @@ template <int kD, int kNT, bool kInt8>
 __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_kernel(const __grid_constant__ AttnKernelParams p) {
   using L = Layout<kD, kNT>;
   using R = Ring<kD>;
-  constexpr int kS = L::kStages, kKS = kD / 16, kWarps = L::kWarps;
+  constexpr int kKS = kD / 16;
   constexpr int kRows = 8 * kNT;
   extern __shared__ __align__(1024) uint8_t smem[];
   auto& ctl = *reinterpret_cast<typename L::Ctl*>(smem + L::kRings + L::kMerge);
-  float* const merge = reinterpret_cast<float*>(smem + L::kRings);
-  long long* const s_prefix = reinterpret_cast<long long*>(merge);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int group = warp / kGroup, wg = warp % kGroup;
+  // (the first groups of all CTAs come first: a call too small for all of them spreads over the SMs)
+  const int me = group * gridDim.x + blockIdx.x;
+  float* const merge = reinterpret_cast<float*>(smem + L::kRings) + group * kGroup * 8 * kD;
+  auto& ml = *reinterpret_cast<float(*)[kGroup][kRows][2]>(ctl.ml[group * kGroup]);
+  uint8_t* const own = smem + warp * R::kStageBytes;  // this warp's tile: K, then V
+  uint64_t* const full = ctl.full[warp];
 
   griddep_launch();
   if (threadIdx.x == 0) {
@@ -275,82 +279,65 @@ __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_ker
     prefetch_tmap(&p.map[0]);
     prefetch_tmap(&p.map[1]);
   }
-  if (threadIdx.x < kS) {
-    mbar_init(&ctl.full[threadIdx.x], 1);
-    mbar_init(&ctl.free[threadIdx.x], 1);
-  }
+  if (lane < 2) mbar_init(full + lane, 1);
   mbar_fence_init();
   griddep_wait();
-  tile_prefix(p, s_prefix, s_prefix + kScan + 1);
-  const long long total = s_prefix[kScan] * p.c.hkv * p.row_tiles;
-  const long long shares = n_shares(total, p.ctas);
-  if (blockIdx.x >= shares || total == 0) {
-    if (threadIdx.x == 0) p.cut[blockIdx.x] = make_int4(0, 0, 0, 0);
+  tile_prefix(p, ctl.prefix, ctl.prefix + kScan + 1);
+  const long long total = ctl.prefix[kScan] * p.c.hkv * p.row_tiles;
+  const long long shares = n_shares(total, p.groups);
+  if (me >= shares || total == 0) {
+    if (me < p.groups && threadIdx.x % (kGroup * 32) == 0) p.cut[me] = make_int4(0, 0, 0, 0);
     return;
   }
-  const long long begin = share_begin(total, shares, blockIdx.x), end = share_begin(total, shares, blockIdx.x + 1);
-  Cursor cc = cursor_at(p, s_prefix, begin);
-  __syncthreads();  // (the prefix sums make room)
+  const long long begin = share_begin(total, shares, me), end = share_begin(total, shares, me + 1);
+  const int box = min(p.c.bs, kTok);
 
-  if (warp == kWarps) {
-    // ---------------------------------------------------------------- loads: every lane looks up a tile of the next 32
-    const int bs = p.c.bs, box = min(bs, kTok);
-    Cursor lc = cc;
-    lc.skip(p, lane, end);
-    bool ok = true;
-    int at = 0;  // index of the tile within the share
-    int st = 0, round = 0;
-    const int n = static_cast<int>(end - begin);
-    while (at < n && ok) {
-      int row[2] = {0, 0};
-      float4 sc[2] = {make_float4(1.f, 0.f, 1.f, 0.f), make_float4(1.f, 0.f, 1.f, 0.f)};
-      if (lc.at < end) {
-        const int slot = tile_slot(lc.s, lc.i), h = lc.item / p.row_tiles, j = slot / bs;
-        // a tile is part of one block, or two blocks of 16; the second may lie behind the sequence's end: not looked at
-        int pg[2];
-        pg[0] = table_entry(p.table, p.table_stride, lc.b, j, p.c.num_blocks, p.status, p.mirror);
-        pg[1] = pg[0];
-        if (bs < kTok) pg[1] = slot + bs < lc.s.len ? table_entry(p.table, p.table_stride, lc.b, j + 1, p.c.num_blocks, p.status, p.mirror) : pg[0];
+  // The tiles of this warp, counted: tile i is the share's tile wg + i * kGroup.  Looks 32 of them up, one a lane.
+  const int n_own = static_cast<int>((end - begin - wg + kGroup - 1) / kGroup);
+  auto look_up = [&](int i) {
+    const long long at = begin + wg + static_cast<long long>(i + lane) * kGroup;
+    __syncwarp();
+    if (at < end) {
+      const Cursor lc = cursor_at(p, ctl.prefix, at);
+      const int bs = p.c.bs, slot = tile_slot(lc.s, lc.i), h = lc.item / p.row_tiles, j = slot / bs;
+      // a tile is part of one block, or two blocks of 16; the second may lie behind the sequence's end: not looked at
+      int pg[2], row[2];
+      pg[0] = table_entry(p.table, p.table_stride, lc.b, j, p.c.num_blocks, p.status, p.mirror);
+      pg[1] = pg[0];
+      if (bs < kTok && slot + bs < lc.s.len) pg[1] = table_entry(p.table, p.table_stride, lc.b, j + 1, p.c.num_blocks, p.status, p.mirror);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int page = max(pg[t], 0);  // (reported; any block will do then)
-          const long long ph = static_cast<long long>(page) * p.c.hkv + h;
-          row[t] = (page * p.c.hkv + h) * bs + slot % bs;
-          if (slot + 16 * t < lc.s.len) {  // (tokens behind the end: their block may not even have a scale)
-            const float sv = p.c.scale[1][ph];
-            sc[t] = make_float4(p.c.scale[0][ph], __log2f(sv), 1.f / sv, 0.f);
-          }
+      for (int t = 0; t < 2; ++t) {
+        const int page = max(pg[t], 0);  // (reported; any block will do then)
+        const long long ph = static_cast<long long>(page) * p.c.hkv + h;
+        row[t] = static_cast<int>(ph) * bs + slot % bs;
+        float4 sc = make_float4(1.f, 0.f, 1.f, 0.f);
+        if (slot + 16 * t < lc.s.len) {  // (tokens behind the end: their block may not even have a scale)
+          const float sv = p.c.scale[1][ph];
+          sc = make_float4(p.c.scale[0][ph], __log2f(sv), 1.f / sv, 0.f);
         }
+        ctl.scale[warp][lane][t] = sc;
       }
-      lc.skip(p, 32, end);
-      __syncwarp();
-#pragma unroll 1
-      for (int k = 0; k < 32 && at < n && ok; ++k, ++at) {
-        if (round > 0) ok = mbar_wait_w<20>(&ctl.free[st], (round - 1) & 1, &ctl.err, kErrWaitProducer);
-        if (ok && lane == k) {
-          ctl.scale[st][0] = sc[0];
-          ctl.scale[st][1] = sc[1];
-          mbar_expect_tx(&ctl.full[st], R::kStageBytes);
-          uint8_t* const dst = smem + st * R::kStageBytes;
-#pragma unroll
-          for (int kv = 0; kv < 2; ++kv) {
-            tma_load_rows(dst + kv * R::kTileBytes, &p.map[kv], &ctl.full[st], row[0]);
-            if (box < kTok) tma_load_rows(dst + kv * R::kTileBytes + box * kD, &p.map[kv], &ctl.full[st], row[1]);
-          }
-        }
-        if (++st == kS) st = 0, ++round;
-      }
+      ctl.row[warp][lane] = make_int2(row[0], row[1]);
     }
-    if (!ok) {
-      // the copies still on their way must not outlive the CTA's shared memory; each wait is limited
-      int own_err = 0;
-      for (int i = max(0, at - 1 - kS); i < at - 1; ++i) mbar_wait(&ctl.full[i % kS], (i / kS) & 1, &own_err, kErrWaitProducer);
-      if (lane == 0) raise_status(p.status, p.mirror, kErrWaitProducer);
+    __syncwarp();
+  };
+  int loaded[2] = {0, 0};  // the last tile loaded
+  auto load = [&](int i, int kv) {
+    loaded[kv] = i;
+    if (lane == 0) {
+      const int2 row = ctl.row[warp][i & 31];
+      mbar_expect_tx(full + kv, R::kTileBytes);
+      tma_load_rows(own + kv * R::kTileBytes, &p.map[kv], full + kv, row.x);
+      if (box < kTok) tma_load_rows(own + kv * R::kTileBytes + box * kD, &p.map[kv], full + kv, row.y);
     }
-    return;
+  };
+  if (n_own > 0) {
+    look_up(0);
+    load(0, 0);
+    load(0, 1);
   }
-
-  int st = warp, phase = 0;  // of this warp's next tile
+  Cursor cc = cursor_at(p, ctl.prefix, begin);
+  int own_i = 0;  // this warp's next tile
   bool dead = false;
   while (cc.at < end) {
     const long long piece_end = min(end, cc.at + cc.s.n - cc.i);
@@ -425,13 +412,12 @@ __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_ker
       m[nt][0] = m[nt][1] = -INFINITY;
       l[nt][0] = l[nt][1] = 0.f;
     }
-    // this warp's tiles of the piece: those whose index from `begin` is `warp` modulo kWarps
-    const int lag = static_cast<int>((cc.at - begin) % kWarps);
-    for (long long at = cc.at + (warp + kWarps - lag) % kWarps; at < piece_end; at += kWarps) {
-      if (!dead) dead = !mbar_wait_w(&ctl.full[st], phase, &ctl.err, kErrWaitProducer);
+    // this warp's tiles of the piece: those whose index from `begin` is `wg` modulo kGroup
+    for (long long at = begin + wg + static_cast<long long>(own_i) * kGroup; at < piece_end; at += kGroup) {
+      const float4 sc0 = ctl.scale[warp][own_i & 31][0], sc1 = ctl.scale[warp][own_i & 31][1];
+      if (!dead) dead = !mbar_wait_w(full, own_i & 1, &ctl.err, kErrWaitProducer);
       const int slot = tile_slot(cc.s, cc.i + static_cast<int>(at - cc.at));
-      const uint32_t k_base = smem_u32(smem + st * R::kStageBytes), v_base = k_base + R::kTileBytes;
-      const float4 sc0 = ctl.scale[st][0], sc1 = ctl.scale[st][1];
+      const uint32_t k_base = smem_u32(own), v_base = k_base + R::kTileBytes;
       const float sk[2] = {sc0.x, sc1.x}, lv[2] = {sc0.y, sc1.y}, iv[2] = {sc0.z, sc1.z};
       // ---- scores
       float acc[2][kNT][4];
@@ -451,6 +437,11 @@ __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_ker
           mma16816(acc[1][nt], lo[2], lo[3], hi[2], hi[3], qf[nt][s][0], qf[nt][s][1]);
         }
       }
+      // every lane has read K: the next tile's
+      const bool more = own_i + 1 < n_own && !dead;
+      if (more && ((own_i + 1) & 31) == 0) look_up(own_i + 1);
+      __syncwarp();
+      if (more) load(own_i + 1, 0);
       // ---- to base 2, hidden ones to -inf
       const bool plain = slot + kTok - 1 <= last_min && (slot >= first_max || slot + kTok <= p.n_sink);
 #pragma unroll
@@ -529,6 +520,7 @@ __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_ker
         }
       }
       // ---- output
+      if (!dead) dead = !mbar_wait_w(full + 1, own_i & 1, &ctl.err, kErrWaitProducer);
 #pragma unroll
       for (int s = 0; s < kKS; ++s) {
         uint32_t w[4], lo[4], hi[4];
@@ -541,10 +533,9 @@ __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_ker
           mma16816(o[nt][s], lo[2], hi[2], lo[3], hi[3], pf[1][nt][0], pf[1][nt][1]);
         }
       }
-      __syncwarp();  // every lane has read the stage
-      if (lane == 0) mbar_arrive(&ctl.free[st]);
-      st += kWarps;
-      if (st >= kS) st -= kS, phase ^= 1;
+      __syncwarp();  // every lane has read V
+      if (more && !dead) load(own_i + 1, 1);
+      ++own_i;
     }
 
     // ---- the warps' sums of this piece
@@ -559,32 +550,34 @@ __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_ker
         x += __shfl_xor_sync(0xffffffffu, x, 8);
         x += __shfl_xor_sync(0xffffffffu, x, 16);
         if (g == 0) {
-          ctl.ml[warp][nt * 8 + 2 * c + k][0] = m[nt][k];
-          ctl.ml[warp][nt * 8 + 2 * c + k][1] = x;
+          ml[wg][nt * 8 + 2 * c + k][0] = m[nt][k];
+          ml[wg][nt * 8 + 2 * c + k][1] = x;
         }
       }
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
       // (float d of row r lies at d ^ 8 * (r / 2): no bank twice in a half-warp's stores)
-      float* const mine = merge + warp * 8 * kD;
+      float* const mine = merge + wg * 8 * kD;
 #pragma unroll
       for (int s = 0; s < kKS; ++s) {
         *reinterpret_cast<float2*>(mine + (2 * c) * kD + ((s * 16 + 2 * g) ^ (8 * c))) = make_float2(o[nt][s][0], o[nt][s][2]);
         *reinterpret_cast<float2*>(mine + (2 * c + 1) * kD + ((s * 16 + 2 * g) ^ (8 * c))) = make_float2(o[nt][s][1], o[nt][s][3]);
       }
-      sync_warps<kWarps>();
-      for (int r = threadIdx.x / (kD / 4); r < 8; r += kWarps * 32 / (kD / 4)) {
-        const int row = row0 + nt * 8 + r, d4 = threadIdx.x % (kD / 4);
+      sync_group(group);
+      const int t = threadIdx.x % (kGroup * 32), d4 = t % (kD / 4);
+#pragma unroll
+      for (int r = t / (kD / 4); r < 8; r += kGroup * 32 / (kD / 4)) {
+        const int row = row0 + nt * 8 + r;
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ctl.ml[w][nt * 8 + r][0]);
+        for (int w = 0; w < kGroup; ++w) top = fmaxf(top, ml[w][nt * 8 + r][0]);
         float sum = 0.f;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float lw = ctl.ml[w][nt * 8 + r][1];
+        for (int w = 0; w < kGroup; ++w) {
+          const float lw = ml[w][nt * 8 + r][1];
           if (lw == 0.f) continue;  // (no visible token)
-          const float f = ex2f(ctl.ml[w][nt * 8 + r][0] - top);
+          const float f = ex2f(ml[w][nt * 8 + r][0] - top);
           const float4 y = *reinterpret_cast<const float4*>(merge + (w * 8 + r) * kD + ((d4 * 4) ^ (r / 2 * 8)));
           sum += lw * f;
           x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
@@ -593,85 +586,90 @@ __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_ker
           if (whole) {
             store_row<kD, kInt8>(p, cc.b, h, row, d4, x, top, sum);
           } else {
-            const long long to = (static_cast<long long>(blockIdx.x) * 2 + (from_start ? 1 : 0)) * kRows + nt * 8 + r;
+            const long long to = (static_cast<long long>(me) * 2 + (from_start ? 1 : 0)) * kRows + nt * 8 + r;
             *reinterpret_cast<float4*>(p.part_o + to * kD + d4 * 4) = x;
             if (d4 == 0) *reinterpret_cast<float2*>(p.part_ml + to * 2) = make_float2(top, sum);
           }
         }
       }
-      sync_warps<kWarps>();
+      sync_group(group);
     }
-    if (piece_end == end && threadIdx.x == 0) {
+    if (piece_end == end && wg == 0 && lane == 0) {
       // (an item whose first piece this is and that goes on behind the share)
       const long long first = cc.at - cc.i;
-      const int pieces = from_start && !to_end ? static_cast<int>(share_of(total, shares, first + cc.s.n - 1) - blockIdx.x + 1) : 0;
-      p.cut[blockIdx.x] = make_int4(cc.b, cc.item, pieces, 0);
+      const int pieces = from_start && !to_end ? static_cast<int>(share_of(total, shares, first + cc.s.n - 1) - me + 1) : 0;
+      p.cut[me] = make_int4(cc.b, cc.item, pieces, 0);
     }
     cc.skip(p, piece_end - cc.at, end);
   }
-  if (dead && lane == 0) raise_status(p.status, p.mirror, kErrWaitProducer);
+  if (dead) {
+    // copies still on their way must not outlive the CTA's shared memory (each wait is limited)
+    int own_err = 0;
+    if (n_own > 0)
+      for (int kv = 0; kv < 2; ++kv) mbar_wait(full + kv, loaded[kv] & 1, &own_err, kErrWaitProducer);
+    if (lane == 0) raise_status(p.status, p.mirror, kErrWaitProducer);
+  }
 }
 
-// Joins the pieces of every item that more than one CTA worked on, in the CTAs' order: block (c, r) row r of the item that the
-// first kernel's CTA c began and did not finish.  The pieces are dealt out to the warps, whose sums are added in order.
+// Joins the pieces of every item that more than one group worked on, in the groups' order: block c the item that group c
+// began and did not finish.  A row's pieces are dealt out to several threads, whose sums are added in order.
 // And writes the rows of sequences that have nothing to attend to.
 template <int kD, int kNT, bool kInt8>
 __global__ void __launch_bounds__(kJoin) cache_join_kernel(const __grid_constant__ AttnKernelParams p) {
-  constexpr int kRows = 8 * kNT, kParts = kJoin / (kD / 4);
-  __shared__ float4 s_x[kParts][kD / 4];
-  __shared__ float2 s_ml[kParts];
+  constexpr int kRows = 8 * kNT, kParts = kJoin / (kD / 4) / kRows;
+  __shared__ float4 s_x[kParts][kRows][kD / 4];
+  __shared__ float2 s_ml[kParts][kRows];
   griddep_launch();
   griddep_wait();
-  const int r = blockIdx.y, d4 = threadIdx.x % (kD / 4), part = threadIdx.x / (kD / 4);
-  if (blockIdx.x < p.ctas) {
-    const int4 cut = p.cut[blockIdx.x];
+  const int d4 = threadIdx.x % (kD / 4), r = threadIdx.x / (kD / 4) % kRows, part = threadIdx.x / (kD / 4) / kRows;
+  const int4 cut = blockIdx.x < p.groups ? p.cut[blockIdx.x] : make_int4(0, 0, 0, 0);
+  if (cut.z > 0) {
     const int h = cut.y / p.row_tiles, row = (cut.y - h * p.row_tiles) * kRows + r;
-    if (cut.z > 0 && row < p.rows) {
-      const auto place = [&](int k) { return (static_cast<long long>(blockIdx.x + k) * 2 + (k == 0 ? 1 : 0)) * kRows + r; };
-      float top = -INFINITY, sum = 0.f;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    const auto place = [&](int k) { return (static_cast<long long>(blockIdx.x + k) * 2 + (k == 0 ? 1 : 0)) * kRows + r; };
+    float top = -INFINITY, sum = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (row < p.rows) {
+#pragma unroll 4
       for (int k = part; k < cut.z; k += kParts) top = fmaxf(top, p.part_ml[place(k) * 2]);
+#pragma unroll 4
       for (int k = part; k < cut.z; k += kParts) {
         const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + place(k) * 2);
         const float4 y = *reinterpret_cast<const float4*>(p.part_o + place(k) * kD + d4 * 4);
-        if (ml.y == 0.f) continue;
-        const float f = ex2f(ml.x - top);
+        const float f = ml.y == 0.f ? 0.f : ex2f(ml.x - top);
         sum += ml.y * f;
         x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
       }
-      s_x[part][d4] = x;
-      if (d4 == 0) s_ml[part] = make_float2(top, sum);
-      __syncthreads();
-      if (part == 0) {
-        top = -INFINITY, sum = 0.f;
-        x = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    s_x[part][r][d4] = x;
+    if (d4 == 0) s_ml[part][r] = make_float2(top, sum);
+    __syncthreads();
+    if (part == 0 && row < p.rows) {
+      float all = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < kParts; ++k) top = fmaxf(top, s_ml[k].x);
+      for (int k = 0; k < kParts; ++k) all = fmaxf(all, s_ml[k][r].x);
+      x = make_float4(0.f, 0.f, 0.f, 0.f), sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < kParts; ++k) {
-          if (s_ml[k].y == 0.f) continue;
-          const float f = ex2f(s_ml[k].x - top);
-          const float4 y = s_x[k][d4];
-          sum += s_ml[k].y * f;
-          x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
-        }
-        store_row<kD, kInt8>(p, cut.x, h, row, d4, x, top, sum);
+      for (int k = 0; k < kParts; ++k) {
+        const float f = s_ml[k][r].y == 0.f ? 0.f : ex2f(s_ml[k][r].x - all);
+        const float4 y = s_x[k][r][d4];
+        sum += s_ml[k][r].y * f;
+        x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
       }
+      store_row<kD, kInt8>(p, cut.x, h, row, d4, x, all, sum);
     }
   }
-  if (blockIdx.y == 0)
-    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-      if (seq_tiles(p, b).n > 0) continue;
-      for (int row = part; row < p.rows * p.c.hkv; row += kParts)
-        store_row<kD, kInt8>(p, b, row / p.rows, row % p.rows, d4, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
-    }
+  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+    if (seq_tiles(p, b).n > 0) continue;
+    for (int row = threadIdx.x / (kD / 4); row < p.rows * p.c.hkv; row += kJoin / (kD / 4))
+      store_row<kD, kInt8>(p, b, row / p.rows, row % p.rows, d4, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
+  }
 }
 
 // Adds every visible slot's softmax weights up, from the scores that the first kernel kept and the final log-sum-exp.
 // One CTA per (sequence, head) and kWeightTiles tiles.
 constexpr int kWeightTiles = 16;
 template <int kNT>
-__global__ void __launch_bounds__(kJoin) cache_weights_kernel(const __grid_constant__ AttnKernelParams p, int chunks) {
+__global__ void __launch_bounds__(kAdd) cache_weights_kernel(const __grid_constant__ AttnKernelParams p, int chunks) {
   constexpr int kRows = 8 * kNT;
   extern __shared__ float s_lse[];  // [row_tiles * kRows], base 2; +inf for rows that see nothing and rows behind the last
   griddep_wait();
@@ -679,7 +677,7 @@ __global__ void __launch_bounds__(kJoin) cache_weights_kernel(const __grid_const
   const SeqTiles s = seq_tiles(p, b);
   const int t0 = (blockIdx.x - bh * chunks) * kWeightTiles;
   if (t0 >= s.n) return;
-  for (int r = threadIdx.x; r < p.row_tiles * kRows; r += kJoin) {
+  for (int r = threadIdx.x; r < p.row_tiles * kRows; r += kAdd) {
     float x = INFINITY;
     if (r < p.rows) {
       const int i = r / p.group;
@@ -691,7 +689,7 @@ __global__ void __launch_bounds__(kJoin) cache_weights_kernel(const __grid_const
   __syncthreads();
   const long long first = p.first[b] + static_cast<long long>(h) * p.row_tiles * s.n;
   const int t1 = min(t0 + kWeightTiles, s.n);
-  for (int k = t0 * kTok + threadIdx.x; k < t1 * kTok; k += kJoin) {
+  for (int k = t0 * kTok + threadIdx.x; k < t1 * kTok; k += kAdd) {
     const int tile = k / kTok, tok = tile_slot(s, tile) + k % kTok;
     if (tok >= s.len) continue;
     float sum = 0.f;
@@ -710,7 +708,7 @@ __global__ void __launch_bounds__(kJoin) cache_weights_kernel(const __grid_const
 }
 
 struct Plan {
-  int nt, row_tiles, ctas;
+  int nt, row_tiles, groups, ctas;
   long long most_tiles;  // of a sequence, per head and row tile
   int64_t o_bytes, ml_bytes, cut_bytes, first_bytes, score_bytes;
   int64_t total() const { return o_bytes + ml_bytes + cut_bytes + first_bytes + score_bytes; }
@@ -736,12 +734,13 @@ int make_plan(const rswa_cache_attn_params_t& a, Plan& plan) {
     return RSWA_E_UNSUPPORTED;
   }
   plan.row_tiles = static_cast<int>(row_tiles);
-  const long long share = items * most / kMinShare;
-  const int sms = sm_count();
-  plan.ctas = static_cast<int>(share < 1 ? 1 : share < sms ? share : sms);
-  plan.o_bytes = 2LL * plan.ctas * per_tile * a.cache.head_dim * 4;
-  plan.ml_bytes = (2LL * plan.ctas * per_tile * 2 * 4 + 255) / 256 * 256;
-  plan.cut_bytes = (plan.ctas * 16LL + 255) / 256 * 256;
+  const long long shares = items * most / kMinShare;
+  const int sms = sm_count(), per_sm = plan.nt == 1 ? Layout<128, 1>::kGroups : Layout<128, 2>::kGroups;
+  plan.groups = static_cast<int>(shares < 1 ? 1 : shares < sms * per_sm ? shares : sms * per_sm);
+  plan.ctas = plan.groups < sms ? plan.groups : sms;
+  plan.o_bytes = 2LL * plan.groups * per_tile * a.cache.head_dim * 4;
+  plan.ml_bytes = (2LL * plan.groups * per_tile * 2 * 4 + 255) / 256 * 256;
+  plan.cut_bytes = (plan.groups * 16LL + 255) / 256 * 256;
   plan.first_bytes = a.weights != nullptr ? (a.table.batch * 8LL + 255) / 256 * 256 : 0;
   plan.score_bytes = a.weights != nullptr ? items * most * kTok * per_tile * 4 : 0;
   return RSWA_OK;
@@ -784,15 +783,14 @@ cudaError_t launch_attn(const AttnKernelParams& kp, const Plan& plan, cudaStream
   }
   e = launch_kernel(kern, dim3(plan.ctas), Layout<kD, kNT>::kThreads, smem, s, true, kp);
   if (e != cudaSuccess) return e;
-  const int blocks = plan.ctas > kp.batch ? plan.ctas : kp.batch < sm_count() ? kp.batch : sm_count();
-  const int most_rows = plan.row_tiles > 1 ? 8 * kNT : kp.rows;
-  e = launch_kernel(cache_join_kernel<kD, kNT, kInt8>, dim3(blocks, most_rows), kJoin, 0, s, true, kp);
+  const int blocks = plan.groups > kp.batch ? plan.groups : kp.batch < sm_count() ? kp.batch : sm_count();
+  e = launch_kernel(cache_join_kernel<kD, kNT, kInt8>, dim3(blocks), kJoin, 0, s, true, kp);
   if (e != cudaSuccess) return e;
   count_launches(2);
   if (kp.weights != nullptr && plan.most_tiles > 0) {
     const long long chunks = (plan.most_tiles + kWeightTiles - 1) / kWeightTiles;
     const dim3 grid(static_cast<unsigned>(static_cast<long long>(kp.batch) * kp.c.hkv * chunks));
-    e = launch_kernel(cache_weights_kernel<kNT>, grid, kJoin, plan.row_tiles * 8 * kNT * 4, s, true, kp, static_cast<int>(chunks));
+    e = launch_kernel(cache_weights_kernel<kNT>, grid, kAdd, plan.row_tiles * 8 * kNT * 4, s, true, kp, static_cast<int>(chunks));
     if (e != cudaSuccess) return e;
     count_launches(1);
   }
@@ -877,7 +875,7 @@ extern "C" int rswa_cache_attn(const rswa_cache_attn_params_t* p, void* stream) 
   kp.scores = p->weights != nullptr ? reinterpret_cast<float*>(ws + plan.first_bytes) : nullptr;
   kp.weights = p->weights;
   kp.w_sb = p->w_stride_b, kp.w_sh = p->w_stride_h;
-  kp.ctas = plan.ctas;
+  kp.groups = plan.groups;
   kp.status = p->status;
   kp.mirror = status_mirror(p->status);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
