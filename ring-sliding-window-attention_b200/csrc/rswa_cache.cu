@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const __grid_con
   const float need = scale_for<kInt8>(amax);
   const bool grows = first == 0 || need > before || need != need;
   const float after = grows ? need : before;
+  const bool poisoned = after != after;
   const float inv = 1.f / after;
   uint8_t* const dst = p.c.data[which] + (static_cast<long long>(page) * p.c.hkv + h) * bs * kD;
   if (threadIdx.x == 0 && grows) *scale_at = after;
@@ -135,7 +136,9 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const __grid_con
   for (int i = 0; i < kPasses; ++i) {
     const int at = i * kThreads + threadIdx.x, row = at / kCols;
     uint2* const to = reinterpret_cast<uint2*>(dst) + at;
-    if (row >= first && row < end) {
+    if (poisoned) {
+      if (row < end) *to = make_uint2(0, 0);
+    } else if (row >= first && row < end) {
       const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
       float2 f[4];
 #pragma unroll

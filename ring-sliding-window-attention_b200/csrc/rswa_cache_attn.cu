@@ -11,8 +11,8 @@
 // group of up to 8 rows wastes nothing on the operand that costs: the one converted from bytes.  (tcgen05 wants 128
 // rows of A, both operands in the same 8-bit or 16-bit type in shared memory: the bytes would have to be converted and
 // written back there, or the queries and weights rounded to 8 bits.)  A word of four stored bytes becomes two operand
-// registers in place: bytes 0, 2 and bytes 1, 3.  For K the order of the head dimension inside a product is free (the
-// queries are laid out the same way); for V the two registers are two columns of the head, whose weights are the same.
+// registers in place.  For K the order of the head dimension inside a product is free (the queries are laid out the
+// same way); for V the two registers are two columns of the head, whose weights are the same.
 //   S^T[token][row] = K q^T        ldmatrix: lane (g, c) of a quad layout holds d = 16 s + 4c .. 4c + 3 of token g
 //   O^T[d][row]    += V^T P^T      ldmatrix.trans: lane holds d = 16 m + 2g, 2g + 1 of tokens 2c, 2c + 1
 // P^T comes out of S^T's accumulators by two 8x8 transposes (movmatrix) per 16 tokens.
@@ -247,7 +247,7 @@ __device__ __forceinline__ void sync_group(int group) { asm volatile("bar.sync %
 template <int kD, bool kInt8>
 __device__ __forceinline__ void store_row(const AttnKernelParams& p, int b, int h, int row, int d4, float4 x, float top, float sum) {
   const int i = row / p.group, hd = h * p.group + row - i * p.group;
-  const float inv = sum == 0.f ? 0.f : kHalfFactor<kInt8> / sum;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint16_t* const to = p.out + ((static_cast<long long>(b) * p.q_len + i) * p.hq + hd) * kD + d4 * 4;
   *reinterpret_cast<uint2*>(to) = p.bf16 ? make_uint2(pack2<true>(x.x * inv, x.y * inv), pack2<true>(x.z * inv, x.w * inv))
                                          : make_uint2(pack2<false>(x.x * inv, x.y * inv), pack2<false>(x.z * inv, x.w * inv));
@@ -355,8 +355,8 @@ __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_ker
 #pragma unroll
         for (int s = 0; s < kKS; ++s) {
           const uint2 x = *reinterpret_cast<const uint2*>(src + s * 16);
-          qf[nt][s][0] = __byte_perm(x.x, x.y, 0x5410);  // elements 0, 2
-          qf[nt][s][1] = __byte_perm(x.x, x.y, 0x7632);  // elements 1, 3
+          qf[nt][s][0] = x.x;
+          qf[nt][s][1] = x.y;
         }
         factor = 1.f;
       } else {
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_ker
           }
         factor *= __uint_as_float(static_cast<uint32_t>(e - 14) << 23);
       }
-      factor *= p.scale_log2 * kHalfFactor<kInt8>;
+      factor *= p.scale_log2;
       rs[nt][0] = __shfl_sync(0xffffffffu, factor, c * 8);
       rs[nt][1] = __shfl_sync(0xffffffffu, factor, c * 8 + 4);
     }
@@ -430,7 +430,7 @@ __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_ker
         uint32_t w[4], lo[4], hi[4];
         ldsm4(w, piece<kD>(k_base, lane, s));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) to_half2<kInt8>(w[k], lo[k], hi[k]);
+        for (int k = 0; k < 4; ++k) to_half2<kInt8, true>(w[k], lo[k], hi[k]);
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) {
           mma16816(acc[0][nt], lo[0], lo[1], hi[0], hi[1], qf[nt][s][0], qf[nt][s][1]);
@@ -521,12 +521,19 @@ __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_ker
       }
       // ---- output
       if (!dead) dead = !mbar_wait_w(full + 1, own_i & 1, &ctl.err, kErrWaitProducer);
+      if (!kInt8 && slot + kTok > cc.s.len) {
+        // the slots behind the last token hold anything: a weight of 0 does not take a NaN away
+        if (slot + lane >= cc.s.len)
+          for (int k = 0; k < kD / 16; ++k) *reinterpret_cast<uint4*>(own + R::kTileBytes + lane * kD + k * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();  // (the next load of V comes behind these stores)
+        __syncwarp();
+      }
 #pragma unroll
       for (int s = 0; s < kKS; ++s) {
         uint32_t w[4], lo[4], hi[4];
         ldsm4_t(w, piece<kD>(v_base, lane, s));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) to_half2<kInt8>(w[k], lo[k], hi[k]);
+        for (int k = 0; k < 4; ++k) to_half2<kInt8, false>(w[k], lo[k], hi[k]);
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) {
           mma16816(o[nt][s], lo[0], hi[0], lo[1], hi[1], pf[0][nt][0], pf[0][nt][1]);

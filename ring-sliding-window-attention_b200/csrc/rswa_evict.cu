@@ -236,11 +236,12 @@ __global__ void __launch_bounds__(kPack) evict_pack_kernel(const __grid_constant
     const int at = i * kPack + threadIdx.x, row = at / kCols;
     if (row >= rows) continue;
     const float scale = s_scale[row];
+    if (after != after) x[i] = make_uint4(0, 0, 0, 0);
     uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const float4 f = to_float4<kInt8>(w[k]);
-      w[k] = to_bytes<kInt8>(f.x * scale * inv, f.y * scale * inv, f.z * scale * inv, f.w * scale * inv);
+      if (after == after) w[k] = to_bytes<kInt8>(f.x * scale * inv, f.y * scale * inv, f.z * scale * inv, f.w * scale * inv);
     }
     dst[at] = make_uint4(w[0], w[1], w[2], w[3]);
   }
