@@ -358,7 +358,10 @@ int rswa_cache_read(const rswa_cache_read_params_t* p, void* stream);
  * zero row and lse -inf.
  * weights (or NULL): float [batch, n_kv_heads, >= max_blocks * block_size], tokens contiguous; every slot seen has
  * the softmax weights added that it got from the queries and heads of its key/value head.  Needs lse.
- * `workspace`: rswa_cache_attn_workspace_bytes() of device memory, 256-byte aligned, for the time of the call. */
+ * `workspace`: rswa_cache_attn_workspace_bytes() of device memory, 256-byte aligned, for the time of the call.
+ * `arrived`: RSWA_CACHE_ATTN_COUNTERS ints of device memory that are 0 before the call and are 0 again behind it; calls
+ * that may overlap on the GPU (other streams, a captured graph beside anything else) need one each. */
+#define RSWA_CACHE_ATTN_COUNTERS 1024
 typedef struct rswa_cache_attn_params {
   rswa_cache_t cache;
   rswa_block_table_t table;
@@ -375,6 +378,7 @@ typedef struct rswa_cache_attn_params {
   int64_t w_stride_b, w_stride_h;
   void* workspace;
   int64_t workspace_bytes;
+  int32_t* arrived;
   int32_t* status;
 } rswa_cache_attn_params_t;
 

@@ -23,12 +23,14 @@
 // the sum of the weights takes it back out.  Scores, sums and the output are 32-bit.
 //
 // Work: the 32-token tiles of all (sequence, key/value head, 8 or 16 query rows) in one order, cut evenly whatever the
-// lengths over groups of four warps (one CTA of three or four groups per SM).  The warps of a group take its tiles in turn and
-// add up at the end of each piece; groups rather than CTAs because the end of a piece and the next one's queries cost every
-// warp that takes part as much as several tiles.  Every warp loads for itself: K of its next tile as soon as the scores are
-// formed, V as soon as the output is, on over sequence boundaries; its lanes look 32 tiles up in the block table at a
-// time, so that the table's latency is paid once for all of them.  A piece that is not a whole (sequence, head) goes to
-// the workspace and a second kernel joins the pieces in order: results do not depend on timing.
+// lengths over groups of warps.  The warps of a group take its tiles in turn and add up at the end of each piece.  Where there
+// are more (sequence, head, row tile)s than SMs a group is four warps, because the end of a piece and the next one's queries
+// cost every warp that takes part as much as several tiles (32 requests of 300 to 8192 tokens, 8 heads: 48 us, and 69 with
+// all 16 warps of an SM in one group); else it is all warps of the SM, which leaves fewer pieces to join.
+// Every warp loads for itself: K of its next tile as soon as the scores are formed, V as soon as the output is, on over
+// sequence boundaries; its lanes look 32 tiles up in the block table at a time, so that the table's latency is paid once for
+// all of them.  The pieces of an item that is cut go to the workspace, and the group that delivers the last one joins them,
+// in order: results do not depend on timing.
 #include <atomic>
 
 #include "rswa_cache.cuh"
@@ -44,9 +46,7 @@ namespace {
 
 constexpr int kTok = 32;     // tokens of a tile
 constexpr int kScan = 256;   // threads of the prefix sums over sequences
-constexpr int kGroup = 4;    // warps that share the work of a piece
-constexpr int kMinShare = 4; // tiles of a group at least
-constexpr int kJoin = 1024, kAdd = 256;  // threads of the kernels behind the first one
+constexpr int kAdd = 256;    // threads of a CTA that adds weights up
 constexpr float kRoom = 14.f;  // a weight may grow to 2^14 before the reference is raised (fp16 ends at 2^16)
 constexpr float kLow = 4.f;    // and is raised to the maximum minus 4, so that not every new maximum raises it
 
@@ -67,9 +67,9 @@ struct AttnKernelParams {
   float* lse;        // or null
   float* part_o;     // [groups][2][8 * kNT][head_dim]
   float* part_ml;    // [groups][2][8 * kNT][2]
-  int4* cut;         // [groups]: an item whose first piece is the group's last one: sequence, head * row tiles + row tile, pieces (or 0)
+  int* arrived;      // [groups], 0 between calls: pieces of the item that a group begins and does not finish
   float* scores;     // [tiles][kTok][8 * kNT], or null: what the weights need
-  long long* first;  // [batch]: index of a sequence's first tile, with scores
+  int* first;        // [batch]: index of a sequence's first tile, with scores
   float* weights;
   long long w_sb, w_sh;
   int groups;
@@ -98,17 +98,27 @@ __device__ __forceinline__ SeqTiles seq_tiles(const AttnKernelParams& p, int b) 
 }
 __device__ __forceinline__ int tile_slot(const SeqTiles& s, int i) { return (i < s.n_sink_tiles ? i : s.first + i - s.n_sink_tiles) * kTok; }
 
-// Where the work of a group begins and ends: equal shares of all tiles, none of fewer than kMinShare.
-__device__ __forceinline__ long long n_shares(long long total, int groups) { return min(static_cast<long long>(groups), max(1LL, total / kMinShare)); }
-__device__ __forceinline__ long long share_begin(long long total, long long shares, long long c) { return total * c / shares; }
-__device__ __forceinline__ long long share_of(long long total, long long shares, long long tile) { return ((tile + 1) * shares - 1) / total; }
+// Where the work of a group begins and ends: equal shares of all tiles, none of fewer than a tile per warp.
+struct Shares {
+  int n, each, more;  // `more` shares have each + 1 tiles, the others each
+  __device__ __forceinline__ Shares(int total, int groups, int least) {
+    n = min(groups, max(1, total / least));
+    each = total / n;
+    more = total - each * n;
+  }
+  __device__ __forceinline__ int begin(int c) const { return c * each + min(c, more); }
+  __device__ __forceinline__ int of(int tile) const {
+    const int large = more * (each + 1);
+    return tile < large ? tile / (each + 1) : more + (tile - large) / each;
+  }
+};
 
 // Prefix sums of the sequences' tiles (per key/value head and row tile): thread i of the first kScan holds `per`
 // sequences.  s_prefix[i]: tiles in front of thread i's sequences; s_prefix[kScan]: all.
-__device__ __forceinline__ void tile_prefix(const AttnKernelParams& p, long long* s_prefix, long long* s_warp) {
+__device__ __forceinline__ void tile_prefix(const AttnKernelParams& p, int* s_prefix, int* s_warp) {
   const int per = (p.batch + kScan - 1) / kScan;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long mine = 0, sum = 0;
+  int mine = 0, sum = 0;
   if (threadIdx.x < kScan) {
     for (int i = 0; i < per; ++i) {
       const int b = threadIdx.x * per + i;
@@ -117,20 +127,20 @@ __device__ __forceinline__ void tile_prefix(const AttnKernelParams& p, long long
     sum = mine;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
-      const long long o = __shfl_up_sync(0xffffffffu, sum, d);
+      const int o = __shfl_up_sync(0xffffffffu, sum, d);
       if (lane >= d) sum += o;
     }
     if (lane == 31) s_warp[warp] = sum;
   }
   __syncthreads();
   if (threadIdx.x < kScan) {
-    long long before = 0;
+    int before = 0;
     for (int w = 0; w < warp; ++w) before += s_warp[w];
     before += sum - mine;
     s_prefix[threadIdx.x] = before;
     if (threadIdx.x == kScan - 1) s_prefix[kScan] = before + mine;
     if (p.first != nullptr && blockIdx.x == 0) {
-      const long long items = static_cast<long long>(p.c.hkv) * p.row_tiles;
+      const int items = p.c.hkv * p.row_tiles;
       for (int i = 0; i < per; ++i) {
         const int b = threadIdx.x * per + i;
         if (b >= p.batch) break;
@@ -146,12 +156,12 @@ __device__ __forceinline__ void tile_prefix(const AttnKernelParams& p, long long
 struct Cursor {
   int b, item, i;       // item = head * row_tiles + row tile
   SeqTiles s;
-  long long at;         // index among all tiles
+  int at;         // index among all tiles
   // moves forward by n tiles; false: behind the last
-  __device__ __forceinline__ void skip(const AttnKernelParams& p, long long n, long long end) {
+  __device__ __forceinline__ void skip(const AttnKernelParams& p, int n, int end) {
     at += n;
     if (at >= end) return;
-    long long k = i + n;
+    int k = i + n;
     const int items = p.c.hkv * p.row_tiles;
     while (k >= s.n) {
       k -= s.n;
@@ -160,11 +170,11 @@ struct Cursor {
         do s = seq_tiles(p, ++b); while (s.n == 0);
       }
     }
-    i = static_cast<int>(k);
+    i = k;
   }
 };
-__device__ __forceinline__ Cursor cursor_at(const AttnKernelParams& p, const long long* s_prefix, long long tile) {
-  const long long items = static_cast<long long>(p.c.hkv) * p.row_tiles;
+__device__ __forceinline__ Cursor cursor_at(const AttnKernelParams& p, const int* s_prefix, int tile) {
+  const int items = p.c.hkv * p.row_tiles;
   const int per = (p.batch + kScan - 1) / kScan;
   int lo = 0, hi = kScan - 1;  // the last thread whose prefix is not behind the tile
   while (lo < hi) {
@@ -176,14 +186,14 @@ __device__ __forceinline__ Cursor cursor_at(const AttnKernelParams& p, const lon
   Cursor c;
   c.at = tile;
   c.b = lo * per;
-  long long rest = tile - s_prefix[lo] * items;
+  int rest = tile - s_prefix[lo] * items;
   c.s = seq_tiles(p, c.b);
   while (rest >= c.s.n * items) {
     rest -= c.s.n * items;
     c.s = seq_tiles(p, ++c.b);
   }
-  c.item = static_cast<int>(rest / c.s.n);
-  c.i = static_cast<int>(rest % c.s.n);
+  c.item = rest / c.s.n;
+  c.i = rest - c.item * c.s.n;
   return c;
 }
 
@@ -195,16 +205,18 @@ struct Ring {
 
 // 16 warps of 128 registers a thread, or for 16 query rows 12 of 168.  A tile in flight per warp is 96 KB or more, where
 // the latency of a load asks for about 50.
-template <int kD, int kNT>
+// kAll: all warps are one group.
+template <int kD, int kNT, bool kAll>
 struct Layout {
   static constexpr int kWarps = kNT == 1 ? 16 : 12;
-  static constexpr int kThreads = kWarps * 32, kGroups = kWarps / kGroup;
+  static constexpr int kThreads = kWarps * 32, kGroup = kAll ? kWarps : 4, kGroups = kWarps / kGroup;
   struct Ctl {
     uint64_t full[kWarps][2];           // K, V
     float4 scale[kWarps][32][2];        // the looked-up tiles: of the first 16 tokens and the last 16 K's scale, log2 of V's, 1 / V's
     int2 row[kWarps][32];               // and where their K and V lie
     float ml[kWarps][8 * kNT][2];       // reference and sum of every warp's piece
-    long long prefix[kScan + 1 + kScan / 32];
+    int prefix[kScan + 1 + kScan / 32];
+    int last[kGroups];                  // whether the group's piece was the last one to arrive
     int err;
   };
   static constexpr int kRings = kWarps * Ring<kD>::kStageBytes;
@@ -242,9 +254,12 @@ __device__ __forceinline__ uint32_t piece(uint32_t base, int row, int chunk) {
   return base + row * kD + ((kD == 128 ? chunk ^ (row & 7) : chunk ^ ((row >> 1) & 3)) << 4);
 }
 
-__device__ __forceinline__ void sync_group(int group) { asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(kGroup * 32) : "memory"); }
+template <int kThreads>
+__device__ __forceinline__ void sync_group(int group) {
+  asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(kThreads) : "memory");
+}
 // four elements of a finished row, and its log-sum-exp
-template <int kD, bool kInt8>
+template <int kD>
 __device__ __forceinline__ void store_row(const AttnKernelParams& p, int b, int h, int row, int d4, float4 x, float top, float sum) {
   const int i = row / p.group, hd = h * p.group + row - i * p.group;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -255,12 +270,69 @@ __device__ __forceinline__ void store_row(const AttnKernelParams& p, int b, int 
     p.lse[(static_cast<long long>(b) * p.hq + hd) * p.q_len + i] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.6931471805599453f;
 }
 
+// The rows of the sequences that have nothing to attend to, by the first kPeers threads of every CTA.
+template <int kD, int kPeers>
+__device__ __forceinline__ void empty_rows(const AttnKernelParams& p) {
+  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+    if (seq_tiles(p, b).n > 0) continue;
+    for (int row = threadIdx.x / (kD / 4); row < p.rows * p.c.hkv; row += kPeers / (kD / 4))
+      store_row<kD>(p, b, row / p.rows, row % p.rows, threadIdx.x % (kD / 4), make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
+  }
+}
+
+// Joins the pieces of an item in the order of the groups `lo` to lo + pieces - 1 that worked on it; by the kPeers threads
+// of one group.  With more threads than a row tile has 16-byte parts the pieces are dealt out to several of them, whose sums
+// are added in order.  (The other groups' pieces are read past L1, which does not see what other SMs write.)
+template <int kD, int kNT, int kPeers>
+__device__ __forceinline__ void join_pieces(const AttnKernelParams& p, float* merge, int group, int b, int h, int row0, int lo, int pieces) {
+  constexpr int kRows = 8 * kNT, kUnits = kRows * kD / 4, kParts = kPeers >= 2 * kUnits ? kPeers / kUnits : 1;
+  const int t = threadIdx.x - group * kPeers;
+  const int part = kParts > 1 ? t / kUnits : 0;
+  float4* const s_x = reinterpret_cast<float4*>(merge);                              // [kParts][kUnits]
+  float2* const s_ml = reinterpret_cast<float2*>(merge + kParts * kUnits * 4);       // [kParts][kRows]
+  for (int u = kParts > 1 ? t % kUnits : t; u < kUnits; u += kParts > 1 ? kUnits : kPeers) {
+    const int r = u / (kD / 4), d4 = u % (kD / 4), row = row0 + r;
+    const auto place = [&](int k) { return (static_cast<long long>(lo + k) * 2 + (k == 0 ? 1 : 0)) * kRows + r; };
+    float top = -INFINITY, sum = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    const auto add = [&](float m, float l, float4 y) {  // a later piece
+      const float next = fmaxf(top, m);
+      const float f = sum == 0.f ? 0.f : ex2f(top - next), w = l == 0.f ? 0.f : ex2f(m - next);
+      top = next;
+      sum = sum * f + l * w;
+      x.x = x.x * f + y.x * w, x.y = x.y * f + y.y * w, x.z = x.z * f + y.z * w, x.w = x.w * f + y.w * w;
+    };
+    if (row < p.rows && part < kParts) {
+#pragma unroll 4
+      for (int k = part; k < pieces; k += kParts) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + place(k) * 2));
+        add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(p.part_o + place(k) * kD + d4 * 4)));
+      }
+      if (kParts == 1) store_row<kD>(p, b, h, row, d4, x, top, sum);
+    }
+    if (kParts > 1) {
+      s_x[part * kUnits + u] = x;
+      if (d4 == 0) s_ml[part * kRows + r] = make_float2(top, sum);
+      sync_group<kPeers>(group);
+      if (part == 0 && row < p.rows) {
+#pragma unroll
+        for (int k = 1; k < kParts; ++k) {
+          const float2 ml = s_ml[k * kRows + r];
+          add(ml.x, ml.y, s_x[k * kUnits + u]);
+        }
+        store_row<kD>(p, b, h, row, d4, x, top, sum);
+      }
+      sync_group<kPeers>(group);  // (before the next piece's sums)
+    }
+  }
+}
+
 // kNT: query rows in columns of 8.
-template <int kD, int kNT, bool kInt8>
-__global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_kernel(const __grid_constant__ AttnKernelParams p) {
-  using L = Layout<kD, kNT>;
+template <int kD, int kNT, bool kInt8, bool kAll>
+__global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_attn_kernel(const __grid_constant__ AttnKernelParams p) {
+  using L = Layout<kD, kNT, kAll>;
   using R = Ring<kD>;
-  constexpr int kKS = kD / 16;
+  constexpr int kKS = kD / 16, kGroup = L::kGroup, kPeers = kGroup * 32;
   constexpr int kRows = 8 * kNT;
   extern __shared__ __align__(1024) uint8_t smem[];
   auto& ctl = *reinterpret_cast<typename L::Ctl*>(smem + L::kRings + L::kMerge);
@@ -283,19 +355,19 @@ __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_ker
   mbar_fence_init();
   griddep_wait();
   tile_prefix(p, ctl.prefix, ctl.prefix + kScan + 1);
-  const long long total = ctl.prefix[kScan] * p.c.hkv * p.row_tiles;
-  const long long shares = n_shares(total, p.groups);
-  if (me >= shares || total == 0) {
-    if (me < p.groups && threadIdx.x % (kGroup * 32) == 0) p.cut[me] = make_int4(0, 0, 0, 0);
+  const int total = ctl.prefix[kScan] * p.c.hkv * p.row_tiles;
+  const Shares shares(total, p.groups, kGroup);
+  if (me >= shares.n || total == 0) {
+    if (group == 0) empty_rows<kD, kPeers>(p);
     return;
   }
-  const long long begin = share_begin(total, shares, me), end = share_begin(total, shares, me + 1);
+  const int begin = shares.begin(me), end = shares.begin(me + 1);
   const int box = min(p.c.bs, kTok);
 
   // The tiles of this warp, counted: tile i is the share's tile wg + i * kGroup.  Looks 32 of them up, one a lane.
-  const int n_own = static_cast<int>((end - begin - wg + kGroup - 1) / kGroup);
+  const int n_own = (end - begin - wg + kGroup - 1) / kGroup;
   auto look_up = [&](int i) {
-    const long long at = begin + wg + static_cast<long long>(i + lane) * kGroup;
+    const int at = begin + wg + (i + lane) * kGroup;
     __syncwarp();
     if (at < end) {
       const Cursor lc = cursor_at(p, ctl.prefix, at);
@@ -340,7 +412,7 @@ __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_ker
   int own_i = 0;  // this warp's next tile
   bool dead = false;
   while (cc.at < end) {
-    const long long piece_end = min(end, cc.at + cc.s.n - cc.i);
+    const int piece_end = min(end, cc.at + cc.s.n - cc.i);
     const int h = cc.item / p.row_tiles, row0 = (cc.item - h * p.row_tiles) * kRows;
     // the queries of this piece as operands: row g of each column block, d = 16 s + 4c .. 4c + 3
     uint32_t qf[kNT][kKS][2];
@@ -413,10 +485,10 @@ __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_ker
       l[nt][0] = l[nt][1] = 0.f;
     }
     // this warp's tiles of the piece: those whose index from `begin` is `wg` modulo kGroup
-    for (long long at = begin + wg + static_cast<long long>(own_i) * kGroup; at < piece_end; at += kGroup) {
+    for (int at = begin + wg + own_i * kGroup; at < piece_end; at += kGroup) {
       const float4 sc0 = ctl.scale[warp][own_i & 31][0], sc1 = ctl.scale[warp][own_i & 31][1];
       if (!dead) dead = !mbar_wait_w(full, own_i & 1, &ctl.err, kErrWaitProducer);
-      const int slot = tile_slot(cc.s, cc.i + static_cast<int>(at - cc.at));
+      const int slot = tile_slot(cc.s, cc.i + at - cc.at);
       const uint32_t k_base = smem_u32(own), v_base = k_base + R::kTileBytes;
       const float sk[2] = {sc0.x, sc1.x}, lv[2] = {sc0.y, sc1.y}, iv[2] = {sc0.z, sc1.z};
       // ---- scores
@@ -462,7 +534,7 @@ __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_ker
             }
       }
       if (p.scores != nullptr) {
-        float* const to = p.scores + at * (kTok * kRows);
+        float* const to = p.scores + static_cast<long long>(at) * (kTok * kRows);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -570,10 +642,10 @@ __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_ker
         *reinterpret_cast<float2*>(mine + (2 * c) * kD + ((s * 16 + 2 * g) ^ (8 * c))) = make_float2(o[nt][s][0], o[nt][s][2]);
         *reinterpret_cast<float2*>(mine + (2 * c + 1) * kD + ((s * 16 + 2 * g) ^ (8 * c))) = make_float2(o[nt][s][1], o[nt][s][3]);
       }
-      sync_group(group);
-      const int t = threadIdx.x % (kGroup * 32), d4 = t % (kD / 4);
+      sync_group<kPeers>(group);
+      const int t = threadIdx.x - group * kPeers, d4 = t % (kD / 4);
 #pragma unroll
-      for (int r = t / (kD / 4); r < 8; r += kGroup * 32 / (kD / 4)) {
+      for (int r = t / (kD / 4); r < 8; r += kPeers / (kD / 4)) {
         const int row = row0 + nt * 8 + r;
         float top = -INFINITY;
 #pragma unroll
@@ -591,7 +663,7 @@ __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_ker
         }
         if (row < p.rows) {
           if (whole) {
-            store_row<kD, kInt8>(p, cc.b, h, row, d4, x, top, sum);
+            store_row<kD>(p, cc.b, h, row, d4, x, top, sum);
           } else {
             const long long to = (static_cast<long long>(me) * 2 + (from_start ? 1 : 0)) * kRows + nt * 8 + r;
             *reinterpret_cast<float4*>(p.part_o + to * kD + d4 * 4) = x;
@@ -599,13 +671,22 @@ __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_ker
           }
         }
       }
-      sync_group(group);
+      sync_group<kPeers>(group);
     }
-    if (piece_end == end && wg == 0 && lane == 0) {
-      // (an item whose first piece this is and that goes on behind the share)
-      const long long first = cc.at - cc.i;
-      const int pieces = from_start && !to_end ? static_cast<int>(share_of(total, shares, first + cc.s.n - 1) - me + 1) : 0;
-      p.cut[me] = make_int4(cc.b, cc.item, pieces, 0);
+    if (!whole) {
+      // the group that delivers an item's last piece joins them all
+      const int first = cc.at - cc.i, lo = shares.of(first), pieces = shares.of(first + cc.s.n - 1) - lo + 1;
+      if (threadIdx.x == group * kPeers) {
+        __threadfence();
+        const int last = atomicAdd(p.arrived + lo, 1) == pieces - 1;
+        if (last) {
+          p.arrived[lo] = 0;
+          __threadfence();
+        }
+        ctl.last[group] = last;
+      }
+      sync_group<kPeers>(group);
+      if (ctl.last[group] != 0) join_pieces<kD, kNT, kPeers>(p, merge, group, cc.b, h, row0, lo, pieces);
     }
     cc.skip(p, piece_end - cc.at, end);
   }
@@ -616,60 +697,7 @@ __global__ void __launch_bounds__((Layout<kD, kNT>::kThreads), 1) cache_attn_ker
       for (int kv = 0; kv < 2; ++kv) mbar_wait(full + kv, loaded[kv] & 1, &own_err, kErrWaitProducer);
     if (lane == 0) raise_status(p.status, p.mirror, kErrWaitProducer);
   }
-}
-
-// Joins the pieces of every item that more than one group worked on, in the groups' order: block c the item that group c
-// began and did not finish.  A row's pieces are dealt out to several threads, whose sums are added in order.
-// And writes the rows of sequences that have nothing to attend to.
-template <int kD, int kNT, bool kInt8>
-__global__ void __launch_bounds__(kJoin) cache_join_kernel(const __grid_constant__ AttnKernelParams p) {
-  constexpr int kRows = 8 * kNT, kParts = kJoin / (kD / 4) / kRows;
-  __shared__ float4 s_x[kParts][kRows][kD / 4];
-  __shared__ float2 s_ml[kParts][kRows];
-  griddep_launch();
-  griddep_wait();
-  const int d4 = threadIdx.x % (kD / 4), r = threadIdx.x / (kD / 4) % kRows, part = threadIdx.x / (kD / 4) / kRows;
-  const int4 cut = blockIdx.x < p.groups ? p.cut[blockIdx.x] : make_int4(0, 0, 0, 0);
-  if (cut.z > 0) {
-    const int h = cut.y / p.row_tiles, row = (cut.y - h * p.row_tiles) * kRows + r;
-    const auto place = [&](int k) { return (static_cast<long long>(blockIdx.x + k) * 2 + (k == 0 ? 1 : 0)) * kRows + r; };
-    float top = -INFINITY, sum = 0.f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (row < p.rows) {
-#pragma unroll 4
-      for (int k = part; k < cut.z; k += kParts) top = fmaxf(top, p.part_ml[place(k) * 2]);
-#pragma unroll 4
-      for (int k = part; k < cut.z; k += kParts) {
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + place(k) * 2);
-        const float4 y = *reinterpret_cast<const float4*>(p.part_o + place(k) * kD + d4 * 4);
-        const float f = ml.y == 0.f ? 0.f : ex2f(ml.x - top);
-        sum += ml.y * f;
-        x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
-      }
-    }
-    s_x[part][r][d4] = x;
-    if (d4 == 0) s_ml[part][r] = make_float2(top, sum);
-    __syncthreads();
-    if (part == 0 && row < p.rows) {
-      float all = -INFINITY;
-#pragma unroll
-      for (int k = 0; k < kParts; ++k) all = fmaxf(all, s_ml[k][r].x);
-      x = make_float4(0.f, 0.f, 0.f, 0.f), sum = 0.f;
-#pragma unroll
-      for (int k = 0; k < kParts; ++k) {
-        const float f = s_ml[k][r].y == 0.f ? 0.f : ex2f(s_ml[k][r].x - all);
-        const float4 y = s_x[k][r][d4];
-        sum += s_ml[k][r].y * f;
-        x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
-      }
-      store_row<kD, kInt8>(p, cut.x, h, row, d4, x, all, sum);
-    }
-  }
-  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-    if (seq_tiles(p, b).n > 0) continue;
-    for (int row = threadIdx.x / (kD / 4); row < p.rows * p.c.hkv; row += kJoin / (kD / 4))
-      store_row<kD, kInt8>(p, b, row / p.rows, row % p.rows, d4, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
-  }
+  if (group == 0) empty_rows<kD, kPeers>(p);
 }
 
 // Adds every visible slot's softmax weights up, from the scores that the first kernel kept and the final log-sum-exp.
@@ -694,14 +722,14 @@ __global__ void __launch_bounds__(kAdd) cache_weights_kernel(const __grid_consta
     s_lse[r] = x;
   }
   __syncthreads();
-  const long long first = p.first[b] + static_cast<long long>(h) * p.row_tiles * s.n;
+  const int first = p.first[b] + h * p.row_tiles * s.n;
   const int t1 = min(t0 + kWeightTiles, s.n);
   for (int k = t0 * kTok + threadIdx.x; k < t1 * kTok; k += kAdd) {
     const int tile = k / kTok, tok = tile_slot(s, tile) + k % kTok;
     if (tok >= s.len) continue;
     float sum = 0.f;
     for (int rt = 0; rt < p.row_tiles; ++rt) {
-      const float4* from = reinterpret_cast<const float4*>(p.scores + ((first + static_cast<long long>(rt) * s.n + tile) * kTok + k % kTok) * kRows);
+      const float4* from = reinterpret_cast<const float4*>(p.scores + (static_cast<long long>(first + rt * s.n + tile) * kTok + k % kTok) * kRows);
 #pragma unroll
       for (int v = 0; v < kRows / 4; ++v) {
         const float4 x = from[v];
@@ -716,9 +744,10 @@ __global__ void __launch_bounds__(kAdd) cache_weights_kernel(const __grid_consta
 
 struct Plan {
   int nt, row_tiles, groups, ctas;
+  bool all;  // all warps of a CTA are one group
   long long most_tiles;  // of a sequence, per head and row tile
-  int64_t o_bytes, ml_bytes, cut_bytes, first_bytes, score_bytes;
-  int64_t total() const { return o_bytes + ml_bytes + cut_bytes + first_bytes + score_bytes; }
+  int64_t o_bytes, ml_bytes, first_bytes, score_bytes;
+  int64_t total() const { return o_bytes + ml_bytes + first_bytes + score_bytes; }
 };
 
 // kNT = 1 up to 8 query rows per key/value head, else row tiles of 16.
@@ -736,19 +765,20 @@ int make_plan(const rswa_cache_attn_params_t& a, Plan& plan) {
   plan.most_tiles = most;
   const long long items = static_cast<long long>(a.table.batch) * a.cache.n_kv_heads * row_tiles;
   // (a row tile's log-sum-exps lie in shared memory while the weights are added up)
-  if (row_tiles > 512 || items > 0x7fffffffLL || items * ((most + kWeightTiles - 1) / kWeightTiles) > 0x7fffffffLL) {
+  if (row_tiles > 512 || items > 0x7fffffffLL || items * most > 0x7fffffffLL) {
     set_error("rswa_cache_attn: too many queries in one call");
     return RSWA_E_UNSUPPORTED;
   }
   plan.row_tiles = static_cast<int>(row_tiles);
-  const long long shares = items * most / kMinShare;
-  const int sms = sm_count(), per_sm = plan.nt == 1 ? Layout<128, 1>::kGroups : Layout<128, 2>::kGroups;
-  plan.groups = static_cast<int>(shares < 1 ? 1 : shares < sms * per_sm ? shares : sms * per_sm);
+  const int sms = sm_count(), warps = plan.nt == 1 ? Layout<128, 1, true>::kWarps : Layout<128, 2, true>::kWarps;
+  plan.all = items <= sms;
+  const long long shares = items * most / (plan.all ? warps : 4), most_groups = plan.all ? sms : static_cast<long long>(sms) * warps / 4;
+  plan.groups = static_cast<int>(shares < 1 ? 1 : shares < most_groups ? shares : most_groups);
+  if (plan.groups > RSWA_CACHE_ATTN_COUNTERS) plan.groups = RSWA_CACHE_ATTN_COUNTERS;
   plan.ctas = plan.groups < sms ? plan.groups : sms;
   plan.o_bytes = 2LL * plan.groups * per_tile * a.cache.head_dim * 4;
   plan.ml_bytes = (2LL * plan.groups * per_tile * 2 * 4 + 255) / 256 * 256;
-  plan.cut_bytes = (plan.groups * 16LL + 255) / 256 * 256;
-  plan.first_bytes = a.weights != nullptr ? (a.table.batch * 8LL + 255) / 256 * 256 : 0;
+  plan.first_bytes = a.weights != nullptr ? (a.table.batch * 4LL + 255) / 256 * 256 : 0;
   plan.score_bytes = a.weights != nullptr ? items * most * kTok * per_tile * 4 : 0;
   return RSWA_OK;
 }
@@ -775,25 +805,27 @@ int check_attn(const rswa_cache_attn_params_t* p) {
   return RSWA_OK;
 }
 
-template <int kD, int kNT, bool kInt8>
-cudaError_t launch_attn(const AttnKernelParams& kp, const Plan& plan, cudaStream_t s) {
-  const auto kern = cache_attn_kernel<kD, kNT, kInt8>;
-  constexpr int smem = Layout<kD, kNT>::kBytes;
+template <int kD, int kNT, bool kInt8, bool kAll>
+cudaError_t launch_tiles(const AttnKernelParams& kp, const Plan& plan, cudaStream_t s) {
+  using L = Layout<kD, kNT, kAll>;
+  const auto kern = cache_attn_kernel<kD, kNT, kInt8, kAll>;
   static std::atomic<uint64_t> set{0};  // devices on which the kernel's shared memory has been allowed
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !(set.load(std::memory_order_relaxed) >> dev & 1)) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
     if (e != cudaSuccess) return e;
     if (dev < 64) set.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
-  e = launch_kernel(kern, dim3(plan.ctas), Layout<kD, kNT>::kThreads, smem, s, true, kp);
+  return launch_kernel(kern, dim3(plan.ctas), L::kThreads, L::kBytes, s, true, kp);
+}
+
+template <int kD, int kNT, bool kInt8>
+cudaError_t launch_attn(const AttnKernelParams& kp, const Plan& plan, cudaStream_t s) {
+  cudaError_t e = plan.all ? launch_tiles<kD, kNT, kInt8, true>(kp, plan, s) : launch_tiles<kD, kNT, kInt8, false>(kp, plan, s);
   if (e != cudaSuccess) return e;
-  const int blocks = plan.groups > kp.batch ? plan.groups : kp.batch < sm_count() ? kp.batch : sm_count();
-  e = launch_kernel(cache_join_kernel<kD, kNT, kInt8>, dim3(blocks), kJoin, 0, s, true, kp);
-  if (e != cudaSuccess) return e;
-  count_launches(2);
+  count_launches(1);
   if (kp.weights != nullptr && plan.most_tiles > 0) {
     const long long chunks = (plan.most_tiles + kWeightTiles - 1) / kWeightTiles;
     const dim3 grid(static_cast<unsigned>(static_cast<long long>(kp.batch) * kp.c.hkv * chunks));
@@ -838,6 +870,10 @@ extern "C" int rswa_cache_attn(const rswa_cache_attn_params_t* p, void* stream) 
     set_error("%s: q and out must be 16-byte aligned, q with strides that are multiples of 8 elements", what);
     return RSWA_E_ARG;
   }
+  if (p->arrived == nullptr) {
+    set_error("%s: arrived is required", what);
+    return RSWA_E_ARG;
+  }
   if (p->weights != nullptr && p->lse == nullptr) {
     set_error("%s: weights need lse", what);
     return RSWA_E_ARG;
@@ -876,13 +912,13 @@ extern "C" int rswa_cache_attn(const rswa_cache_attn_params_t* p, void* stream) 
   uint8_t* ws = static_cast<uint8_t*>(p->workspace);
   kp.part_o = reinterpret_cast<float*>(ws);
   kp.part_ml = reinterpret_cast<float*>(ws += plan.o_bytes);
-  kp.cut = reinterpret_cast<int4*>(ws += plan.ml_bytes);
-  ws += plan.cut_bytes;
-  kp.first = p->weights != nullptr ? reinterpret_cast<long long*>(ws) : nullptr;
+  ws += plan.ml_bytes;
+  kp.first = p->weights != nullptr ? reinterpret_cast<int*>(ws) : nullptr;
   kp.scores = p->weights != nullptr ? reinterpret_cast<float*>(ws + plan.first_bytes) : nullptr;
   kp.weights = p->weights;
   kp.w_sb = p->w_stride_b, kp.w_sh = p->w_stride_h;
   kp.groups = plan.groups;
+  kp.arrived = p->arrived;
   kp.status = p->status;
   kp.mirror = status_mirror(p->status);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);

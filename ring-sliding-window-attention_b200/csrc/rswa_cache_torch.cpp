@@ -17,6 +17,8 @@
 
 #include <cmath>
 #include <cstring>
+#include <map>
+#include <mutex>
 
 #include "../../include/rswa.h"
 
@@ -125,6 +127,20 @@ bool ready(int dev) {
 void* stream_of(int dev) { return c10::cuda::getCurrentCUDAStream(dev).stream(); }
 void written(const at::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// The zeroed counters of rswa_cache_attn.  Calls on one stream follow one another and share them; a call that is being
+// captured gets its own from the graph's memory, zeroed by the graph each time, since the graph may run beside anything.
+at::Tensor counters(int dev, const at::TensorOptions& options) {
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev).stream();
+  cudaStreamCaptureStatus st;
+  if (cudaStreamIsCapturing(stream, &st) != cudaSuccess || st != cudaStreamCaptureStatusNone) return at::zeros({RSWA_CACHE_ATTN_COUNTERS}, options.dtype(at::kInt));
+  static std::mutex mutex;
+  static auto* kept = new std::map<std::pair<int, cudaStream_t>, at::Tensor>();  // (never freed: the process may end before its streams do)
+  const std::lock_guard<std::mutex> lock(mutex);
+  at::Tensor& t = (*kept)[{dev, stream}];
+  if (!t.defined()) t = at::zeros({RSWA_CACHE_ATTN_COUNTERS}, options.dtype(at::kInt));
+  return t;
 }
 
 // accumulated weights [batch, num_kv_heads, >= tokens]
@@ -306,6 +322,8 @@ PyObject* py_cache_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
     p.workspace = ws.data_ptr();
     p.workspace_bytes = bytes;
+    const at::Tensor arrived = counters(dev, q.options());
+    p.arrived = arrived.data_ptr<int32_t>();
     check(rswa_cache_attn(&p, stream_of(dev)), what);
     if (weights.defined()) written(weights);
   }

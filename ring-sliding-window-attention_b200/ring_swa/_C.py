@@ -125,7 +125,7 @@ class CacheAttnParams(C.Structure):
         ("q", C.c_void_p), ("q_stride_b", C.c_int64), ("q_stride_t", C.c_int64), ("q_stride_h", C.c_int64),
         ("out", C.c_void_p), ("lse", C.c_void_p),
         ("weights", C.c_void_p), ("w_stride_b", C.c_int64), ("w_stride_h", C.c_int64),
-        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("status", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("arrived", C.c_void_p), ("status", C.c_void_p),
     ]
 
 
