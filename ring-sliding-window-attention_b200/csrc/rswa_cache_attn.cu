@@ -23,7 +23,9 @@
 // the sum of the weights takes it back out.  Scores, sums and the output are 32-bit.
 //
 // Work: the 32-token tiles of all (sequence, key/value head, 8 or 16 query rows) in one order, cut evenly whatever the
-// lengths over groups of warps.  The warps of a group take its tiles in turn and add up at the end of each piece.  Where there
+// lengths over groups of warps.  The warps of a group take its tiles in turn and add up at the end of each piece; each item
+// counts one tile per warp more than it has, for that and for its queries (32 requests of 300 to 8192 tokens: the last
+// group ended 13 us behind the median one without, 4 us with it).  Where there
 // are more (sequence, head, row tile)s than SMs a group is four warps, because the end of a piece and the next one's queries
 // cost every warp that takes part as much as several tiles (32 requests of 300 to 8192 tokens, 8 heads: 48 us, and 69 with
 // all 16 warps of an SM in one group); else it is all warps of the SM, which leaves fewer pieces to join.
@@ -78,9 +80,11 @@ struct AttnKernelParams {
 };
 
 // The tiles of one sequence: the ones its sink tokens lie in, then the ones from its oldest visible token on.
+// An item of n tiles counts as n + kOver (kOver ones that are not there, then its tiles), one without any as none.
 struct SeqTiles {
   int len, n_sink_tiles, first, n;
 };
+template <int kOver>
 __device__ __forceinline__ SeqTiles seq_tiles(const AttnKernelParams& p, int b) {
   SeqTiles s;
   int len = p.lens[b];
@@ -93,7 +97,8 @@ __device__ __forceinline__ SeqTiles seq_tiles(const AttnKernelParams& p, int b) 
   s.len = len;
   s.first = oldest / kTok;
   s.n_sink_tiles = min((min(p.n_sink, len) + kTok - 1) / kTok, s.first);
-  s.n = s.n_sink_tiles + (len + kTok - 1) / kTok - s.first;
+  const int n = s.n_sink_tiles + (len + kTok - 1) / kTok - s.first;
+  s.n = n > 0 ? n + kOver : 0;
   return s;
 }
 __device__ __forceinline__ int tile_slot(const SeqTiles& s, int i) { return (i < s.n_sink_tiles ? i : s.first + i - s.n_sink_tiles) * kTok; }
@@ -113,8 +118,10 @@ struct Shares {
   }
 };
 
+// (counted with the kOver from here on)
 // Prefix sums of the sequences' tiles (per key/value head and row tile): thread i of the first kScan holds `per`
 // sequences.  s_prefix[i]: tiles in front of thread i's sequences; s_prefix[kScan]: all.
+template <int kOver>
 __device__ __forceinline__ void tile_prefix(const AttnKernelParams& p, int* s_prefix, int* s_warp) {
   const int per = (p.batch + kScan - 1) / kScan;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -122,7 +129,7 @@ __device__ __forceinline__ void tile_prefix(const AttnKernelParams& p, int* s_pr
   if (threadIdx.x < kScan) {
     for (int i = 0; i < per; ++i) {
       const int b = threadIdx.x * per + i;
-      if (b < p.batch) mine += seq_tiles(p, b).n;
+      if (b < p.batch) mine += seq_tiles<kOver>(p, b).n;
     }
     sum = mine;
 #pragma unroll
@@ -145,7 +152,7 @@ __device__ __forceinline__ void tile_prefix(const AttnKernelParams& p, int* s_pr
         const int b = threadIdx.x * per + i;
         if (b >= p.batch) break;
         p.first[b] = before * items;
-        before += seq_tiles(p, b).n;
+        before += seq_tiles<kOver>(p, b).n;
       }
     }
   }
@@ -153,6 +160,7 @@ __device__ __forceinline__ void tile_prefix(const AttnKernelParams& p, int* s_pr
 }
 
 // A place in the order of all tiles: sequence, then head, then row tile, then tile.
+template <int kOver>
 struct Cursor {
   int b, item, i;       // item = head * row_tiles + row tile
   SeqTiles s;
@@ -167,13 +175,14 @@ struct Cursor {
       k -= s.n;
       if (++item == items) {
         item = 0;
-        do s = seq_tiles(p, ++b); while (s.n == 0);
+        do s = seq_tiles<kOver>(p, ++b); while (s.n == 0);
       }
     }
     i = k;
   }
 };
-__device__ __forceinline__ Cursor cursor_at(const AttnKernelParams& p, const int* s_prefix, int tile) {
+template <int kOver>
+__device__ __forceinline__ Cursor<kOver> cursor_at(const AttnKernelParams& p, const int* s_prefix, int tile) {
   const int items = p.c.hkv * p.row_tiles;
   const int per = (p.batch + kScan - 1) / kScan;
   int lo = 0, hi = kScan - 1;  // the last thread whose prefix is not behind the tile
@@ -183,14 +192,14 @@ __device__ __forceinline__ Cursor cursor_at(const AttnKernelParams& p, const int
   }
   // (threads of no tiles share a prefix: the last of them holds the tile, or has no sequences and the walk starts
   // at a sequence of its own)
-  Cursor c;
+  Cursor<kOver> c;
   c.at = tile;
   c.b = lo * per;
   int rest = tile - s_prefix[lo] * items;
-  c.s = seq_tiles(p, c.b);
+  c.s = seq_tiles<kOver>(p, c.b);
   while (rest >= c.s.n * items) {
     rest -= c.s.n * items;
-    c.s = seq_tiles(p, ++c.b);
+    c.s = seq_tiles<kOver>(p, ++c.b);
   }
   c.item = rest / c.s.n;
   c.i = rest - c.item * c.s.n;
@@ -274,7 +283,7 @@ __device__ __forceinline__ void store_row(const AttnKernelParams& p, int b, int 
 template <int kD, int kPeers>
 __device__ __forceinline__ void empty_rows(const AttnKernelParams& p) {
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-    if (seq_tiles(p, b).n > 0) continue;
+    if (seq_tiles<0>(p, b).n > 0) continue;
     for (int row = threadIdx.x / (kD / 4); row < p.rows * p.c.hkv; row += kPeers / (kD / 4))
       store_row<kD>(p, b, row / p.rows, row % p.rows, threadIdx.x % (kD / 4), make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
   }
@@ -332,7 +341,7 @@ template <int kD, int kNT, bool kInt8, bool kAll>
 __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_attn_kernel(const __grid_constant__ AttnKernelParams p) {
   using L = Layout<kD, kNT, kAll>;
   using R = Ring<kD>;
-  constexpr int kKS = kD / 16, kGroup = L::kGroup, kPeers = kGroup * 32;
+  constexpr int kKS = kD / 16, kGroup = L::kGroup, kPeers = kGroup * 32, kOver = kGroup;
   constexpr int kRows = 8 * kNT;
   extern __shared__ __align__(1024) uint8_t smem[];
   auto& ctl = *reinterpret_cast<typename L::Ctl*>(smem + L::kRings + L::kMerge);
@@ -354,9 +363,9 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
   if (lane < 2) mbar_init(full + lane, 1);
   mbar_fence_init();
   griddep_wait();
-  tile_prefix(p, ctl.prefix, ctl.prefix + kScan + 1);
+  tile_prefix<kOver>(p, ctl.prefix, ctl.prefix + kScan + 1);
   const int total = ctl.prefix[kScan] * p.c.hkv * p.row_tiles;
-  const Shares shares(total, p.groups, kGroup);
+  const Shares shares(total, p.groups, kOver + kGroup);
   if (me >= shares.n || total == 0) {
     if (group == 0) empty_rows<kD, kPeers>(p);
     return;
@@ -365,37 +374,46 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
   const int box = min(p.c.bs, kTok);
 
   // The tiles of this warp, counted: tile i is the share's tile wg + i * kGroup.  Looks 32 of them up, one a lane.
+  // (The warp is told of a tile that is not there by a row of -1.)
   const int n_own = (end - begin - wg + kGroup - 1) / kGroup;
+  int page[2], tokens;  // of this lane's tile
   auto look_up = [&](int i) {
     const int at = begin + wg + (i + lane) * kGroup;
+    page[0] = page[1] = -1, tokens = 0;
     __syncwarp();
     if (at < end) {
-      const Cursor lc = cursor_at(p, ctl.prefix, at);
-      const int bs = p.c.bs, slot = tile_slot(lc.s, lc.i), h = lc.item / p.row_tiles, j = slot / bs;
-      // a tile is part of one block, or two blocks of 16; the second may lie behind the sequence's end: not looked at
-      int pg[2], row[2];
-      pg[0] = table_entry(p.table, p.table_stride, lc.b, j, p.c.num_blocks, p.status, p.mirror);
-      pg[1] = pg[0];
-      if (bs < kTok && slot + bs < lc.s.len) pg[1] = table_entry(p.table, p.table_stride, lc.b, j + 1, p.c.num_blocks, p.status, p.mirror);
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int page = max(pg[t], 0);  // (reported; any block will do then)
-        const long long ph = static_cast<long long>(page) * p.c.hkv + h;
-        row[t] = static_cast<int>(ph) * bs + slot % bs;
-        float4 sc = make_float4(1.f, 0.f, 1.f, 0.f);
-        if (slot + 16 * t < lc.s.len) {  // (tokens behind the end: their block may not even have a scale)
-          const float sv = p.c.scale[1][ph];
-          sc = make_float4(p.c.scale[0][ph], __log2f(sv), 1.f / sv, 0.f);
-        }
-        ctl.scale[warp][lane][t] = sc;
+      const auto lc = cursor_at<kOver>(p, ctl.prefix, at);
+      int2 row = make_int2(-1, -1);
+      if (lc.i >= kOver) {
+        const int bs = p.c.bs, slot = tile_slot(lc.s, lc.i - kOver), h = lc.item / p.row_tiles, j = slot / bs;
+        // a tile is part of one block, or two blocks of 16; the second may lie behind the sequence's end: not looked at
+        // (an entry that is no block has been reported; any block will do then)
+        page[0] = max(0, table_entry(p.table, p.table_stride, lc.b, j, p.c.num_blocks, p.status, p.mirror)) * p.c.hkv + h;
+        page[1] = page[0];
+        if (bs < kTok && slot + bs < lc.s.len)
+          page[1] = max(0, table_entry(p.table, p.table_stride, lc.b, j + 1, p.c.num_blocks, p.status, p.mirror)) * p.c.hkv + h;
+        tokens = lc.s.len - slot;
+        row = make_int2(page[0] * bs + slot % bs, page[1] * bs + slot % bs);
       }
-      ctl.row[warp][lane] = make_int2(row[0], row[1]);
+      ctl.row[warp][lane] = row;
     }
     __syncwarp();
   };
-  int loaded[2] = {0, 0};  // the last tile loaded
+  auto look_up_scales = [&]() {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      float4 sc = make_float4(1.f, 0.f, 1.f, 0.f);
+      if (16 * t < tokens) {  // (tokens behind the end: their block may not even have a scale)
+        const float sv = p.c.scale[1][page[t]];
+        sc = make_float4(p.c.scale[0][page[t]], __log2f(sv), 1.f / sv, 0.f);
+      }
+      ctl.scale[warp][lane][t] = sc;
+    }
+    __syncwarp();
+  };
+  int loaded[2] = {0, 0};  // loads so far
   auto load = [&](int i, int kv) {
-    loaded[kv] = i;
+    ++loaded[kv];
     if (lane == 0) {
       const int2 row = ctl.row[warp][i & 31];
       mbar_expect_tx(full + kv, R::kTileBytes);
@@ -403,16 +421,42 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
       if (box < kTok) tma_load_rows(own + kv * R::kTileBytes + box * kD, &p.map[kv], full + kv, row.y);
     }
   };
+  int own_i = 0, done = 0;  // this warp's next tile, and how many it has been through
+  auto advance = [&](int i) {  // the next tile from i on that is there
+    while (i < n_own) {
+      if ((i & 31) == 0 && i > 0) {
+        look_up(i);
+        look_up_scales();
+      }
+      if (ctl.row[warp][i & 31].x >= 0) break;
+      ++i;
+    }
+    return i;
+  };
   if (n_own > 0) {
     look_up(0);
-    load(0, 0);
-    load(0, 1);
+    while (own_i < min(n_own, 32) && ctl.row[warp][own_i].x < 0) ++own_i;
+    if (own_i < min(n_own, 32)) {
+      load(own_i, 0);
+      load(own_i, 1);
+    }
+    look_up_scales();
+    if (own_i == 32) {  // (none of them is there: sequences of hardly any tokens)
+      own_i = advance(own_i);
+      if (own_i < n_own) {
+        load(own_i, 0);
+        load(own_i, 1);
+      }
+    }
   }
-  Cursor cc = cursor_at(p, ctl.prefix, begin);
-  int own_i = 0;  // this warp's next tile
+  auto cc = cursor_at<kOver>(p, ctl.prefix, begin);
   bool dead = false;
   while (cc.at < end) {
     const int piece_end = min(end, cc.at + cc.s.n - cc.i);
+    if (cc.i + piece_end - cc.at <= kOver) {  // none of its tiles is this group's
+      cc.skip(p, piece_end - cc.at, end);
+      continue;
+    }
     const int h = cc.item / p.row_tiles, row0 = (cc.item - h * p.row_tiles) * kRows;
     // the queries of this piece as operands: row g of each column block, d = 16 s + 4c .. 4c + 3
     uint32_t qf[kNT][kKS][2];
@@ -485,10 +529,10 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
       l[nt][0] = l[nt][1] = 0.f;
     }
     // this warp's tiles of the piece: those whose index from `begin` is `wg` modulo kGroup
-    for (int at = begin + wg + own_i * kGroup; at < piece_end; at += kGroup) {
+    for (int at; (at = begin + wg + own_i * kGroup) < piece_end && own_i < n_own;) {
       const float4 sc0 = ctl.scale[warp][own_i & 31][0], sc1 = ctl.scale[warp][own_i & 31][1];
-      if (!dead) dead = !mbar_wait_w(full, own_i & 1, &ctl.err, kErrWaitProducer);
-      const int slot = tile_slot(cc.s, cc.i + at - cc.at);
+      if (!dead) dead = !mbar_wait_w(full, done & 1, &ctl.err, kErrWaitProducer);
+      const int slot = tile_slot(cc.s, cc.i + at - cc.at - kOver);
       const uint32_t k_base = smem_u32(own), v_base = k_base + R::kTileBytes;
       const float sk[2] = {sc0.x, sc1.x}, lv[2] = {sc0.y, sc1.y}, iv[2] = {sc0.z, sc1.z};
       // ---- scores
@@ -510,10 +554,9 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
         }
       }
       // every lane has read K: the next tile's
-      const bool more = own_i + 1 < n_own && !dead;
-      if (more && ((own_i + 1) & 31) == 0) look_up(own_i + 1);
+      const int next_i = advance(own_i + 1);
       __syncwarp();
-      if (more) load(own_i + 1, 0);
+      if (next_i < n_own && !dead) load(next_i, 0);
       // ---- to base 2, hidden ones to -inf
       const bool plain = slot + kTok - 1 <= last_min && (slot >= first_max || slot + kTok <= p.n_sink);
 #pragma unroll
@@ -592,7 +635,7 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
         }
       }
       // ---- output
-      if (!dead) dead = !mbar_wait_w(full + 1, own_i & 1, &ctl.err, kErrWaitProducer);
+      if (!dead) dead = !mbar_wait_w(full + 1, done & 1, &ctl.err, kErrWaitProducer);
       if (!kInt8 && slot + kTok > cc.s.len) {
         // the slots behind the last token hold anything: a weight of 0 does not take a NaN away
         if (slot + lane >= cc.s.len)
@@ -613,13 +656,15 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
         }
       }
       __syncwarp();  // every lane has read V
-      if (more && !dead) load(own_i + 1, 1);
-      ++own_i;
+      if (next_i < n_own && !dead) load(next_i, 1);
+      own_i = next_i;
+      ++done;
     }
 
     // ---- the warps' sums of this piece
-    const bool from_start = cc.i == 0, to_end = piece_end - cc.at == cc.s.n - cc.i;
-    const bool whole = from_start && to_end;
+    // (the first piece is the one with the item's first tile)
+    const int item0 = cc.at - cc.i, lo = shares.of(item0 + kOver), pieces = shares.of(item0 + cc.s.n - 1) - lo + 1;
+    const bool whole = pieces == 1;
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
@@ -665,7 +710,7 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
           if (whole) {
             store_row<kD>(p, cc.b, h, row, d4, x, top, sum);
           } else {
-            const long long to = (static_cast<long long>(me) * 2 + (from_start ? 1 : 0)) * kRows + nt * 8 + r;
+            const long long to = (static_cast<long long>(me) * 2 + (me == lo ? 1 : 0)) * kRows + nt * 8 + r;
             *reinterpret_cast<float4*>(p.part_o + to * kD + d4 * 4) = x;
             if (d4 == 0) *reinterpret_cast<float2*>(p.part_ml + to * 2) = make_float2(top, sum);
           }
@@ -675,7 +720,6 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
     }
     if (!whole) {
       // the group that delivers an item's last piece joins them all
-      const int first = cc.at - cc.i, lo = shares.of(first), pieces = shares.of(first + cc.s.n - 1) - lo + 1;
       if (threadIdx.x == group * kPeers) {
         __threadfence();
         const int last = atomicAdd(p.arrived + lo, 1) == pieces - 1;
@@ -693,8 +737,8 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
   if (dead) {
     // copies still on their way must not outlive the CTA's shared memory (each wait is limited)
     int own_err = 0;
-    if (n_own > 0)
-      for (int kv = 0; kv < 2; ++kv) mbar_wait(full + kv, loaded[kv] & 1, &own_err, kErrWaitProducer);
+    for (int kv = 0; kv < 2; ++kv)
+      if (loaded[kv] > 0) mbar_wait(full + kv, (loaded[kv] - 1) & 1, &own_err, kErrWaitProducer);
     if (lane == 0) raise_status(p.status, p.mirror, kErrWaitProducer);
   }
   if (group == 0) empty_rows<kD, kPeers>(p);
@@ -703,15 +747,16 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
 // Adds every visible slot's softmax weights up, from the scores that the first kernel kept and the final log-sum-exp.
 // One CTA per (sequence, head) and kWeightTiles tiles.
 constexpr int kWeightTiles = 16;
-template <int kNT>
+template <int kNT, int kOver>
 __global__ void __launch_bounds__(kAdd) cache_weights_kernel(const __grid_constant__ AttnKernelParams p, int chunks) {
   constexpr int kRows = 8 * kNT;
   extern __shared__ float s_lse[];  // [row_tiles * kRows], base 2; +inf for rows that see nothing and rows behind the last
   griddep_wait();
   const int bh = blockIdx.x / chunks, b = bh / p.c.hkv, h = bh - b * p.c.hkv;
-  const SeqTiles s = seq_tiles(p, b);
+  const SeqTiles s = seq_tiles<kOver>(p, b);
   const int t0 = (blockIdx.x - bh * chunks) * kWeightTiles;
-  if (t0 >= s.n) return;
+  const int n = s.n - kOver;  // tiles
+  if (t0 >= n) return;
   for (int r = threadIdx.x; r < p.row_tiles * kRows; r += kAdd) {
     float x = INFINITY;
     if (r < p.rows) {
@@ -723,13 +768,13 @@ __global__ void __launch_bounds__(kAdd) cache_weights_kernel(const __grid_consta
   }
   __syncthreads();
   const int first = p.first[b] + h * p.row_tiles * s.n;
-  const int t1 = min(t0 + kWeightTiles, s.n);
+  const int t1 = min(t0 + kWeightTiles, n);
   for (int k = t0 * kTok + threadIdx.x; k < t1 * kTok; k += kAdd) {
     const int tile = k / kTok, tok = tile_slot(s, tile) + k % kTok;
     if (tok >= s.len) continue;
     float sum = 0.f;
     for (int rt = 0; rt < p.row_tiles; ++rt) {
-      const float4* from = reinterpret_cast<const float4*>(p.scores + (static_cast<long long>(first + rt * s.n + tile) * kTok + k % kTok) * kRows);
+      const float4* from = reinterpret_cast<const float4*>(p.scores + (static_cast<long long>(first + rt * s.n + kOver + tile) * kTok + k % kTok) * kRows);
 #pragma unroll
       for (int v = 0; v < kRows / 4; ++v) {
         const float4 x = from[v];
@@ -745,7 +790,8 @@ __global__ void __launch_bounds__(kAdd) cache_weights_kernel(const __grid_consta
 struct Plan {
   int nt, row_tiles, groups, ctas;
   bool all;  // all warps of a CTA are one group
-  long long most_tiles;  // of a sequence, per head and row tile
+  long long most_tiles;  // of a sequence, per head and row tile, and as they are counted
+  int over;
   int64_t o_bytes, ml_bytes, first_bytes, score_bytes;
   int64_t total() const { return o_bytes + ml_bytes + first_bytes + score_bytes; }
 };
@@ -765,14 +811,20 @@ int make_plan(const rswa_cache_attn_params_t& a, Plan& plan) {
   plan.most_tiles = most;
   const long long items = static_cast<long long>(a.table.batch) * a.cache.n_kv_heads * row_tiles;
   // (a row tile's log-sum-exps lie in shared memory while the weights are added up)
-  if (row_tiles > 512 || items > 0x7fffffffLL || items * most > 0x7fffffffLL) {
+  if (row_tiles > 512 || items > 0x7fffffffLL || items > 0x7fffffffLL) {
     set_error("rswa_cache_attn: too many queries in one call");
     return RSWA_E_UNSUPPORTED;
   }
   plan.row_tiles = static_cast<int>(row_tiles);
   const int sms = sm_count(), warps = plan.nt == 1 ? Layout<128, 1, true>::kWarps : Layout<128, 2, true>::kWarps;
   plan.all = items <= sms;
-  const long long shares = items * most / (plan.all ? warps : 4), most_groups = plan.all ? sms : static_cast<long long>(sms) * warps / 4;
+  plan.over = plan.all ? warps : 4;
+  most += plan.over;
+  if (items * most > 0x7fffffffLL) {
+    set_error("rswa_cache_attn: too many tokens in one call");
+    return RSWA_E_UNSUPPORTED;
+  }
+  const long long shares = items * most / (2 * plan.over), most_groups = plan.all ? sms : static_cast<long long>(sms) * warps / 4;
   plan.groups = static_cast<int>(shares < 1 ? 1 : shares < most_groups ? shares : most_groups);
   if (plan.groups > RSWA_CACHE_ATTN_COUNTERS) plan.groups = RSWA_CACHE_ATTN_COUNTERS;
   plan.ctas = plan.groups < sms ? plan.groups : sms;
@@ -829,7 +881,8 @@ cudaError_t launch_attn(const AttnKernelParams& kp, const Plan& plan, cudaStream
   if (kp.weights != nullptr && plan.most_tiles > 0) {
     const long long chunks = (plan.most_tiles + kWeightTiles - 1) / kWeightTiles;
     const dim3 grid(static_cast<unsigned>(static_cast<long long>(kp.batch) * kp.c.hkv * chunks));
-    e = launch_kernel(cache_weights_kernel<kNT>, grid, kAdd, plan.row_tiles * 8 * kNT * 4, s, true, kp, static_cast<int>(chunks));
+    e = launch_kernel(plan.all ? cache_weights_kernel<kNT, Layout<kD, kNT, true>::kGroup> : cache_weights_kernel<kNT, Layout<kD, kNT, false>::kGroup>, grid, kAdd,
+                      plan.row_tiles * 8 * kNT * 4, s, true, kp, static_cast<int>(chunks));
     if (e != cudaSuccess) return e;
     count_launches(1);
   }
