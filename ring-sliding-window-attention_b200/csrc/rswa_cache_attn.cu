@@ -433,6 +433,31 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
     }
     return i;
   };
+  // The piece this group works on, and its end: a piece has at least one tile that is there.  Its queries (row g of each
+  // column block, elements 16 s + 4c .. 4c + 3) are fetched while the one before it is added up; 16 rows of them do not
+  // fit the registers then and are fetched behind that.
+  auto cc = cursor_at<kOver>(p, ctl.prefix, begin);
+  int piece_end = begin;
+  uint2 raw[kNT][kKS];
+  auto next_piece = [&](int from) {
+    cc.skip(p, from - cc.at, end);
+    while (cc.at < end) {
+      piece_end = min(end, cc.at + cc.s.n - cc.i);
+      if (cc.i + piece_end - cc.at > kOver) break;
+      cc.skip(p, piece_end - cc.at, end);
+    }
+  };
+  auto fetch_queries = [&]() {
+    if (cc.at >= end) return;
+    const int h = cc.item / p.row_tiles, row0 = (cc.item - h * p.row_tiles) * kRows;
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+      const int row = row0 + nt * 8 + g, i = row / p.group, hd = h * p.group + row - i * p.group;
+      const uint16_t* src = p.q + cc.b * p.q_sb + i * p.q_st + hd * p.q_sh + c * 4;
+#pragma unroll
+      for (int s = 0; s < kKS; ++s) raw[nt][s] = row < p.rows ? *reinterpret_cast<const uint2*>(src + s * 16) : make_uint2(0, 0);
+    }
+  };
   if (n_own > 0) {
     look_up(0);
     while (own_i < min(n_own, 32) && ctl.row[warp][own_i].x < 0) ++own_i;
@@ -440,6 +465,8 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
       load(own_i, 0);
       load(own_i, 1);
     }
+    next_piece(begin);
+    if (kNT == 1) fetch_queries();
     look_up_scales();
     if (own_i == 32) {  // (none of them is there: sequences of hardly any tokens)
       own_i = advance(own_i);
@@ -448,37 +475,21 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
         load(own_i, 1);
       }
     }
+  } else {
+    next_piece(begin);
+    if (kNT == 1) fetch_queries();
   }
-  auto cc = cursor_at<kOver>(p, ctl.prefix, begin);
   bool dead = false;
   while (cc.at < end) {
-    const int piece_end = min(end, cc.at + cc.s.n - cc.i);
-    if (cc.i + piece_end - cc.at <= kOver) {  // none of its tiles is this group's
-      cc.skip(p, piece_end - cc.at, end);
-      continue;
-    }
     const int h = cc.item / p.row_tiles, row0 = (cc.item - h * p.row_tiles) * kRows;
-    // the queries of this piece as operands: row g of each column block, d = 16 s + 4c .. 4c + 3
+    if (kNT > 1) fetch_queries();
     uint32_t qf[kNT][kKS][2];
     float rs[kNT][2];  // factor of the scores of rows 2c, 2c + 1, log2(e) in it
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt) {
-      const int row = row0 + nt * 8 + g;
-      float factor = 0.f;
-      if (row < p.rows) {
-        const int i = row / p.group, hd = h * p.group + row - i * p.group;
-        const uint16_t* src = p.q + cc.b * p.q_sb + i * p.q_st + hd * p.q_sh + c * 4;
 #pragma unroll
-        for (int s = 0; s < kKS; ++s) {
-          const uint2 x = *reinterpret_cast<const uint2*>(src + s * 16);
-          qf[nt][s][0] = x.x;
-          qf[nt][s][1] = x.y;
-        }
-        factor = 1.f;
-      } else {
-#pragma unroll
-        for (int s = 0; s < kKS; ++s) qf[nt][s][0] = qf[nt][s][1] = 0;
-      }
+      for (int s = 0; s < kKS; ++s) qf[nt][s][0] = raw[nt][s].x, qf[nt][s][1] = raw[nt][s].y;
+      float factor = row0 + nt * 8 + g < p.rows ? 1.f : 0.f;
       if (p.bf16) {
         uint32_t most = 0;
 #pragma unroll
@@ -665,6 +676,9 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
     // (the first piece is the one with the item's first tile)
     const int item0 = cc.at - cc.i, lo = shares.of(item0 + kOver), pieces = shares.of(item0 + cc.s.n - 1) - lo + 1;
     const bool whole = pieces == 1;
+    const int b = cc.b;
+    next_piece(piece_end);
+    if (kNT == 1) fetch_queries();
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
@@ -700,15 +714,14 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
 #pragma unroll
         for (int w = 0; w < kGroup; ++w) {
           const float lw = ml[w][nt * 8 + r][1];
-          if (lw == 0.f) continue;  // (no visible token)
-          const float f = ex2f(ml[w][nt * 8 + r][0] - top);
+          const float f = lw == 0.f ? 0.f : ex2f(ml[w][nt * 8 + r][0] - top);  // (0: no visible token)
           const float4 y = *reinterpret_cast<const float4*>(merge + (w * 8 + r) * kD + ((d4 * 4) ^ (r / 2 * 8)));
           sum += lw * f;
           x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
         }
         if (row < p.rows) {
           if (whole) {
-            store_row<kD>(p, cc.b, h, row, d4, x, top, sum);
+            store_row<kD>(p, b, h, row, d4, x, top, sum);
           } else {
             const long long to = (static_cast<long long>(me) * 2 + (me == lo ? 1 : 0)) * kRows + nt * 8 + r;
             *reinterpret_cast<float4*>(p.part_o + to * kD + d4 * 4) = x;
@@ -730,9 +743,8 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
         ctl.last[group] = last;
       }
       sync_group<kPeers>(group);
-      if (ctl.last[group] != 0) join_pieces<kD, kNT, kPeers>(p, merge, group, cc.b, h, row0, lo, pieces);
+      if (ctl.last[group] != 0) join_pieces<kD, kNT, kPeers>(p, merge, group, b, h, row0, lo, pieces);
     }
-    cc.skip(p, piece_end - cc.at, end);
   }
   if (dead) {
     // copies still on their way must not outlive the CTA's shared memory (each wait is limited)
