@@ -6,9 +6,13 @@
 //
 // S^T = K Q^T on the tensor cores with the keys as rows: a thread then owns a key, and the sum over queries is a sum
 // over the columns it reads from tensor memory, with no exchange between threads.  A step of the pipeline is 256 keys
-// (two tiles, one per compute warpgroup) by 128 queries of one head: each Q tile that comes out of L2 feeds two products.
+// (two tiles) by 128 queries of one head: each Q tile that comes out of L2 feeds two products.  Eight warps work on a tile, 64
+// query columns each: four a scheduler, so that one's loads from tensor memory hide behind the others' arithmetic (with 128
+// columns and half the warps a step took 3270 cycles).
 // 2 * head_dim FLOPs and one exponential per (query head, pair): at 128 elements the exponentials (16 per clock and SM,
-// 2048 cycles a step) outweigh the products (1024).
+// 2048 cycles a step) outweigh the products (1024).  One pair in eight is computed on the FMA pipe (fma_exp2): none
+// 713 us, 1/8 701, 1/4 720, 3/8 788 (16384 tokens, 32/8 heads, window 4096): the card is at its power cap there
+// (1.5 GHz), and an exponential on the FMA pipe costs more than it saves beyond that.  A step takes about 2400 cycles.
 //
 // Work: the steps of all (batch row, key/value head, 256 keys) in one order, cut into equal shares, one per CTA, whatever
 // the mask makes of an item's length (a sink token is seen by its whole sequence): nothing is longer than the rest.  An
@@ -25,7 +29,8 @@ using namespace tc05;
 namespace {
 
 constexpr int kKeys = 2 * kTile;   // keys of an item
-constexpr int kThreads = 384;      // warp 0 TMA, warp 1 MMA, warp 2 log-sum-exps, warp 3 idle, warps 4-7 and 8-11 compute
+constexpr int kSumWarps = 16;
+constexpr int kThreads = 128 + kSumWarps * 32;  // warp 0 TMA, warp 1 MMA, warp 2 log-sum-exps, warp 3 idle, warps 4-19 sums
 constexpr int kScan = 256;         // threads of the prefix sums
 constexpr int kQStages = 3;
 constexpr int kTmemCols = 512;
@@ -121,13 +126,42 @@ __device__ __forceinline__ Item item_at(const SumsKernelParams& p, const long lo
   return it;
 }
 
+// 2^x for two values on the FMA pipe: x = n + f with n = round(x) and f in [-0.5, 0.5]; 2^f by the polynomial of degree 5 with
+// the least relative error there (7.5e-8, found by exchange of its extrema; 2.1e-7 in 32 bits), times 2^n from n's bits.  Below
+// -125 (hidden scores are -inf) 2^-125; NaN stays NaN.
+__device__ __forceinline__ float2 fma_exp2(float2 x) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-125.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-125.f));
+  const float2 t = __fadd2_rn(x, make_float2(12582912.f, 12582912.f));  // 1.5 * 2^23: n lands in the low mantissa bits
+  const float2 n = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
+  const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+  float2 q = __ffma2_rn(make_float2(0.0013276472454890609f, 0.0013276472454890609f), f, make_float2(0.009675540961325169f, 0.009675540961325169f));
+  q = __ffma2_rn(q, f, make_float2(0.05550713092088699f, 0.05550713092088699f));
+  q = __ffma2_rn(q, f, make_float2(0.24022120237350464f, 0.24022120237350464f));
+  q = __ffma2_rn(q, f, make_float2(0.6931469440460205f, 0.6931469440460205f));
+  q = __ffma2_rn(q, f, make_float2(1.0000001192092896f, 1.0000001192092896f));
+  const float2 p = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
+  return __fmul2_rn(q, p);
+}
+
+// barrier of the summing warps; whether all of them are well
+__device__ __forceinline__ bool all_sum_warps(bool ok) {
+  int all;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, %2, p;\n\tselp.s32 %0, 1, 0, q;\n\t}\n"
+               : "=r"(all)
+               : "r"(static_cast<int>(ok)), "n"(kSumWarps * 32)
+               : "memory");
+  return all != 0;
+}
+
 struct Ctl {
-  uint64_t k_full[2], k_free[2], q_full[kQStages], q_free[kQStages], s_ready[2], s_free[2], l_full[2], drained;
+  uint64_t k_full[2], k_free[2], q_full[kQStages], q_free[kQStages], s_ready[2][2], s_free[2][2], drained;  // (of the steps' parity, and of the two tiles)
   uint32_t tmem_base;
   int err;
 };
 
-constexpr int kSmemK = 0, kSmemQ = 4 * kTileBytes, kSmemLse = kSmemQ + kQStages * kTileBytes, kSmemCtl = kSmemLse + 2 * kTile * 4;
+constexpr int kSmemK = 0, kSmemQ = 4 * kTileBytes, kSmemLse = kSmemQ + kQStages * kTileBytes;
+constexpr int kSmemHalf = kSmemLse + 2 * kTile * 4, kSmemCtl = kSmemHalf + kKeys * 4;
 constexpr int kSmemBytes = kSmemCtl + 256;
 static_assert(sizeof(Ctl) <= 256 && kSmemBytes <= 232448, "shared memory budget");
 
@@ -146,9 +180,10 @@ __global__ void __launch_bounds__(kThreads, 1) weight_sums_kernel(const __grid_c
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl->k_full[i], 1);
       mbar_init(&ctl->k_free[i], 1);
-      mbar_init(&ctl->s_ready[i], 1);
-      mbar_init(&ctl->s_free[i], 8);
-      mbar_init(&ctl->l_full[i], 1);
+      for (int t = 0; t < 2; ++t) {
+        mbar_init(&ctl->s_ready[i][t], 2);  // the products, and their row of log-sum-exps
+        mbar_init(&ctl->s_free[i][t], kSumWarps / 2);
+      }
     }
     for (int i = 0; i < kQStages; ++i) {
       mbar_init(&ctl->q_full[i], 1);
@@ -230,17 +265,19 @@ __global__ void __launch_bounds__(kThreads, 1) weight_sums_kernel(const __grid_c
       for (int i = static_cast<int>(at - it.first); i < stop && ok; ++i, ++g) {
         const int st = g % kQStages, sb = g & 1;
         ok = mbar_wait(&ctl->q_full[st], (g / kQStages) & 1, err, kErrWaitMma);
-        if (ok && g >= 2) ok = mbar_wait(&ctl->s_free[sb], ((g >> 1) - 1) & 1, err, kErrWaitMma);
-        if (!ok) break;
-        tc_fence_after();
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t) {
+          if (ok && g >= 2) ok = mbar_wait(&ctl->s_free[sb][t], ((g >> 1) - 1) & 1, err, kErrWaitMma);
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
           for (int k = 0; k < kD / 16; ++k) {
             const uint32_t off = ((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4;
             mma_ss(tmem + sb * 256 + t * 128, dK + (kb * 2 + t) * kTile16 + off, dQ + st * kTile16 + off, id, k > 0 ? 1u : 0u);
           }
-        mma_commit(&ctl->s_ready[sb]);
+          mma_commit(&ctl->s_ready[sb][t]);
+        }
+        if (!ok) break;
         mma_commit(&ctl->q_free[st]);
       }
       mma_commit(&ctl->k_free[kb]);
@@ -269,19 +306,20 @@ __global__ void __launch_bounds__(kThreads, 1) weight_sums_kernel(const __grid_c
           x[k] = q0 + r < p.len ? src[r] * -1.4426950408889634f : -INFINITY;
           if (x[k] == INFINITY) x[k] = -INFINITY;  // a query that saw nothing
         }
-        if (g >= 2) ok = mbar_wait_w<100>(&ctl->s_free[sb], ((g >> 1) - 1) & 1, err, kErrWaitProducer);
+        for (int t = 0; t < 2 && ok && g >= 2; ++t) ok = mbar_wait_w<100>(&ctl->s_free[sb][t], ((g >> 1) - 1) & 1, err, kErrWaitProducer);
         if (!ok) break;
 #pragma unroll
         for (int k = 0; k < 4; ++k) sLse[sb * kTile + k * 32 + lane] = x[k];
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->l_full[sb]);
+        if (lane < 2) mbar_arrive(&ctl->s_ready[sb][lane]);
       }
       at = it.first + stop;
     }
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- sums
-    const int tile = (warp - 4) >> 2, key = tile * kTile + (warp & 3) * 32 + lane;
+    const int tile = (warp - 4) >> 3, half = (warp - 4) >> 2 & 1, key = tile * kTile + (warp & 3) * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    float* const s_half = reinterpret_cast<float*>(smem + kSmemHalf);  // [kKeys]: the sums of the upper 64 columns
     const float2 sl = make_float2(p.scale_log2, p.scale_log2);
     bool ok = true;
     int g = 0;
@@ -300,37 +338,39 @@ __global__ void __launch_bounds__(kThreads, 1) weight_sums_kernel(const __grid_c
       float sum = 0.f, lost = 0.f;
       const int stop = static_cast<int>(min(end, it.first + it.n) - it.first);
       const int start = static_cast<int>(at - it.first);
+      int qt = start % it.n_qt - 1;
       for (int i = start; i < stop; ++i, ++g) {
-        const int sb = g & 1, q0 = t0 + i % it.n_qt * kTile;
-        ok = mbar_wait_w(&ctl->s_ready[sb], (g >> 1) & 1, err, kErrWaitSoftmax);
-        if (ok) ok = mbar_wait_w(&ctl->l_full[sb], (g >> 1) & 1, err, kErrWaitSoftmax);
+        if (++qt == it.n_qt) qt = 0;
+        const int sb = g & 1, q0 = t0 + qt * kTile + half * 64;
+        ok = mbar_wait_w(&ctl->s_ready[sb][tile], (g >> 1) & 1, err, kErrWaitSoftmax);
         if (!ok) break;
         tc_fence_after();
-        const bool none = q0 + kTile - 1 < lo || q0 > hi, full = q0 >= lo && q0 + kTile - 1 <= hi;
+        const bool none = q0 + 63 < lo || q0 > hi, full = q0 >= lo && q0 + 63 <= hi;
         if (!__all_sync(0xffffffffu, none)) {
           const bool masked = !__all_sync(0xffffffffu, full);
-          const float* lse = sLse + sb * kTile;
-          const uint32_t from = tmem + sb * 256 + tile * 128 + lane_off;
+          const float* lse = sLse + sb * kTile + half * 64;
+          const uint32_t from = tmem + sb * 256 + tile * 128 + half * 64 + lane_off;
           float2 acc[4] = {};
-          uint32_t r[2][32];
-          tmem_ld32(from, r[0]);
+          uint32_t x[2][32];
+          tmem_ld32(from, x[0]);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 2; ++c) {
             tmem_ld_wait();
-            if (c < 3) tmem_ld32(from + (c + 1) * 32, r[(c + 1) & 1]);
-            uint32_t(&x)[32] = r[c & 1];
+            if (c == 0) tmem_ld32(from + 32, x[1]);
             if (masked) {
               const uint32_t at0 = static_cast<uint32_t>(q0 + c * 32 - lo);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) x[k] = at0 + k < seen ? x[k] : 0xff800000u;
+              for (int k = 0; k < 32; ++k) x[c][k] = at0 + k < seen ? x[c][k] : 0xff800000u;
             }
 #pragma unroll
             for (int k = 0; k < 32; k += 4) {
               const float4 l = *reinterpret_cast<const float4*>(lse + c * 32 + k);
-              const float2 a = __ffma2_rn(make_float2(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), sl, make_float2(l.x, l.y));
-              const float2 b = __ffma2_rn(make_float2(__uint_as_float(x[k + 2]), __uint_as_float(x[k + 3])), sl, make_float2(l.z, l.w));
-              acc[k / 4 % 2 * 2] = __fadd2_rn(acc[k / 4 % 2 * 2], make_float2(ex2f(a.x), ex2f(a.y)));
-              acc[k / 4 % 2 * 2 + 1] = __fadd2_rn(acc[k / 4 % 2 * 2 + 1], make_float2(ex2f(b.x), ex2f(b.y)));
+              const float2 a = __ffma2_rn(make_float2(__uint_as_float(x[c][k]), __uint_as_float(x[c][k + 1])), sl, make_float2(l.x, l.y));
+              const float2 b = __ffma2_rn(make_float2(__uint_as_float(x[c][k + 2]), __uint_as_float(x[c][k + 3])), sl, make_float2(l.z, l.w));
+              const float2 ea = make_float2(ex2f(a.x), ex2f(a.y));
+              const float2 eb = k % 16 == 0 ? fma_exp2(b) : make_float2(ex2f(b.x), ex2f(b.y));
+              acc[k / 4 % 2 * 2] = __fadd2_rn(acc[k / 4 % 2 * 2], ea);
+              acc[k / 4 % 2 * 2 + 1] = __fadd2_rn(acc[k / 4 % 2 * 2 + 1], eb);
             }
           }
           const float2 s2 = __fadd2_rn(__fadd2_rn(acc[0], acc[1]), __fadd2_rn(acc[2], acc[3]));
@@ -341,9 +381,14 @@ __global__ void __launch_bounds__(kThreads, 1) weight_sums_kernel(const __grid_c
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->s_free[sb]);
+        if (lane == 0) mbar_arrive(&ctl->s_free[sb][tile]);
       }
-      if (ok) {
+      // the two halves of the columns.  (All of these warps come here, whatever happened, and go on or leave together.)
+      if (half == 1) s_half[key] = sum;
+      ok = all_sum_warps(ok);
+      if (half == 0) sum += s_half[key];
+      ok = all_sum_warps(ok);
+      if (ok && half == 0) {
         const bool whole = start == 0 && stop == it.n;
         if (whole) {
           if (t < p.len) p.out[static_cast<long long>(it.bh) * p.len + t] = sum;
