@@ -149,10 +149,8 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const __grid_con
                        to_bytes<kInt8>(f[2].x * inv, f[2].y * inv, f[3].x * inv, f[3].y * inv));
     } else if (row < first && grows) {
       const uint2 old = *to;
-      const float4 u = to_float4<kInt8>(old.x), v = to_float4<kInt8>(old.y);
-      // (the value, rounded as it would be read, then divided: for powers of two both are exact)
-      *to = make_uint2(to_bytes<kInt8>(u.x * before * inv, u.y * before * inv, u.z * before * inv, u.w * before * inv),
-                       to_bytes<kInt8>(v.x * before * inv, v.y * before * inv, v.z * before * inv, v.w * before * inv));
+      const Rescale<kInt8> to_new(before * inv);
+      *to = make_uint2(to_new(old.x), to_new(old.y));
     }
   }
 }

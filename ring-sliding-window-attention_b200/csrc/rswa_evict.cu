@@ -1,6 +1,6 @@
 // Thinning out cached sequences by accumulated attention weight (see rswa_cache_evict in rswa.h), in two kernels:
 // one chooses the slots that stay, per sequence and key/value head, the other packs their keys and values into new blocks.
-#include <type_traits>
+#include <atomic>
 
 #include "rswa_cache.cuh"
 
@@ -13,6 +13,7 @@ namespace {
 constexpr int kSelect = 1024;     // threads of a choosing CTA
 constexpr int kBins = 2048;       // of a radix pass: 11, 11 and 10 bits
 constexpr int kPack = 128;        // threads of a packing CTA
+constexpr int kCacheKeys = 49152; // keys that a choosing CTA keeps in shared memory
 
 struct EvictKernelParams {
   CacheView c;
@@ -48,13 +49,23 @@ __device__ __forceinline__ uint32_t order_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// s[0] + ... + s[warp - 1], for all lanes of a warp (at most 32 values)
+__device__ __forceinline__ int sum_below(const int* s, int warp) {
+  const int lane = threadIdx.x & 31;
+  return __reduce_add_sync(0xffffffffu, lane < warp ? s[lane] : 0);
+}
+
 // One CTA per (sequence, head).  The k-th largest key between the sinks and the newest tokens is found digit by digit
 // (11, 11, 10 bits; a histogram of the candidates' digits each time), then two ordered sweeps write what is above it and
-// the first ones of those equal to it.  The weights come from L2 after the first of the five sweeps.
-__global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_constant__ EvictKernelParams p) {
-  __shared__ int s_hist[kBins];
+// the first ones of those equal to it.  The weights are read once, into shared memory, unless there are more than fit
+// (then the later sweeps read them from L2); the kept ones a second time.
+// Bound by latency: 64 CTAs of 16384 weights 28 us with the sweeps from L2 and one histogram, 13 so.
+__global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_constant__ EvictKernelParams p, int n_cached) {
+  extern __shared__ uint32_t s_keys[];  // [n_cached]
+  __shared__ int s_hist[2][kBins];      // (two: neighbouring lanes count apart where the weights are much alike)
   __shared__ int s_warp[kSelect / 32], s_warp_eq[kSelect / 32];
   __shared__ int s_digit, s_left;
+  griddep_launch();
   griddep_wait();
   const int b = blockIdx.x / p.c.hkv, h = blockIdx.x - b * p.c.hkv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -64,6 +75,12 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
   int* const kept = p.kept + static_cast<long long>(blockIdx.x) * p.budget;
   float* const new_w = p.new_weights + static_cast<long long>(blockIdx.x) * p.new_w_len;
   if (h == 0 && threadIdx.x == 0) p.new_lens[b] = keep;
+  const bool cached = len <= n_cached;
+  if (cached && len > p.budget) {
+#pragma unroll 8
+    for (int i = threadIdx.x; i < len; i += kSelect) s_keys[i] = order_key(w[i]);
+  }
+  const auto key_of = [&](int i) { return cached ? s_keys[i] : order_key(w[i]); };
   // candidates: slots [lo, hi), of which `left` stay
   int lo = 0, hi = len, left = len;
   uint32_t bound = 0;  // keys above it stay, and `left` of those equal to it
@@ -75,16 +92,17 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
 #pragma unroll
       for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass < 2 ? 2048 : 1024;
-        for (int i = threadIdx.x; i < bins; i += kSelect) s_hist[i] = 0;
+        for (int i = threadIdx.x; i < 2 * kBins; i += kSelect) s_hist[0][i] = 0;
         __syncthreads();
+#pragma unroll 4
         for (int i = lo + threadIdx.x; i < hi; i += kSelect) {
-          const uint32_t key = order_key(w[i]);
-          if ((key & mask) == bound) atomicAdd(&s_hist[(key >> shift) & (bins - 1)], 1);
+          const uint32_t key = key_of(i);
+          if ((key & mask) == bound) atomicAdd(&s_hist[lane & 1][(key >> shift) & (bins - 1)], 1);
         }
         __syncthreads();
         // the digit with which the count from above reaches `left`: every thread two bins, largest first
         const int at = bins - 1 - 2 * threadIdx.x;
-        const int c0 = at >= 1 ? s_hist[at] : 0, c1 = at >= 1 ? s_hist[at - 1] : 0;
+        const int c0 = at >= 1 ? s_hist[0][at] + s_hist[1][at] : 0, c1 = at >= 1 ? s_hist[0][at - 1] + s_hist[1][at - 1] : 0;
         int sum = c0 + c1;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
@@ -93,8 +111,7 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
         }
         if (lane == 31) s_warp[warp] = sum;
         __syncthreads();
-        int before = 0;
-        for (int i = 0; i < warp; ++i) before += s_warp[i];
+        const int before = sum_below(s_warp, warp);
         const int above = before + sum - c0 - c1;  // keys of larger digits
         if (at >= 1 && above < left && above + c0 + c1 >= left) {
           const bool first = above + c0 >= left;
@@ -116,18 +133,18 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
   const int piece = (len + kSelect / 32 * 32 - 1) / (kSelect / 32 * 32) * 32;
   const int begin = min(len, warp * piece), end = min(len, begin + piece);
   int n_above = 0, n_equal = 0;
+#pragma unroll 4
   for (int i = begin; i < end; i += 32) {
     const int slot = i + lane;
-    bool above = false, equal = false;
     if (slot < end) {
       const bool must = all || slot < lo || slot >= hi;
-      const uint32_t key = must ? 0 : order_key(w[slot]);
-      above = must || key > bound;
-      equal = !must && key == bound;
+      const uint32_t key = must ? 0 : key_of(slot);
+      n_above += must || key > bound;
+      n_equal += !must && key == bound;
     }
-    n_above += __popc(__ballot_sync(0xffffffffu, above));
-    n_equal += __popc(__ballot_sync(0xffffffffu, equal));
   }
+  n_above = __reduce_add_sync(0xffffffffu, n_above);
+  n_equal = __reduce_add_sync(0xffffffffu, n_equal);
   if (lane == 0) s_warp[warp] = n_above, s_warp_eq[warp] = n_equal;
   __syncthreads();
   int at = 0, equal_before = 0;
@@ -136,6 +153,7 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
     at += s_warp[i] + max(0, min(s_warp_eq[i], left - equal_before));
     equal_before += s_warp_eq[i];
   }
+#pragma unroll 4
   for (int i = begin; i < end; i += 32) {
     const int slot = i + lane;
     bool stays = false, equal = false;
@@ -143,7 +161,7 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
     if (slot < end) {
       x = w[slot];
       const bool must = all || slot < lo || slot >= hi;
-      const uint32_t key = order_key(x);
+      const uint32_t key = must ? 0 : key_of(slot);
       stays = must || key > bound;
       equal = !must && key == bound;
     }
@@ -163,94 +181,114 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
   for (int i = keep + threadIdx.x; i < p.new_w_len; i += kSelect) new_w[i] = 0.f;
 }
 
-// One CTA per new block, head and K or V: the kept rows (scattered, head_dim bytes each) are read once, stay in
-// registers while their largest magnitude is found, and are written at the new block's scale.
-// Bound by HBM: one byte in, one out per element.
+// A CTA packs `run` new blocks of a head, K and V (or one block, K or V, where there are too few for that): it looks all
+// their rows up first, then reads the rows of one block while it finds the largest magnitude of the one before and writes
+// it at its new scale.  A row is read once (head_dim bytes, scattered) and stays in registers.
+// Bound by HBM, one byte in and one out per element; what a CTA waits for before its first byte (length, kept slots,
+// block table, scales: four loads in a row) is paid once a run: 134 MB
+constexpr int kRun = 4;
 template <int kD, int kBs, bool kInt8>
-__global__ void __launch_bounds__(kPack) evict_pack_kernel(const __grid_constant__ EvictKernelParams p) {
+__global__ void __launch_bounds__(kPack) evict_pack_kernel(const __grid_constant__ EvictKernelParams p, int run) {
   constexpr int kCols = kD / 16;  // 16-byte pieces of a row
   constexpr int kPasses = (kBs * kCols + kPack - 1) / kPack;
-  __shared__ long long s_row[kBs];  // offset of the row, -1: none
-  __shared__ float s_scale[kBs];
-  __shared__ float s_max[kPack / 32];
-  __shared__ int s_nan;
-  const int j = blockIdx.x % p.new_max_blocks, b = blockIdx.x / p.new_max_blocks;
-  const int which = blockIdx.y & 1, h = blockIdx.y >> 1;
+  __shared__ int s_page[kRun * kBs], s_slot[kRun * kBs];  // block and head of a row (-1: none), token in the block
+  __shared__ float s_scale[2][kRun * kBs];
+  __shared__ float s_max[2][kPack / 32];
+  const int groups = (p.new_max_blocks + run - 1) / run;
+  const int b = blockIdx.x / groups, j0 = (blockIdx.x - b * groups) * run;
+  // which of K and V
+  const int h = run > 1 ? blockIdx.y : blockIdx.y >> 1, first = run > 1 ? 0 : blockIdx.y & 1, kinds = run > 1 ? 2 : 1;
   griddep_wait();
   const int keep = min(checked_len(p, b), p.budget);
-  const int rows = min(keep - j * kBs, kBs);
+  const int rows = min(keep - j0 * kBs, run * kBs);
   if (rows <= 0) return;
-  const int to = table_entry(p.new_table, p.new_table_stride, b, j, p.c.num_blocks, p.status, p.mirror);
-  if (to < 0) return;
-  const int* kept = p.kept + (static_cast<long long>(b) * p.c.hkv + h) * p.budget + static_cast<long long>(j) * kBs;
-  for (int r = threadIdx.x; r < kBs; r += kPack) {
-    long long at = -1;
-    float scale = 0.f;
-    if (r < rows) {
-      const int slot = kept[r];
-      const int page = table_entry(p.table, p.table_stride, b, slot / kBs, p.c.num_blocks, p.status, p.mirror);
-      if (page >= 0) {
-        at = static_cast<long long>(page) * p.c.hkv + h;
-        scale = p.c.scale[which][at];
-        at = at * kBs + slot % kBs;
+  const int* kept = p.kept + (static_cast<long long>(b) * p.c.hkv + h) * p.budget + static_cast<long long>(j0) * kBs;
+  for (int r = threadIdx.x; r < rows; r += kPack) {
+    const int slot = kept[r];
+    const int page = table_entry(p.table, p.table_stride, b, slot / kBs, p.c.num_blocks, p.status, p.mirror);
+    const int at = page < 0 ? -1 : page * p.c.hkv + h;
+    s_page[r] = at;
+    s_slot[r] = slot % kBs;
+    for (int k = 0; k < 2; ++k) s_scale[k][r] = at < 0 ? 0.f : p.c.scale[k][at];
+  }
+  __syncthreads();
+  const int units = (rows + kBs - 1) / kBs * kinds;  // (block, K or V)
+  const auto load = [&](int u, uint4 (&x)[kPasses]) {
+    const int base = u / kinds * kBs;
+    const uint8_t* const data = p.c.data[first + u % kinds];
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int at = i * kPack + threadIdx.x, row = base + at / kCols;
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (at < kBs * kCols && row < rows && s_page[row] >= 0)
+        x[i] = *reinterpret_cast<const uint4*>(data + (static_cast<long long>(s_page[row]) * kBs + s_slot[row]) * kD + at % kCols * 16);
+    }
+  };
+  const auto store = [&](int u, uint4 (&x)[kPasses]) {
+    const int j = u / kinds, base = j * kBs, which = first + u % kinds;
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int at = i * kPack + threadIdx.x, row = base + at / kCols;
+      if (at >= kBs * kCols || row >= rows) continue;
+      Largest<kInt8> m;
+      m.add(x[i].x), m.add(x[i].y), m.add(x[i].z), m.add(x[i].w);
+      // (a scale that is not finite makes the new block's NaN: infinity stands for that here)
+      const float scale = s_scale[which][row];
+      most = fmaxf(most, scale <= 3.4028235e38f ? m.value() * scale : INFINITY);
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+    float* const all = s_max[u & 1];
+    if ((threadIdx.x & 31) == 0) all[threadIdx.x >> 5] = most;
+    __syncthreads();
+    most = fmaxf(fmaxf(all[0], all[1]), fmaxf(all[2], all[3]));
+    const float after = scale_for<kInt8>(most);
+    const float inv = 1.f / after;
+    const int to = table_entry(p.new_table, p.new_table_stride, b, j0 + j, p.c.num_blocks, p.status, p.mirror);
+    if (to < 0) return;
+    const long long block = static_cast<long long>(to) * p.c.hkv + h;
+    if (threadIdx.x == 0) p.c.scale[which][block] = after;
+    uint4* const dst = reinterpret_cast<uint4*>(p.c.data[which] + block * kBs * kD);
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int at = i * kPack + threadIdx.x, row = base + at / kCols;
+      if (at >= kBs * kCols || row >= rows) continue;
+      if (after != after) {
+        dst[at] = make_uint4(0, 0, 0, 0);
+        continue;
       }
+      const Rescale<kInt8> to_new(s_scale[which][row] * inv);
+      dst[at] = make_uint4(to_new(x[i].x), to_new(x[i].y), to_new(x[i].z), to_new(x[i].w));
     }
-    s_row[r] = at;
-    s_scale[r] = scale;
-  }
-  if (threadIdx.x == 0) s_nan = 0;
-  __syncthreads();
-  uint4 x[kPasses];
-#pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int at = i * kPack + threadIdx.x, row = at / kCols;
-    x[i] = make_uint4(0, 0, 0, 0);
-    if (row < rows && s_row[row] >= 0) x[i] = *reinterpret_cast<const uint4*>(p.c.data[which] + s_row[row] * kD + at % kCols * 16);
-  }
-  float most = 0.f;
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int row = (i * kPack + threadIdx.x) / kCols;
-    if (row >= rows) continue;
-    uint32_t m = __vmaxu4(__vmaxu4(abs_bytes<kInt8>(x[i].x), abs_bytes<kInt8>(x[i].y)), __vmaxu4(abs_bytes<kInt8>(x[i].z), abs_bytes<kInt8>(x[i].w)));
-    m = __vmaxu4(m, m >> 16);
-    m = max(m & 0xffu, (m >> 8) & 0xffu);
-    const float scale = s_scale[row];
-    most = fmaxf(most, byte_to_float<kInt8>(m) * scale);
-    bad = bad || !(scale <= 3.4028235e38f);
-  }
-  if (bad) s_nan = 1;
-#pragma unroll
-  for (int d = 16; d > 0; d /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = most;
-  __syncthreads();
-  most = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-  const float after = s_nan != 0 ? __uint_as_float(0x7fffffffu) : scale_for<kInt8>(most);
-  const float inv = 1.f / after;
-  const long long block = static_cast<long long>(to) * p.c.hkv + h;
-  if (threadIdx.x == 0) p.c.scale[which][block] = after;
-  uint4* const dst = reinterpret_cast<uint4*>(p.c.data[which] + block * kBs * kD);
-#pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int at = i * kPack + threadIdx.x, row = at / kCols;
-    if (row >= rows) continue;
-    const float scale = s_scale[row];
-    if (after != after) x[i] = make_uint4(0, 0, 0, 0);
-    uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float4 f = to_float4<kInt8>(w[k]);
-      if (after == after) w[k] = to_bytes<kInt8>(f.x * scale * inv, f.y * scale * inv, f.z * scale * inv, f.w * scale * inv);
-    }
-    dst[at] = make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  uint4 x[2][kPasses];
+  load(0, x[0]);
+  for (int u = 0; u < units; u += 2) {
+    if (u + 1 < units) load(u + 1, x[1]);
+    store(u, x[0]);
+    if (u + 1 >= units) break;
+    if (u + 2 < units) load(u + 2, x[0]);
+    store(u + 1, x[1]);
   }
 }
 
+// The choosing kernel may use as much shared memory as it needs at most: set once per device.
+cudaError_t allow_shared(int bytes) {
+  if (bytes <= 24 * 1024) return cudaSuccess;  // (48 KB with what it has of fixed size need no permission)
+  static std::atomic<uint64_t> set{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (set.load(std::memory_order_relaxed) >> dev & 1))) return e;
+  e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCacheKeys * 4);
+  if (e == cudaSuccess && dev < 64) set.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return e;
+}
+
 template <int kD, int kBs>
-cudaError_t launch_pack(const EvictKernelParams& kp, dim3 grid, cudaStream_t s) {
-  return kp.c.kind == RSWA_CACHE_INT8 ? launch_kernel(evict_pack_kernel<kD, kBs, true>, grid, kPack, 0, s, true, kp)
-                                      : launch_kernel(evict_pack_kernel<kD, kBs, false>, grid, kPack, 0, s, true, kp);
+cudaError_t launch_pack(const EvictKernelParams& kp, dim3 grid, int run, cudaStream_t s) {
+  return kp.c.kind == RSWA_CACHE_INT8 ? launch_kernel(evict_pack_kernel<kD, kBs, true>, grid, kPack, 0, s, true, kp, run)
+                                      : launch_kernel(evict_pack_kernel<kD, kBs, false>, grid, kPack, 0, s, true, kp, run);
 }
 
 }  // namespace
@@ -304,20 +342,25 @@ extern "C" int rswa_cache_evict(const rswa_cache_evict_params_t* p, void* stream
   kp.status = p->status;
   kp.mirror = status_mirror(p->status);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t e = launch_kernel(evict_select_kernel, dim3(static_cast<unsigned>(items)), kSelect, 0, s, true, kp);
+  const int64_t keys = cap < kCacheKeys ? cap : kCacheKeys;
+  const int smem = static_cast<int>(keys) * 4;
+  cudaError_t e = allow_shared(smem);
+  if (e == cudaSuccess) e = launch_kernel(evict_select_kernel, dim3(static_cast<unsigned>(items)), kSelect, smem, s, true, kp, static_cast<int>(keys));
   if (e == cudaSuccess) count_launches(1);
   if (e == cudaSuccess && units > 0) {
-    const dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>(2 * p->cache.n_kv_heads));
+    // (four blocks, K and V, a CTA where that still gives every SM four CTAs)
+    const int run = units * p->cache.n_kv_heads >= 16LL * sm_count() ? kRun : 1;
+    const dim3 grid(static_cast<unsigned>(p->table.batch * ((p->new_table.max_blocks + run - 1LL) / run)), static_cast<unsigned>((run > 1 ? 1 : 2) * p->cache.n_kv_heads));
     const int key = p->cache.head_dim * 1000 + p->cache.block_size;
     switch (key) {
-      case 64016: e = launch_pack<64, 16>(kp, grid, s); break;
-      case 64032: e = launch_pack<64, 32>(kp, grid, s); break;
-      case 64064: e = launch_pack<64, 64>(kp, grid, s); break;
-      case 64128: e = launch_pack<64, 128>(kp, grid, s); break;
-      case 128016: e = launch_pack<128, 16>(kp, grid, s); break;
-      case 128032: e = launch_pack<128, 32>(kp, grid, s); break;
-      case 128064: e = launch_pack<128, 64>(kp, grid, s); break;
-      default: e = launch_pack<128, 128>(kp, grid, s); break;
+      case 64016: e = launch_pack<64, 16>(kp, grid, run, s); break;
+      case 64032: e = launch_pack<64, 32>(kp, grid, run, s); break;
+      case 64064: e = launch_pack<64, 64>(kp, grid, run, s); break;
+      case 64128: e = launch_pack<64, 128>(kp, grid, run, s); break;
+      case 128016: e = launch_pack<128, 16>(kp, grid, run, s); break;
+      case 128032: e = launch_pack<128, 32>(kp, grid, run, s); break;
+      case 128064: e = launch_pack<128, 64>(kp, grid, run, s); break;
+      default: e = launch_pack<128, 128>(kp, grid, run, s); break;
     }
     if (e == cudaSuccess) count_launches(1);
   }
