@@ -56,6 +56,7 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const __grid_con
   __shared__ uint32_t s_max[kThreads / 32];
   const int lane = threadIdx.x & 31;
   const int bs = p.c.bs;
+  griddep_launch();
   griddep_wait();
   // which block of which sequence: every warp counts the touched blocks of 32 sequences at a time (or divides)
   int b = 0, unit = blockIdx.x, n = 0, len = 0;
@@ -96,8 +97,7 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const __grid_con
     if (!found) return;
   }
   const int j = len / bs + unit;  // block of the sequence
-  const int page = table_entry(p.table, p.table_stride, b, j, p.c.num_blocks, p.status, p.mirror);
-  if (page < 0) return;
+  const int page = p.table[b * p.table_stride + j];  // (looked at below: the values do not wait for it)
   const int which = blockIdx.y & 1, h = blockIdx.y >> 1;
   const int first = max(len - j * bs, 0);                                   // slots before it hold older tokens
   const int end = static_cast<int>(min(static_cast<long long>(bs), static_cast<long long>(len) + n - static_cast<long long>(j) * bs));
@@ -119,6 +119,10 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const __grid_con
     most = __vmaxu2(most, __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu));
   }
   most = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
+  if (page < 0 || page >= p.c.num_blocks) {
+    raise_status(p.status, p.mirror, kErrBlockTable);
+    return;
+  }
   float* const scale_at = p.c.scale[which] + static_cast<long long>(page) * p.c.hkv + h;
   const float before = first > 0 ? *scale_at : 0.f;
   if (lane == 0) s_max[threadIdx.x >> 5] = most;
@@ -174,8 +178,10 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_const
   const int blocks = (p.rows + bs - 1) / bs;
   const int b = blockIdx.x / blocks, j = blockIdx.x - b * blocks;
   const int which = blockIdx.y & 1, h = blockIdx.y >> 1;
+  griddep_launch();
   griddep_wait();
   const int len_b = p.lens[b];
+  const int entry = j < p.max_blocks ? p.table[b * p.table_stride + j] : -1;  // (of no meaning behind the sequence's end)
   int len = min(len_b, p.rows);
   if (len_b < 0 || len_b > static_cast<long long>(p.max_blocks) * bs) {
     raise_status(p.status, p.mirror, kErrSeqLen);
@@ -186,12 +192,12 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_const
   float scale = 0.f;
   const uint8_t* src = nullptr;
   if (held > 0) {
-    const int page = table_entry(p.table, p.table_stride, b, j, p.c.num_blocks, p.status, p.mirror);
-    if (page >= 0) {
-      const long long at = static_cast<long long>(page) * p.c.hkv + h;
+    if (entry >= 0 && entry < p.c.num_blocks) {
+      const long long at = static_cast<long long>(entry) * p.c.hkv + h;
       scale = p.c.scale[which][at];
       src = p.c.data[which] + at * bs * kD;
     } else {
+      raise_status(p.status, p.mirror, kErrBlockTable);
       held = 0;
     }
   }

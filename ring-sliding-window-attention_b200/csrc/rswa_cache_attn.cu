@@ -769,34 +769,53 @@ __global__ void __launch_bounds__(kAdd) cache_weights_kernel(const __grid_consta
   const int t0 = (blockIdx.x - bh * chunks) * kWeightTiles;
   const int n = s.n - kOver;  // tiles
   if (t0 >= n) return;
-  for (int r = threadIdx.x; r < p.row_tiles * kRows; r += kAdd) {
-    float x = INFINITY;
-    if (r < p.rows) {
-      const int i = r / p.group;
-      x = p.lse[(static_cast<long long>(b) * p.hq + h * p.group + r - i * p.group) * p.q_len + i] * 1.4426950408889634f;
-      if (x == -INFINITY) x = INFINITY;
-    }
-    s_lse[r] = x;
-  }
-  __syncthreads();
+  // (what the loads below depend on is one step behind them: lengths and the sequence's first tile, then everything else)
   const int first = p.first[b] + h * p.row_tiles * s.n;
   const int t1 = min(t0 + kWeightTiles, n);
-  for (int k = t0 * kTok + threadIdx.x; k < t1 * kTok; k += kAdd) {
-    const int tile = k / kTok, tok = tile_slot(s, tile) + k % kTok;
-    if (tok >= s.len) continue;
-    float sum = 0.f;
-    for (int rt = 0; rt < p.row_tiles; ++rt) {
+  constexpr int kEach = kWeightTiles * kTok / kAdd;
+  float4 x[kEach][kRows / 4];
+  float old[kEach];
+  float* to[kEach];
+  const auto load = [&](int rt) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int k = t0 * kTok + e * kAdd + threadIdx.x, tile = k / kTok;
       const float4* from = reinterpret_cast<const float4*>(p.scores + (static_cast<long long>(first + rt * s.n + kOver + tile) * kTok + k % kTok) * kRows);
 #pragma unroll
-      for (int v = 0; v < kRows / 4; ++v) {
-        const float4 x = from[v];
-        const float* lse = s_lse + rt * kRows + v * 4;
-        sum += ex2f(x.x - lse[0]) + ex2f(x.y - lse[1]) + ex2f(x.z - lse[2]) + ex2f(x.w - lse[3]);
-      }
+      for (int v = 0; v < kRows / 4; ++v) x[e][v] = to[e] != nullptr ? from[v] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     }
-    float* const to = p.weights + b * p.w_sb + h * p.w_sh + tok;
-    *to += sum;
+  };
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int k = t0 * kTok + e * kAdd + threadIdx.x, tile = k / kTok, tok = tile_slot(s, tile) + k % kTok;
+    to[e] = tile < t1 && tok < s.len ? p.weights + b * p.w_sb + h * p.w_sh + tok : nullptr;
+    old[e] = to[e] != nullptr ? *to[e] : 0.f;
   }
+  load(0);
+  for (int r = threadIdx.x; r < p.row_tiles * kRows; r += kAdd) {
+    float l = INFINITY;
+    if (r < p.rows) {
+      const int i = r / p.group;
+      l = p.lse[(static_cast<long long>(b) * p.hq + h * p.group + r - i * p.group) * p.q_len + i] * 1.4426950408889634f;
+      if (l == -INFINITY) l = INFINITY;
+    }
+    s_lse[r] = l;
+  }
+  __syncthreads();
+  float sum[kEach] = {};
+  for (int rt = 0; rt < p.row_tiles; ++rt) {
+    if (rt > 0) load(rt);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+#pragma unroll
+      for (int v = 0; v < kRows / 4; ++v) {
+        const float* lse = s_lse + rt * kRows + v * 4;
+        sum[e] += ex2f(x[e][v].x - lse[0]) + ex2f(x[e][v].y - lse[1]) + ex2f(x[e][v].z - lse[2]) + ex2f(x[e][v].w - lse[3]);
+      }
+  }
+#pragma unroll
+  for (int e = 0; e < kEach; ++e)
+    if (to[e] != nullptr) *to[e] = old[e] + sum[e];
 }
 
 struct Plan {

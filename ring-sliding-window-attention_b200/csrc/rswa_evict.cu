@@ -49,6 +49,12 @@ __device__ __forceinline__ uint32_t order_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// the weight a key was made of (a NaN of any kind as the canonical one, -0 as 0)
+__device__ __forceinline__ float key_weight(uint32_t key) {
+  if (key == 0xffffffffu) return __uint_as_float(0x7fffffffu);
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
 // s[0] + ... + s[warp - 1], for all lanes of a warp (at most 32 values)
 __device__ __forceinline__ int sum_below(const int* s, int warp) {
   const int lane = threadIdx.x & 31;
@@ -58,10 +64,10 @@ __device__ __forceinline__ int sum_below(const int* s, int warp) {
 // One CTA per (sequence, head).  The k-th largest key between the sinks and the newest tokens is found digit by digit
 // (11, 11, 10 bits; a histogram of the candidates' digits each time), then two ordered sweeps write what is above it and
 // the first ones of those equal to it.  The weights are read once, into shared memory, unless there are more than fit
-// (then the later sweeps read them from L2); the kept ones a second time.
-// Bound by latency: 64 CTAs of 16384 weights 28 us with the sweeps from L2 and one histogram, 13 so.
+// (then the later sweeps read them from L2).  Bound by latency: 64 CTAs of 16384 weights 20 us with a slot a lane at
+// a time and the kept weights read again, 17 with four.
 __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_constant__ EvictKernelParams p, int n_cached) {
-  extern __shared__ uint32_t s_keys[];  // [n_cached]
+  extern __shared__ __align__(16) uint32_t s_keys[];  // [n_cached]
   __shared__ int s_hist[2][kBins];      // (two: neighbouring lanes count apart where the weights are much alike)
   __shared__ int s_warp[kSelect / 32], s_warp_eq[kSelect / 32];
   __shared__ int s_digit, s_left;
@@ -77,10 +83,14 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
   if (h == 0 && threadIdx.x == 0) p.new_lens[b] = keep;
   const bool cached = len <= n_cached;
   if (cached && len > p.budget) {
-#pragma unroll 8
+#pragma unroll 16
     for (int i = threadIdx.x; i < len; i += kSelect) s_keys[i] = order_key(w[i]);
   }
-  const auto key_of = [&](int i) { return cached ? s_keys[i] : order_key(w[i]); };
+  // the keys of four slots from a multiple of four on (behind the last one: anything)
+  const auto keys4 = [&](int i) {
+    if (cached) return *reinterpret_cast<const uint4*>(s_keys + i);
+    return make_uint4(order_key(w[i]), i + 1 < len ? order_key(w[i + 1]) : 0, i + 2 < len ? order_key(w[i + 2]) : 0, i + 3 < len ? order_key(w[i + 3]) : 0);
+  };
   // candidates: slots [lo, hi), of which `left` stay
   int lo = 0, hi = len, left = len;
   uint32_t bound = 0;  // keys above it stay, and `left` of those equal to it
@@ -94,10 +104,13 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass < 2 ? 2048 : 1024;
         for (int i = threadIdx.x; i < 2 * kBins; i += kSelect) s_hist[0][i] = 0;
         __syncthreads();
-#pragma unroll 4
-        for (int i = lo + threadIdx.x; i < hi; i += kSelect) {
-          const uint32_t key = key_of(i);
-          if ((key & mask) == bound) atomicAdd(&s_hist[lane & 1][(key >> shift) & (bins - 1)], 1);
+#pragma unroll 2
+        for (int i = 4 * threadIdx.x; i < hi; i += 4 * kSelect) {
+          const uint4 k4 = keys4(i);
+          const uint32_t keys[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (i + e >= lo && i + e < hi && (keys[e] & mask) == bound) atomicAdd(&s_hist[lane & 1][(keys[e] >> shift) & (bins - 1)], 1);
         }
         __syncthreads();
         // the digit with which the count from above reaches `left`: every thread two bins, largest first
@@ -130,52 +143,74 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
   }
   // Every warp takes a contiguous piece of all slots: how many of its tokens stay, then where they go.
   const bool all = len <= p.budget;
-  const int piece = (len + kSelect / 32 * 32 - 1) / (kSelect / 32 * 32) * 32;
+  constexpr int kStep = 128;  // slots of a warp at a time, four a lane
+  const int piece = (len + kSelect / 32 * kStep - 1) / (kSelect / 32 * kStep) * kStep;
   const int begin = min(len, warp * piece), end = min(len, begin + piece);
-  int n_above = 0, n_equal = 0;
-#pragma unroll 4
-  for (int i = begin; i < end; i += 32) {
-    const int slot = i + lane;
-    if (slot < end) {
-      const bool must = all || slot < lo || slot >= hi;
-      const uint32_t key = must ? 0 : key_of(slot);
-      n_above += must || key > bound;
-      n_equal += !must && key == bound;
+  // whether the slots i .. i + 3 stay for certain (bits 0 to 3), or if there is room for them (bits 8 to 11)
+  const auto stand = [&](int i, uint32_t (&keys)[4]) {
+    uint32_t r = 0;
+    if (i < end) {
+      if (!all) {
+        const uint4 k4 = keys4(i);
+        keys[0] = k4.x, keys[1] = k4.y, keys[2] = k4.z, keys[3] = k4.w;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int slot = i + e;
+        if (slot >= end) continue;
+        if (all || slot < lo || slot >= hi || keys[e] > bound) r |= 1u << e;
+        else if (keys[e] == bound) r |= 256u << e;
+      }
     }
+    return r;
+  };
+  int n_above = 0, n_equal = 0;
+  for (int i = begin + 4 * lane; i - 4 * lane < end; i += kStep) {
+    uint32_t keys[4] = {0, 0, 0, 0};
+    const uint32_t r = stand(i, keys);
+    n_above += __popc(r & 15u);
+    n_equal += __popc(r >> 8);
   }
   n_above = __reduce_add_sync(0xffffffffu, n_above);
   n_equal = __reduce_add_sync(0xffffffffu, n_equal);
   if (lane == 0) s_warp[warp] = n_above, s_warp_eq[warp] = n_equal;
   __syncthreads();
-  int at = 0, equal_before = 0;
-  for (int i = 0; i < warp; ++i) {
-    // (of the equal ones, those in front take the room first)
-    at += s_warp[i] + max(0, min(s_warp_eq[i], left - equal_before));
-    equal_before += s_warp_eq[i];
-  }
-#pragma unroll 4
-  for (int i = begin; i < end; i += 32) {
-    const int slot = i + lane;
-    bool stays = false, equal = false;
-    float x = 0.f;
-    if (slot < end) {
-      x = w[slot];
-      const bool must = all || slot < lo || slot >= hi;
-      const uint32_t key = must ? 0 : key_of(slot);
-      stays = must || key > bound;
-      equal = !must && key == bound;
+  // (of the equal ones, those in front take the room first)
+  int equal_before = sum_below(s_warp_eq, warp);
+  int at = sum_below(s_warp, warp) + min(equal_before, left);
+  const uint32_t before = (1u << lane) - 1;
+  for (int i = begin + 4 * lane; i - 4 * lane < end; i += kStep) {
+    uint32_t keys[4] = {0, 0, 0, 0};
+    uint32_t r = stand(i, keys);
+    // how many of the lanes in front of this one: four votes each, since a lane has four slots
+    int equal_here = 0, equal_all = 0;
+    if (__any_sync(0xffffffffu, r >> 8)) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t v = __ballot_sync(0xffffffffu, r >> (8 + e) & 1u);
+        equal_here += __popc(v & before);
+        equal_all += __popc(v);
+      }
+      int n = equal_before + equal_here;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (r >> (8 + e) & 1u) r |= (n++ < left ? 1u : 0u) << e;
     }
-    const uint32_t before = (1u << lane) - 1;
-    const uint32_t equals = __ballot_sync(0xffffffffu, equal);
-    stays = stays || (equal && equal_before + __popc(equals & before) < left);
-    const uint32_t stay = __ballot_sync(0xffffffffu, stays);
-    if (stays) {
-      const int to = at + __popc(stay & before);
-      kept[to] = slot;
-      if (to < p.new_w_len) new_w[to] = x;
+    int to = at;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t v = __ballot_sync(0xffffffffu, r >> e & 1u);
+      to += __popc(v & before);
+      at += __popc(v);
     }
-    at += __popc(stay);
-    equal_before += __popc(equals);
+    equal_before += equal_all;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (r >> e & 1u) {
+        kept[to] = i + e;
+        if (to < p.new_w_len) new_w[to] = cached && !all ? key_weight(keys[e]) : w[i + e];
+        ++to;
+      }
   }
   for (int i = keep + threadIdx.x; i < p.budget; i += kSelect) kept[i] = -1;
   for (int i = keep + threadIdx.x; i < p.new_w_len; i += kSelect) new_w[i] = 0.f;
@@ -198,6 +233,7 @@ __global__ void __launch_bounds__(kPack) evict_pack_kernel(const __grid_constant
   const int b = blockIdx.x / groups, j0 = (blockIdx.x - b * groups) * run;
   // which of K and V
   const int h = run > 1 ? blockIdx.y : blockIdx.y >> 1, first = run > 1 ? 0 : blockIdx.y & 1, kinds = run > 1 ? 2 : 1;
+  griddep_launch();
   griddep_wait();
   const int keep = min(checked_len(p, b), p.budget);
   const int rows = min(keep - j0 * kBs, run * kBs);
