@@ -166,9 +166,10 @@ thread_local RowsCache t_rows_cache;
 int make_rows_map(CUtensorMap* map, const void* base, long long rows, int row_bytes, int box_rows) {
   EncodeTiledFn enc = get_encode();
   if (!enc) return RSWA_E_CUDA;
-  static thread_local bool t_context_bound = false;  // (see make_tile_map)
+  static thread_local bool t_context_bound = false;  // (see make_tile_map; this way is allowed inside a stream capture too)
   if (!t_context_bound) {
-    cudaFree(nullptr);
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaSetDevice(dev);
     t_context_bound = true;
   }
   const RowsKey key{base, rows, row_bytes, box_rows};

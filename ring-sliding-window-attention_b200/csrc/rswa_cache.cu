@@ -298,7 +298,7 @@ CacheView cache_view(const rswa_cache_t& c) {
 }
 
 int check_table(const rswa_block_table_t& t, const int32_t* lens, const int32_t* status, int block_size, const char* what) {
-  if (t.batch < 0 || t.max_blocks < 0 || (t.batch > 0 && (t.entries == nullptr || lens == nullptr)) || status == nullptr) {
+  if (t.batch < 0 || t.max_blocks < 0 || (t.batch > 0 && ((t.entries == nullptr && t.max_blocks > 0) || lens == nullptr)) || status == nullptr) {
     set_error("%s: block table, lens and status are required", what);
     return RSWA_E_ARG;
   }

@@ -569,3 +569,163 @@ def test_prompt_then_steps_then_eviction_then_steps():
         for i, n in enumerate(ref_lens):
             assert torch.equal(x[i, :n].cpu(), R.rows(ref, name, new_table[i], n).bfloat16())
             assert not x[i, n:].any()
+
+
+def test_blocks_beyond_32_bit_offsets():
+    """A cache of 5 GB per K and V, used at its far end: every operator's addresses."""
+    ops = _ops()
+    blocks, heads, bs, d = 40000, 8, 128, 128
+    free, _ = torch.cuda.mem_get_info()
+    if free < 24 << 30:
+        pytest.skip("needs 24 GB")
+    cache = ops.KVCache.empty(blocks, heads, bs, d, dtype=torch.float8_e4m3fn)
+    lens = [300, 130]
+    table = torch.tensor([[blocks - 1, 39000, blocks - 2], [32768, 17, -1]], dtype=torch.int32)
+    new_table = torch.tensor([[blocks - 5], [blocks - 4]], dtype=torch.int32)
+    k, v = (normal(sum(lens), heads, d, seed=i, dt="bf16") for i in (0, 1))
+    cu = torch.tensor([0, 300, 430], dtype=torch.int32).cuda()
+    n = torch.tensor(lens, dtype=torch.int32).cuda()
+    ops.cache_append(cache, k.cuda(), v.cuda(), table.cuda(), n * 0, cu_seqlens=cu)
+    # the same in a small cache
+    small = ops.KVCache.empty(8, heads, bs, d, dtype=torch.float8_e4m3fn)
+    names = {blocks - 1: 0, 39000: 1, blocks - 2: 2, 32768: 3, 17: 4, -1: -1, blocks - 5: 5, blocks - 4: 6}
+    s_table, s_new = (torch.tensor([[names[x] for x in row] for row in t.tolist()], dtype=torch.int32).cuda() for t in (table, new_table))
+    ops.cache_append(small, k.cuda(), v.cuda(), s_table, n * 0, cu_seqlens=cu)
+    q = normal(2, 2, 16, d, seed=5, dt="bf16").cuda()
+    w = torch.zeros(2, heads, 3 * bs, device="cuda")
+    ws = w.clone()
+    assert torch.equal(ops.cache_attn(q, cache, table.cuda(), n, weights=w), ops.cache_attn(q, small, s_table, n, weights=ws))
+    assert torch.equal(w, ws)
+    a = ops.cache_evict(cache, table.cuda(), n, w, 100, new_table.cuda(), 4, 10)
+    b = ops.cache_evict(small, s_table, n, ws, 100, s_new, 4, 10)
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+    for t, st, ln in ((table.cuda(), s_table, n), (new_table.cuda(), s_new, a[0])):
+        for x, y in zip(ops.cache_read(cache, t, ln, 300), ops.cache_read(small, st, ln, 300)):
+            assert torch.equal(x, y) and torch.isfinite(x).all()
+
+
+def test_calls_on_two_streams_at_once():
+    """Eager calls that overlap on the GPU share nothing: long ones whose pieces are joined, on two streams, many times."""
+    ops = _ops()
+    lens, bs, d = [9000], 64, 128
+    runs = []
+    for seed in (0, 1):
+        cache, table, _, _, _ = filled("int8", "bf16", lens, 2, bs, d, seed=seed)
+        q = normal(1, 1, 8, d, seed=seed + 7, dt="bf16").cuda()
+        args = (q, cache, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
+        runs.append((args, ops.cache_attn(*args), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(40):
+        for (args, _, stream), got in zip(runs, outs):
+            with torch.cuda.stream(stream):
+                got.append(ops.cache_attn(*args))
+    torch.cuda.synchronize()
+    for (_, want, _), got in zip(runs, outs):
+        assert all(torch.equal(x, want) for x in got)
+
+
+def test_a_first_call_of_a_thread_inside_a_capture():
+    import threading
+    ops = _ops()
+    lens = [500, 20]
+    cache, table, _, _, _ = filled("e4m3", "fp16", lens, 2, 32, 64, seed=3)
+    q = normal(2, 1, 4, 64, seed=4, dt="fp16").cuda()
+    args = (q, cache, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
+    want = ops.cache_attn(*args)
+    torch.cuda.synchronize()
+    got, errors = [], []
+
+    def work():
+        try:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=torch.cuda.Stream()):
+                out = ops.cache_attn(*args)
+            out.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            got.append(out.clone())
+            g.replay()
+            torch.cuda.synchronize()
+            got.append(out.clone())
+            del g
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    assert not errors, errors
+    assert all(torch.equal(x, want) for x in got) and len(got) == 2
+
+
+def test_shared_prefix_and_empty_calls():
+    ops = _ops()
+    heads, bs, d = 2, 16, 64
+    cache = make("int8", 10, heads, bs, d, seed=0)
+    k, v = (normal(1, 2 * bs, heads, d, seed=i, dt="bf16") for i in (0, 1))
+    zero = torch.zeros(1, dtype=torch.int32).cuda()
+    ops.cache_append(cache, k.cuda(), v.cuda(), torch.tensor([[3, 7]], dtype=torch.int32).cuda(), zero)
+    table = torch.tensor([[3, 7, 1], [3, 7, 2], [3, 7, -1]], dtype=torch.int32)  # three sequences that begin alike
+    new = normal(2, 1, heads, d, seed=5, dt="bf16").cuda()
+    ops.cache_append(cache, new, new, table[:2].cuda(), zero.expand(2).contiguous() + 2 * bs)
+    lens = [2 * bs + 1, 2 * bs + 1, 2 * bs]
+    q = normal(3, 1, 4, d, seed=6, dt="bf16")
+    check_attn(cache, table, lens, q, None, 0, weights=torch.zeros(3, heads, 3 * bs))
+    before = host(cache)
+    none = torch.zeros(0, 3, dtype=torch.int32).cuda()
+    n = torch.tensor(lens, dtype=torch.int32).cuda()
+    assert ops.cache_attn(q[:0].cuda(), cache, none, n[:0]).shape == (0, 1, 4, d)
+    assert ops.cache_attn(q[:, :0].cuda(), cache, table.cuda(), n).shape == (3, 0, 4, d)
+    out = ops.cache_attn(q.cuda(), cache, torch.zeros(3, 0, dtype=torch.int32).cuda(), n * 0)
+    assert not out.any()
+    assert [x.shape[1] for x in ops.cache_read(cache, table.cuda(), n, 0)] == [0, 0]
+    ops.cache_append(cache, new[:, :0], new[:, :0], table[:2].cuda(), n[:2])
+    ops.cache_append(cache, new[:0, 0], new[:0, 0], table.cuda(), n, cu_seqlens=torch.zeros(4, dtype=torch.int32).cuda())
+    assert ops.attn_weight_sums(q[:, :0].cuda(), q[:, :0, :2].cuda(), torch.zeros(3, 4, 0).cuda()).shape == (3, 2, 0)
+    assert [x.shape[0] for x in ops.cache_evict(cache, none, n[:0], torch.zeros(0, heads, 48).cuda(), 8, none)] == [0, 0, 0]
+    after = host(cache)
+    for name in before:
+        torch.testing.assert_close(after[name], before[name], rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+def test_queries_that_are_not_finite_spoil_their_rows_alone(dt):
+    ops = _ops()
+    lens = [400]
+    cache, table, _, _, _ = filled("int8", dt, lens, 2, 32, 128, seed=1)
+    q = normal(1, 3, 8, 128, seed=2, dt=dt)
+    args = (cache, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
+    want = ops.cache_attn(q.cuda(), *args)
+    q[0, 1, 2, 5], q[0, 2, 7, 100] = math.nan, math.nan
+    got = ops.cache_attn(q.cuda(), *args)
+    bad = torch.zeros(1, 3, 8, dtype=torch.bool)
+    bad[0, 1, 2] = bad[0, 2, 7] = True
+    assert torch.isnan(got[bad.cuda()]).all() and torch.equal(got[~bad.cuda()], want[~bad.cuda()])
+    # in the sums a NaN spoils the keys its query sees
+    qs, ks = normal(1, 300, 2, 128, seed=3, dt=dt), normal(1, 300, 1, 128, seed=4, dt=dt)
+    lse = torch.full((1, 2, 300), 5.0)
+    qs[0, 200, 1, 3] = math.nan
+    w = ops.attn_weight_sums(qs.cuda(), ks.cuda(), lse.cuda(), 50)
+    nan = torch.isnan(w[0, 0]).cpu()
+    assert nan[150:201].all() and not nan[:150].any() and not nan[201:].any()
+
+
+def test_weight_sums_of_a_batch_with_strides_and_long_prompts():
+    """q, k and lse as slices; a prompt whose items are cut between SMs in every way; against the attention over a cache."""
+    ops = _ops()
+    b, s, hq, hkv, d, window, sink = 2, 2500, 4, 2, 64, 300, 3
+    fused = normal(b, s, hq + 2 * hkv, d, seed=1, dt="bf16").cuda()
+    q, k = fused[:, :, :hq], fused[:, :, hq:hq + hkv]
+    scores = torch.einsum("bihgd,bjhd->bhgij", q.reshape(b, s, hkv, hq // hkv, d).double(), k.double()) * d ** -0.5
+    i, j = torch.arange(s, device="cuda")[:, None], torch.arange(s, device="cuda")[None]
+    seen = (j <= i) & ((i - j <= window) | (j < sink))
+    lse64 = scores.masked_fill(~seen, -math.inf).logsumexp(-1)                    # [b, hkv, group, i]
+    lse = torch.zeros(b, hq, 2 * s, device="cuda")[:, :, 5:5 + s]
+    lse.copy_(lse64.reshape(b, hq, s))
+    want = (scores - lse.double().reshape(b, hkv, -1, s)[..., None]).exp().masked_fill(~seen, 0).sum((2, 3))
+    got = ops.attn_weight_sums(q, k, lse, window, sink)
+    assert ((got.double() - want).abs() <= 4e-5 * want).all()   # (128 terms in 32 bits: 128 * 2^-24; scores 72 * 2^-24 * 30)
+    got = ops.attn_weight_sums(q[:, :, :1], k[:, :, :1].expand(b, s, 1, d), lse[:, :1], None)
+    assert got.shape == (b, 1, s)
