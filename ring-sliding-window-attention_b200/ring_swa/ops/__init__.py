@@ -22,6 +22,7 @@ from .attn import (
     flash_attn_varlen_bwd_func,
 )
 from .merge import merge_attn_out
+# (not in __all__, which is the reference's list of names)
 from .kv_cache import (
     KVCache,
     cache_append,
@@ -46,10 +47,4 @@ __all__ = [
     "flash_attn_varlen_bwd_func",
     "merge_attn_out",
     "get_group_local_to_global_rank_map",
-    "KVCache",
-    "cache_append",
-    "cache_read",
-    "cache_attn",
-    "cache_evict",
-    "attn_weight_sums",
 ]
