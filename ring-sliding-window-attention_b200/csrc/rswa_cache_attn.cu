@@ -212,12 +212,13 @@ struct Ring {
   static constexpr int kStageBytes = 2 * kTileBytes;
 };
 
-// 16 warps of 128 registers a thread, or for 16 query rows 12 of 168.  A tile in flight per warp is 96 KB or more, where
-// the latency of a load asks for about 50.
+// 16 warps of 128 registers a thread, or for 16 query rows 8 of 255 (12 of 168 spill: 4 x 128k tokens with sinks, 4 queries:
+// 32 us, and 28.6 so; a second tile in flight per warp then gives nothing).  A tile in flight per warp is 128 KB or 64 an SM,
+// where the latency of a load asks for about 50.
 // kAll: all warps are one group.
 template <int kD, int kNT, bool kAll>
 struct Layout {
-  static constexpr int kWarps = kNT == 1 ? 16 : 12;
+  static constexpr int kWarps = kNT == 1 ? 16 : 8;
   static constexpr int kThreads = kWarps * 32, kGroup = kAll ? kWarps : 4, kGroups = kWarps / kGroup;
   struct Ctl {
     uint64_t full[kWarps][2];           // K, V
@@ -399,16 +400,18 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
     }
     __syncwarp();
   };
-  auto look_up_scales = [&]() {
+  float scale[2][2];  // K's and V's, of the first 16 tokens and the last 16
+  auto fetch_scales = [&]() {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      float4 sc = make_float4(1.f, 0.f, 1.f, 0.f);
-      if (16 * t < tokens) {  // (tokens behind the end: their block may not even have a scale)
-        const float sv = p.c.scale[1][page[t]];
-        sc = make_float4(p.c.scale[0][page[t]], __log2f(sv), 1.f / sv, 0.f);
-      }
-      ctl.scale[warp][lane][t] = sc;
+      const bool some = 16 * t < tokens;  // (tokens behind the end: their block may not even have a scale)
+      scale[0][t] = some ? p.c.scale[0][page[t]] : 1.f;
+      scale[1][t] = some ? p.c.scale[1][page[t]] : 1.f;
     }
+  };
+  auto put_scales = [&]() {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) ctl.scale[warp][lane][t] = make_float4(scale[0][t], __log2f(scale[1][t]), 1.f / scale[1][t], 0.f);
     __syncwarp();
   };
   int loaded[2] = {0, 0};  // loads so far
@@ -426,7 +429,8 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
     while (i < n_own) {
       if ((i & 31) == 0 && i > 0) {
         look_up(i);
-        look_up_scales();
+        fetch_scales();
+        put_scales();
       }
       if (ctl.row[warp][i & 31].x >= 0) break;
       ++i;
@@ -458,16 +462,19 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
       for (int s = 0; s < kKS; ++s) raw[nt][s] = row < p.rows ? *reinterpret_cast<const uint2*>(src + s * 16) : make_uint2(0, 0);
     }
   };
+  // (Queries and scales are asked for in front of the first tiles: behind them they would wait until 20 MB have
+  // arrived, 2 to 3 us.)
+  next_piece(begin);
+  fetch_queries();
   if (n_own > 0) {
     look_up(0);
+    fetch_scales();
     while (own_i < min(n_own, 32) && ctl.row[warp][own_i].x < 0) ++own_i;
     if (own_i < min(n_own, 32)) {
       load(own_i, 0);
       load(own_i, 1);
     }
-    next_piece(begin);
-    if (kNT == 1) fetch_queries();
-    look_up_scales();
+    put_scales();
     if (own_i == 32) {  // (none of them is there: sequences of hardly any tokens)
       own_i = advance(own_i);
       if (own_i < n_own) {
@@ -475,14 +482,10 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
         load(own_i, 1);
       }
     }
-  } else {
-    next_piece(begin);
-    if (kNT == 1) fetch_queries();
   }
   bool dead = false;
   while (cc.at < end) {
     const int h = cc.item / p.row_tiles, row0 = (cc.item - h * p.row_tiles) * kRows;
-    if (kNT > 1) fetch_queries();
     uint32_t qf[kNT][kKS][2];
     float rs[kNT][2];  // factor of the scores of rows 2c, 2c + 1, log2(e) in it
 #pragma unroll
@@ -745,6 +748,7 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
       sync_group<kPeers>(group);
       if (ctl.last[group] != 0) join_pieces<kD, kNT, kPeers>(p, merge, group, b, h, row0, lo, pieces);
     }
+    if (kNT > 1) fetch_queries();
   }
   if (dead) {
     // copies still on their way must not outlive the CTA's shared memory (each wait is limited)
