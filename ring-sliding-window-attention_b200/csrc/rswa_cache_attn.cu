@@ -4,8 +4,11 @@
 //
 // in one pass over K and V: running maximum and sum per row, K and V brought in by TMA and never in any form but the
 // stored bytes until they are operands.  What has to be moved is 2 * head_dim bytes per visible token and key/value
-// head, 1/64 of what a 16-bit, ungrouped cache of 32 heads on 8 would need; the products are 4 * head_dim FLOPs per
-// query head on them, at 8 query heads 32 per byte: HBM-bound by a factor of 8 on the tensor cores, but not on the FMA pipe.
+// head; the products are 4 * head_dim FLOPs on them per query head, 16 a byte with 8 of them: 105 TFLOP/s at the rate of
+// HBM, which is more than the FMA pipe gives and a fifth of what mma.m16n8k16 does (8 cycles each, measured).
+// Streaming runs at 5 to 6 TB/s; what is left is the way in (lengths, block table, first tiles: 5 us), the end of the
+// pieces and their joining (4 us), and that SMs get unequal shares of the bandwidth (the last group ends 8 us behind
+// the median one of 40).  161 MB (32 requests of 300 to 8192 tokens, 32/8 heads, e4m3) 39.5 us: 4.1 TB/s.
 //
 // Products: mma.m16n8k16 with the KEYS (the V columns) as the 16 rows and the query rows as the 8 columns, so that a
 // group of up to 8 rows wastes nothing on the operand that costs: the one converted from bytes.  (tcgen05 wants 128
@@ -18,16 +21,15 @@
 // P^T comes out of S^T's accumulators by two 8x8 transposes (movmatrix) per 16 tokens.
 //
 // Queries and weights are fp16 operands: a bf16 query is scaled by a power of two to the top of the fp16 range (exact
-// but for elements 2^-30 smaller than the row's largest), the weights are at most 2^14 with 11 bits each.  The scale of
+// but for elements 2^-28 smaller than the row's largest), the weights are at most 2^14 with 11 bits each.  The scale of
 // a V block goes into its tokens' exponents (s + log2 of the scale), so that the running reference covers both;
 // the sum of the weights takes it back out.  Scores, sums and the output are 32-bit.
 //
 // Work: the 32-token tiles of all (sequence, key/value head, 8 or 16 query rows) in one order, cut evenly whatever the
 // lengths over groups of warps.  The warps of a group take its tiles in turn and add up at the end of each piece; each item
-// counts one tile per warp more than it has, for that and for its queries (32 requests of 300 to 8192 tokens: the last
-// group ended 13 us behind the median one without, 4 us with it).  Where there
-// are more (sequence, head, row tile)s than SMs a group is four warps, because the end of a piece and the next one's queries
-// cost every warp that takes part as much as several tiles (32 requests of 300 to 8192 tokens, 8 heads: 48 us, and 69 with
+// counts one tile per warp more than it has, for that and for its queries (32 requests of 300 to 8192 tokens: 43.6 us
+// without, 40 with it).  Where there are more (sequence, head, row tile)s than SMs a group is four warps, because the end of a piece and the next one's queries
+// cost every warp that takes part as much as several tiles (the same requests: 48 us, and 69 with
 // all 16 warps of an SM in one group); else it is all warps of the SM, which leaves fewer pieces to join.
 // Every warp loads for itself: K of its next tile as soon as the scores are formed, V as soon as the output is, on over
 // sequence boundaries; its lanes look 32 tiles up in the block table at a time, so that the table's latency is paid once for
