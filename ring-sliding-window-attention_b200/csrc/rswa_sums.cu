@@ -62,7 +62,8 @@ __device__ __forceinline__ int item_q_tiles(const SumsKernelParams& p, int kt) {
   // (a tile that holds a sink token of the sequence that goes on behind it: all of that sequence)
   const bool sink = p.n_sink > 0 && t0 - s < p.n_sink;
   const int last = sink || e - 1 - t_last <= p.window ? e - 1 : t_last + p.window;
-  return last / kTile - t0 / kTile + 1;
+  // (at least one: boundaries that are not in order must not send the walk over the items astray)
+  return max(1, last / kTile - t0 / kTile + 1);
 }
 
 // prefix sums of the items' query tiles, by the first kScan threads; s_prefix[kScan] is the sum

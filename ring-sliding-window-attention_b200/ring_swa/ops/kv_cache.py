@@ -65,7 +65,7 @@ class KVCache:
     cache_append and cache_evict write scales that are powers of two, the least ones that hold a block's values: moving
     a token to another block or reading it back rounds nothing that the other scale can hold.  int8 has the smaller error
     where a block's values are of one magnitude, float8_e4m3fn where they are not.  Tensors filled elsewhere may have
-    any positive scales.
+    any positive scales (and no NaN among float8_e4m3fn values: a NaN belongs into the scale).
     """
     __slots__ = ("k", "v", "k_scale", "v_scale")
 
@@ -142,7 +142,8 @@ def attn_weight_sums(q: torch.Tensor, k: torch.Tensor, softmax_lse: torch.Tensor
     q [batch, tokens, num_q_heads, head_dim], k [batch, tokens, num_kv_heads, head_dim], bf16 or fp16, head_dim 64 or 128;
     packed [tokens, heads, head_dim] with cu_seqlens (int32, on the device).  The mask is that of cache_attn (and of
     ring_streaming_llm_attn on one GPU); softmax_lse [batch, num_q_heads, tokens] (packed [num_q_heads, tokens]) float32 is
-    the log-sum-exp of the same attention, as wrapped_flash_attn_fwd and torch.ops.ring_swa.swa_fwd return it.
+    the log-sum-exp of the same attention, as wrapped_flash_attn_fwd and torch.ops.ring_swa.swa_fwd return it (for heads of
+    64 elements: of q, k and v padded with zeros to 128, at the scale of 64).
     """
     return _call("weight_sums", q.device, q, k, softmax_lse, window_size, num_sink_tokens, softmax_scale, cu_seqlens)
 
