@@ -105,11 +105,12 @@ __device__ __forceinline__ SeqTiles seq_tiles(const AttnKernelParams& p, int b) 
 }
 __device__ __forceinline__ int tile_slot(const SeqTiles& s, int i) { return (i < s.n_sink_tiles ? i : s.first + i - s.n_sink_tiles) * kTok; }
 
-// Where the work of a group begins and ends: equal shares of all tiles, none of fewer than a tile per warp.
+// Where the work of a group begins and ends: equal shares of all tiles.  Not more of them than there is a tile per warp for,
+// but one for each item at least: a group that takes short items one after the other pays for each of them.
 struct Shares {
   int n, each, more;  // `more` shares have each + 1 tiles, the others each
-  __device__ __forceinline__ Shares(int total, int groups, int least) {
-    n = min(groups, max(1, total / least));
+  __device__ __forceinline__ Shares(int total, int groups, int items, int over, int warps) {
+    n = max(1, min(min(groups, total), max(items, (total - items * over) / warps)));
     each = total / n;
     more = total - each * n;
   }
@@ -368,7 +369,7 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
   griddep_wait();
   tile_prefix<kOver>(p, ctl.prefix, ctl.prefix + kScan + 1);
   const int total = ctl.prefix[kScan] * p.c.hkv * p.row_tiles;
-  const Shares shares(total, p.groups, kOver + kGroup);
+  const Shares shares(total, p.groups, p.batch * p.c.hkv * p.row_tiles, kOver, kGroup);
   if (me >= shares.n || total == 0) {
     if (group == 0) empty_rows<kD, kPeers>(p);
     return;
@@ -861,7 +862,7 @@ int make_plan(const rswa_cache_attn_params_t& a, Plan& plan) {
     set_error("rswa_cache_attn: too many tokens in one call");
     return RSWA_E_UNSUPPORTED;
   }
-  const long long shares = items * most / (2 * plan.over), most_groups = plan.all ? sms : static_cast<long long>(sms) * warps / 4;
+  const long long by_tiles = items * plan.most_tiles / plan.over, shares = by_tiles > items ? by_tiles : items, most_groups = plan.all ? sms : static_cast<long long>(sms) * warps / 4;
   plan.groups = static_cast<int>(shares < 1 ? 1 : shares < most_groups ? shares : most_groups);
   if (plan.groups > RSWA_CACHE_ATTN_COUNTERS) plan.groups = RSWA_CACHE_ATTN_COUNTERS;
   plan.ctas = plan.groups < sms ? plan.groups : sms;
