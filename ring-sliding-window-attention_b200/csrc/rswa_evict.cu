@@ -86,6 +86,7 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
 #pragma unroll 16
     for (int i = threadIdx.x; i < len; i += kSelect) s_keys[i] = order_key(w[i]);
   }
+  __syncthreads();
   // the keys of four slots from a multiple of four on (behind the last one: anything)
   const auto keys4 = [&](int i) {
     if (cached) return *reinterpret_cast<const uint4*>(s_keys + i);
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
 // their rows up first, then reads the rows of one block while it finds the largest magnitude of the one before and writes
 // it at its new scale.  A row is read once (head_dim bytes, scattered) and stays in registers.
 // Bound by HBM, one byte in and one out per element; what a CTA waits for before its first byte (length, kept slots,
-// block table, scales: four loads in a row) is paid once a run: 134 MB
+// block table, scales: four loads in a row) is paid once a run: 134 MB in, 134 MB out take 57 us, 41 at a copy's rate.
 constexpr int kRun = 4;
 template <int kD, int kBs, bool kInt8>
 __global__ void __launch_bounds__(kPack) evict_pack_kernel(const __grid_constant__ EvictKernelParams p, int run) {

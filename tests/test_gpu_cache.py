@@ -427,6 +427,7 @@ EVICT = [
     ([100, 90], 2, 64, 32, 500, 4, 100),              # nothing to do
     ([5000, 33], 1, 64, 16, 1, 0, 0),
     ([70000], 1, 64, 128, 20000, 4, 1000),
+    ([16000, 9100], 2, 64, 16, 9000, 100, 8900),      # sinks and newest alone, of many
 ]
 
 
