@@ -220,22 +220,35 @@ void count_launches(int n);             // kernels of this library launched (rsw
 int sm_count();  // SMs of the current device (cached per device)
 
 // A launch that may start before the kernel in front of it on the stream has finished (`early`; the kernel then
-// waits with griddep_wait), or an ordinary one.
+// waits with griddep_wait), or an ordinary one, in clusters of `cluster` CTAs.
 template <typename... Params, typename... Args>
-cudaError_t launch_kernel(void (*kern)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, bool early, Args... args) {
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
+cudaError_t launch_clusters(void (*kern)(Params...), dim3 grid, int cluster, int threads, size_t smem, cudaStream_t stream, bool early, Args... args) {
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (early) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = early ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = static_cast<unsigned>(n);
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<Params>(args)...);
   if (e != cudaSuccess) cudaGetLastError();  // (reported here, not by whoever asks next)
   return e;
+}
+template <typename... Params, typename... Args>
+cudaError_t launch_kernel(void (*kern)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, bool early, Args... args) {
+  return launch_clusters(kern, grid, 1, threads, smem, stream, early, args...);
 }
 
 }  // namespace rswa

@@ -11,9 +11,11 @@ int check_table(const rswa_block_table_t& t, const int32_t* lens, const int32_t*
 namespace {
 
 constexpr int kSelect = 1024;     // threads of a choosing CTA
-constexpr int kBins = 2048;       // of a radix pass: 11, 11 and 10 bits
+constexpr int kDigits = 3;        // of a key: 11, 11 and 10 bits
 constexpr int kPack = 128;        // threads of a packing CTA
-constexpr int kCacheKeys = 49152; // keys that a choosing CTA keeps in shared memory
+constexpr int kCacheKeys = 47104; // keys that a choosing CTA keeps in shared memory
+constexpr int kMostRanks = 8;     // choosing CTAs of a head at most
+constexpr int kRankKeys = 6144;   // slots that are worth a CTA of their own
 
 struct EvictKernelParams {
   CacheView c;
@@ -61,92 +63,165 @@ __device__ __forceinline__ int sum_below(const int* s, int warp) {
   return __reduce_add_sync(0xffffffffu, lane < warp ? s[lane] : 0);
 }
 
-// One CTA per (sequence, head).  The k-th largest key between the sinks and the newest tokens is found digit by digit
-// (11, 11, 10 bits; a histogram of the candidates' digits each time), then two ordered sweeps write what is above it and
-// the first ones of those equal to it.  The weights are read once, into shared memory, unless there are more than fit
-// (then the later sweeps read them from L2).  Bound by latency: 64 CTAs of 16384 weights 20 us with a slot a lane at
-// a time and the kept weights read again, 17 with four.
-__global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_constant__ EvictKernelParams p, int n_cached) {
+// All threads of a cluster, with what they wrote to shared memory.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// the same place in another CTA's shared memory
+__device__ __forceinline__ uint32_t cluster_addr(const void* at, int rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(tc05::smem_u32(at)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ int ld_cluster(const int* at, int rank) {
+  int x;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(x) : "r"(cluster_addr(at, rank)) : "memory");
+  return x;
+}
+__device__ __forceinline__ int2 ld_cluster(const int2* at, int rank) {
+  int2 x;
+  asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(x.x), "=r"(x.y) : "r"(cluster_addr(at, rank)) : "memory");
+  return x;
+}
+__device__ __forceinline__ int2 operator+(int2 a, int2 b) { return make_int2(a.x + b.x, a.y + b.y); }
+// *at, or the sum of it over a cluster's CTAs
+template <bool kMany, typename T>
+__device__ __forceinline__ T sum_ranks(const T* at, int ranks) {
+  if (!kMany) return *at;
+  T x = {};
+#pragma unroll
+  for (int r = 0; r < kMostRanks; ++r)
+    if (r < ranks) x = x + ld_cluster(at, r);
+  return x;
+}
+
+// One CTA per (sequence, head), or a cluster of `ranks` (kMany), each with a contiguous piece of the slots.  The k-th
+// largest key between the sinks and the newest tokens is found digit by digit (11, 11, 10 bits; a histogram of the
+// candidates' digits each time, added up over the cluster), then two ordered sweeps write what is above it and the first
+// ones of those equal to it.  The weights are read once, into shared memory, unless there are more than fit (then the
+// later sweeps read them from L2).  The number of cluster barriers depends on nothing that is read.
+// Bound by the SM's issue rate, 0.6 us for 1000 slots of a CTA, and 8 us of latencies (13 in a cluster: four exchanges).
+// Whole evictions, by single CTAs and by the clusters chosen below: 8 heads of 131072 slots (8192 stay) 143 and 32 us,
+// of 40000 38 and 24, of 8192 16.5 (two CTAs: 18); 64 heads of 16384 (half stay) 87 and 82.
+template <bool kMany>
+__global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_constant__ EvictKernelParams p, int n_cached, int ranks_) {
   extern __shared__ __align__(16) uint32_t s_keys[];  // [n_cached]
-  __shared__ int s_hist[2][kBins];      // (two: neighbouring lanes count apart where the weights are much alike)
+  // Histograms, two of each digit: neighbouring lanes count apart where the weights are much alike.  Their sums over 64 bins
+  // each, a warp's, largest digits first.
+  __shared__ __align__(16) int s_hist[2 * (2048 + 2048 + 1024)];
+  __shared__ int s_part[kDigits][kSelect / 32];
+  __shared__ int2 s_found[kDigits];
   __shared__ int s_warp[kSelect / 32], s_warp_eq[kSelect / 32];
-  __shared__ int s_digit, s_left;
+  __shared__ int2 s_stay;
   griddep_launch();
+  for (int i = threadIdx.x; i < 2 * (2048 + 2048 + 1024) / 4; i += kSelect) reinterpret_cast<uint4*>(s_hist)[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
   griddep_wait();
-  const int b = blockIdx.x / p.c.hkv, h = blockIdx.x - b * p.c.hkv;
+  const int ranks = kMany ? ranks_ : 1;
+  const int item = blockIdx.x / ranks, rank = blockIdx.x - item * ranks;
+  const int b = item / p.c.hkv, h = item - b * p.c.hkv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int len = checked_len(p, b);
   const int keep = min(len, p.budget);
   const float* const w = p.weights + b * p.w_sb + h * p.w_sh;
-  int* const kept = p.kept + static_cast<long long>(blockIdx.x) * p.budget;
-  float* const new_w = p.new_weights + static_cast<long long>(blockIdx.x) * p.new_w_len;
-  if (h == 0 && threadIdx.x == 0) p.new_lens[b] = keep;
-  const bool cached = len <= n_cached;
-  if (cached && len > p.budget) {
-#pragma unroll 16
-    for (int i = threadIdx.x; i < len; i += kSelect) s_keys[i] = order_key(w[i]);
+  int* const kept = p.kept + static_cast<long long>(item) * p.budget;
+  float* const new_w = p.new_weights + static_cast<long long>(item) * p.new_w_len;
+  if (h == 0 && rank == 0 && threadIdx.x == 0) p.new_lens[b] = keep;
+  // this CTA's slots: [from, to)
+  constexpr int kStep = 128;  // slots of a warp at a time, four a lane
+  const int per = ((len + ranks - 1) / ranks + kStep - 1) / kStep * kStep;
+  const int from = min(static_cast<long long>(len), static_cast<long long>(rank) * per), to = min(static_cast<long long>(len), static_cast<long long>(from) + per);
+  const bool cached = per <= n_cached;
+  // candidates: slots [lo, hi), of which `left` stay
+  const bool all = len <= p.budget;
+  const int lo = all ? 0 : p.n_sink, hi = all ? len : len - p.n_recent;  // (n_sink + n_recent <= budget < len)
+  int left = all ? len : p.budget - p.n_sink - p.n_recent;
+  const bool choose = !all && left > 0;
+  // keys above it stay, and `left` of those equal to it (nothing in between: a NaN would be equal to it, left is 0)
+  uint32_t bound = choose || all ? 0 : 0xffffffffu;
+  if (!all) {
+    constexpr int kAhead = 8;
+    for (int i0 = from + threadIdx.x; i0 < to; i0 += kAhead * kSelect) {
+      float x[kAhead];
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) x[e] = i0 + e * kSelect < to ? w[i0 + e * kSelect] : 0.f;
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) {
+        const int i = i0 + e * kSelect;
+        const uint32_t key = order_key(x[e]);
+        if (cached && i < to) s_keys[i - from] = key;
+        if (choose && i >= lo && i < min(hi, to)) atomicAdd(&s_hist[(lane & 1) * 2048 + (key >> 21)], 1);
+      }
+    }
   }
   __syncthreads();
-  // the keys of four slots from a multiple of four on (behind the last one: anything)
+  // the keys of four slots, from a multiple of four behind the first on (behind the last one: anything)
   const auto keys4 = [&](int i) {
-    if (cached) return *reinterpret_cast<const uint4*>(s_keys + i);
+    if (cached) return *reinterpret_cast<const uint4*>(s_keys + (i - from));
     return make_uint4(order_key(w[i]), i + 1 < len ? order_key(w[i + 1]) : 0, i + 2 < len ? order_key(w[i + 2]) : 0, i + 3 < len ? order_key(w[i + 3]) : 0);
   };
-  // candidates: slots [lo, hi), of which `left` stay
-  int lo = 0, hi = len, left = len;
-  uint32_t bound = 0;  // keys above it stay, and `left` of those equal to it
-  if (len > p.budget) {
-    lo = p.n_sink, hi = len - p.n_recent;  // (n_sink + n_recent <= budget < len)
-    left = p.budget - p.n_sink - p.n_recent;
-    uint32_t mask = 0;
-    if (left > 0) {
+  uint32_t mask = 0;
 #pragma unroll
-      for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass < 2 ? 2048 : 1024;
-        for (int i = threadIdx.x; i < 2 * kBins; i += kSelect) s_hist[0][i] = 0;
-        __syncthreads();
+  for (int pass = 0; pass < kDigits; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass < 2 ? 2048 : 1024;
+    int* const hist = s_hist + pass * 2 * 2048;
+    if (choose) {
+      if (pass > 0) {
 #pragma unroll 2
-        for (int i = 4 * threadIdx.x; i < hi; i += 4 * kSelect) {
+        for (int i = from + 4 * threadIdx.x; i < min(hi, to); i += 4 * kSelect) {
           const uint4 k4 = keys4(i);
           const uint32_t keys[4] = {k4.x, k4.y, k4.z, k4.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (i + e >= lo && i + e < hi && (keys[e] & mask) == bound) atomicAdd(&s_hist[lane & 1][(keys[e] >> shift) & (bins - 1)], 1);
+            if (i + e >= lo && i + e < min(hi, to) && (keys[e] & mask) == bound) atomicAdd(hist + (lane & 1) * bins + ((keys[e] >> shift) & (bins - 1)), 1);
         }
-        __syncthreads();
-        // the digit with which the count from above reaches `left`: every thread two bins, largest first
-        const int at = bins - 1 - 2 * threadIdx.x;
-        const int c0 = at >= 1 ? s_hist[0][at] + s_hist[1][at] : 0, c1 = at >= 1 ? s_hist[0][at - 1] + s_hist[1][at - 1] : 0;
-        int sum = c0 + c1;
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-          const int o = __shfl_up_sync(0xffffffffu, sum, d);
-          if (lane >= d) sum += o;
-        }
-        if (lane == 31) s_warp[warp] = sum;
-        __syncthreads();
-        const int before = sum_below(s_warp, warp);
-        const int above = before + sum - c0 - c1;  // keys of larger digits
-        if (at >= 1 && above < left && above + c0 + c1 >= left) {
-          const bool first = above + c0 >= left;
-          s_digit = first ? at : at - 1;
-          s_left = left - above - (first ? 0 : c0);
-        }
-        __syncthreads();
-        left = s_left;
-        bound |= static_cast<uint32_t>(s_digit) << shift;
-        mask |= static_cast<uint32_t>(bins - 1) << shift;
         __syncthreads();
       }
-    } else {
-      bound = 0xffffffffu;  // nothing in between (a NaN would be equal to it: left is 0)
+      const int at = bins - 2 - 2 * threadIdx.x;
+      int2 c = make_int2(0, 0);
+      if (at >= 0) {
+        int2* const h2 = reinterpret_cast<int2*>(hist + at);
+        c = *h2 + h2[bins / 2];
+        *h2 = c;
+      }
+      const int sum = __reduce_add_sync(0xffffffffu, c.x + c.y);
+      if (lane == 0) s_part[pass][warp] = sum;
+      if (!kMany) __syncthreads();
+    }
+    if (kMany) cluster_sync();
+    if (choose) {
+      // the digit with which the count from above reaches `left`: which 64 bins, then which of them
+      if (warp == 0) {
+        const auto scan = [&](int x) {
+#pragma unroll
+          for (int d = 1; d < 32; d *= 2) {
+            const int o = __shfl_up_sync(0xffffffffu, x, d);
+            if (lane >= d) x += o;
+          }
+          return x;
+        };
+        const int part = sum_ranks<kMany>(&s_part[pass][lane], ranks);
+        int above = scan(part) - part;
+        int src = __ffs(__ballot_sync(0xffffffffu, above < left && above + part >= left)) - 1;
+        above = __shfl_sync(0xffffffffu, above, src);
+        const int at = max(0, bins - 2 - 2 * (32 * src + lane));
+        const int2 c = sum_ranks<kMany>(reinterpret_cast<const int2*>(hist + at), ranks);
+        above += scan(c.x + c.y) - c.x - c.y;
+        src = __ffs(__ballot_sync(0xffffffffu, above < left && above + c.x + c.y >= left)) - 1;
+        const bool first = above + c.y >= left;
+        const int digit = __shfl_sync(0xffffffffu, first ? at + 1 : at, src);
+        above = __shfl_sync(0xffffffffu, above + (first ? 0 : c.y), src);
+        if (lane == 0) s_found[pass] = make_int2(digit, left - above);
+      }
+      __syncthreads();
+      bound |= static_cast<uint32_t>(s_found[pass].x) << shift;
+      left = s_found[pass].y;
+      mask |= static_cast<uint32_t>(bins - 1) << shift;
     }
   }
-  // Every warp takes a contiguous piece of all slots: how many of its tokens stay, then where they go.
-  const bool all = len <= p.budget;
-  constexpr int kStep = 128;  // slots of a warp at a time, four a lane
-  const int piece = (len + kSelect / 32 * kStep - 1) / (kSelect / 32 * kStep) * kStep;
-  const int begin = min(len, warp * piece), end = min(len, begin + piece);
+  // Every warp takes a contiguous piece of the CTA's slots: how many of its tokens stay, then where they go.
+  const int piece = (to - from + kSelect / 32 * kStep - 1) / (kSelect / 32 * kStep) * kStep;
+  const int begin = min(to, from + warp * piece), end = min(to, begin + piece);
   // whether the slots i .. i + 3 stay for certain (bits 0 to 3), or if there is room for them (bits 8 to 11)
   const auto stand = [&](int i, uint32_t (&keys)[4]) {
     uint32_t r = 0;
@@ -177,8 +252,15 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
   if (lane == 0) s_warp[warp] = n_above, s_warp_eq[warp] = n_equal;
   __syncthreads();
   // (of the equal ones, those in front take the room first)
-  int equal_before = sum_below(s_warp_eq, warp);
-  int at = sum_below(s_warp, warp) + min(equal_before, left);
+  int equal_before = sum_below(s_warp_eq, warp), above_before = sum_below(s_warp, warp);
+  if (kMany) {
+    if (threadIdx.x == kSelect - 1) s_stay = make_int2(above_before + n_above, equal_before + n_equal);
+    cluster_sync();
+    const int2 o = lane < rank ? ld_cluster(&s_stay, lane) : make_int2(0, 0);
+    above_before += __reduce_add_sync(0xffffffffu, o.x);
+    equal_before += __reduce_add_sync(0xffffffffu, o.y);
+  }
+  int at = above_before + min(equal_before, left);
   const uint32_t before = (1u << lane) - 1;
   for (int i = begin + 4 * lane; i - 4 * lane < end; i += kStep) {
     uint32_t keys[4] = {0, 0, 0, 0};
@@ -197,24 +279,25 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
       for (int e = 0; e < 4; ++e)
         if (r >> (8 + e) & 1u) r |= (n++ < left ? 1u : 0u) << e;
     }
-    int to = at;
+    int n = at;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t v = __ballot_sync(0xffffffffu, r >> e & 1u);
-      to += __popc(v & before);
+      n += __popc(v & before);
       at += __popc(v);
     }
     equal_before += equal_all;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (r >> e & 1u) {
-        kept[to] = i + e;
-        if (to < p.new_w_len) new_w[to] = cached && !all ? key_weight(keys[e]) : w[i + e];
-        ++to;
+        if (n < p.budget) kept[n] = i + e;  // (always, unless somebody changes the weights meanwhile)
+        if (n < p.new_w_len) new_w[n] = cached && !all ? key_weight(keys[e]) : w[i + e];
+        ++n;
       }
   }
-  for (int i = keep + threadIdx.x; i < p.budget; i += kSelect) kept[i] = -1;
-  for (int i = keep + threadIdx.x; i < p.new_w_len; i += kSelect) new_w[i] = 0.f;
+  for (long long i = keep + rank * kSelect + threadIdx.x; i < p.budget; i += ranks * kSelect) kept[i] = -1;
+  for (long long i = keep + rank * kSelect + threadIdx.x; i < p.new_w_len; i += ranks * kSelect) new_w[i] = 0.f;
+  if (kMany) cluster_sync();  // (nobody's shared memory goes while somebody may read it)
 }
 
 // A CTA packs `run` new blocks of a head, K and V (or one block, K or V, where there are too few for that): it looks all
@@ -312,12 +395,13 @@ __global__ void __launch_bounds__(kPack) evict_pack_kernel(const __grid_constant
 
 // The choosing kernel may use as much shared memory as it needs at most: set once per device.
 cudaError_t allow_shared(int bytes) {
-  if (bytes <= 24 * 1024) return cudaSuccess;  // (48 KB with what it has of fixed size need no permission)
+  if (bytes <= 6 * 1024) return cudaSuccess;  // (48 KB with what it has of fixed size need no permission)
   static std::atomic<uint64_t> set{0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess || (dev < 64 && (set.load(std::memory_order_relaxed) >> dev & 1))) return e;
-  e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kCacheKeys * 4);
+  e = cudaFuncSetAttribute(evict_select_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCacheKeys * 4);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(evict_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCacheKeys * 4);
   if (e == cudaSuccess && dev < 64) set.fetch_or(1ull << dev, std::memory_order_relaxed);
   return e;
 }
@@ -360,7 +444,7 @@ extern "C" int rswa_cache_evict(const rswa_cache_evict_params_t* p, void* stream
   }
   const int64_t items = static_cast<int64_t>(p->table.batch) * p->cache.n_kv_heads;
   const int64_t units = static_cast<int64_t>(p->table.batch) * p->new_table.max_blocks;
-  if (items > 0x7fffffffLL || units > 0x7fffffffLL) {
+  if (items * kMostRanks > 0x7fffffffLL || units > 0x7fffffffLL) {
     set_error("%s: too many sequences in one call", what);
     return RSWA_E_UNSUPPORTED;
   }
@@ -379,10 +463,13 @@ extern "C" int rswa_cache_evict(const rswa_cache_evict_params_t* p, void* stream
   kp.status = p->status;
   kp.mirror = status_mirror(p->status);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int64_t keys = cap < kCacheKeys ? cap : kCacheKeys;
+  // (several CTAs a head where there are SMs for them and enough slots, or where the keys do not fit one's shared memory)
+  int ranks = 1;
+  while (ranks < kMostRanks && ((items * 2 * ranks <= sm_count() && cap >= 2LL * ranks * kRankKeys) || cap > static_cast<int64_t>(ranks) * kCacheKeys)) ranks *= 2;
+  const int64_t per = ((cap + ranks - 1) / ranks + 127) / 128 * 128, keys = per < kCacheKeys ? per : kCacheKeys;
   const int smem = static_cast<int>(keys) * 4;
   cudaError_t e = allow_shared(smem);
-  if (e == cudaSuccess) e = launch_kernel(evict_select_kernel, dim3(static_cast<unsigned>(items)), kSelect, smem, s, true, kp, static_cast<int>(keys));
+  if (e == cudaSuccess) e = launch_clusters(ranks > 1 ? evict_select_kernel<true> : evict_select_kernel<false>, dim3(static_cast<unsigned>(items * ranks)), ranks, kSelect, smem, s, true, kp, static_cast<int>(keys), ranks);
   if (e == cudaSuccess) count_launches(1);
   if (e == cudaSuccess && units > 0) {
     // (four blocks, K and V, a CTA where that still gives every SM four CTAs)

@@ -428,6 +428,9 @@ EVICT = [
     ([5000, 33], 1, 64, 16, 1, 0, 0),
     ([70000], 1, 64, 128, 20000, 4, 1000),
     ([16000, 9100], 2, 64, 16, 9000, 100, 8900),      # sinks and newest alone, of many
+    ([50000, 3, 6000], 2, 64, 64, 5000, 3, 1),        # several CTAs a head, some of them without a slot
+    ([30000, 29999], 8, 64, 128, 25000, 0, 0),
+    ([400000], 1, 64, 128, 1500, 4, 100),             # more than their shared memory holds
 ]
 
 
