@@ -304,12 +304,15 @@ __global__ void __launch_bounds__(kSelect) evict_select_kernel(const __grid_cons
 // their rows up first, then reads the rows of one block while it finds the largest magnitude of the one before and writes
 // it at its new scale.  A row is read once (head_dim bytes, scattered) and stays in registers.
 // Bound by HBM, one byte in and one out per element; what a CTA waits for before its first byte (length, kept slots,
-// block table, scales: four loads in a row) is paid once a run: 134 MB in, 134 MB out take 57 us, 41 at a copy's rate.
-constexpr int kRun = 4;
+// block table, scales: four loads in a row) is paid once a run.  134 MB in and 134 MB out in blocks of 64 take 51 us with
+// runs of two, 57 with four (too few CTAs for even waves), 41 at a copy's rate; in blocks of 16 four are 5 % faster.
+template <int kBs>
+constexpr int kRunOf = kBs >= 64 ? 2 : 4;
 template <int kD, int kBs, bool kInt8>
 __global__ void __launch_bounds__(kPack) evict_pack_kernel(const __grid_constant__ EvictKernelParams p, int run) {
   constexpr int kCols = kD / 16;  // 16-byte pieces of a row
   constexpr int kPasses = (kBs * kCols + kPack - 1) / kPack;
+  constexpr int kRun = kRunOf<kBs>;
   __shared__ int s_page[kRun * kBs], s_slot[kRun * kBs];  // block and head of a row (-1: none), token in the block
   __shared__ float s_scale[2][kRun * kBs];
   __shared__ float s_max[2][kPack / 32];
@@ -472,8 +475,9 @@ extern "C" int rswa_cache_evict(const rswa_cache_evict_params_t* p, void* stream
   if (e == cudaSuccess) e = launch_clusters(ranks > 1 ? evict_select_kernel<true> : evict_select_kernel<false>, dim3(static_cast<unsigned>(items * ranks)), ranks, kSelect, smem, s, true, kp, static_cast<int>(keys), ranks);
   if (e == cudaSuccess) count_launches(1);
   if (e == cudaSuccess && units > 0) {
-    // (four blocks, K and V, a CTA where that still gives every SM four CTAs)
-    const int run = units * p->cache.n_kv_heads >= 16LL * sm_count() ? kRun : 1;
+    // (several blocks, K and V, a CTA where that still gives every SM four CTAs)
+    const int most = bs >= 64 ? kRunOf<64> : kRunOf<16>;
+    const int run = units * p->cache.n_kv_heads >= 4LL * most * sm_count() ? most : 1;
     const dim3 grid(static_cast<unsigned>(p->table.batch * ((p->new_table.max_blocks + run - 1LL) / run)), static_cast<unsigned>((run > 1 ? 1 : 2) * p->cache.n_kv_heads));
     const int key = p->cache.head_dim * 1000 + p->cache.block_size;
     switch (key) {
