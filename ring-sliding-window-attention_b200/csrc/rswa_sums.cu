@@ -11,13 +11,16 @@
 // columns and half the warps a step took 3270 cycles).
 // 2 * head_dim FLOPs and one exponential per (query head, pair): at 128 elements the exponentials (16 per clock and SM,
 // 2048 cycles a step) outweigh the products (1024).  One pair in eight is computed on the FMA pipe (fma_exp2): none
-// 713 us, 1/8 701, 1/4 720, 3/8 788 (16384 tokens, 32/8 heads, window 4096): the card is at its power cap there
-// (1.5 GHz), and an exponential on the FMA pipe costs more than it saves beyond that.  A step takes about 2400 cycles.
+// 624 us, 1/8 621, 1/4 631 (16384 tokens, 32/8 heads, window 4096): the card is at its power cap there when call follows
+// call (548 us on a cool one), and an exponential on the FMA pipe costs more than it saves beyond that.
 //
-// Work: the steps of all (batch row, key/value head, 256 keys) in one order, cut into equal shares, one per CTA, whatever
-// the mask makes of an item's length (a sink token is seen by its whole sequence): nothing is longer than the rest.  An
-// item that is cut leaves partial sums in the workspace, added up in order by a second kernel: deterministic.
+// Work: the steps of all (batch row, key/value head, 256 keys) in one order, cut into equal shares, one per CTA and round,
+// whatever the mask makes of an item's length (a sink token is seen by its whole sequence): nothing is longer than the rest.
+// Rounds, because a query tile is read by as many CTAs as the window has key tiles: with 134 MB of queries in one round
+// they do not meet in L2 (1.3 GB from HBM, whose power the card lacks elsewhere: 680 us; two rounds 621, five 623, ten 641).
+// An item that is cut leaves partial sums in the workspace, added up in order by a second kernel: deterministic.
 // A thread's running sum is compensated: a key may be seen by 10^5 queries and more.
+#include <algorithm>
 #include <atomic>
 
 #include "rswa_common.cuh"
@@ -34,7 +37,9 @@ constexpr int kThreads = 128 + kSumWarps * 32;  // warp 0 TMA, warp 1 MMA, warp 
 constexpr int kScan = 256;         // threads of the prefix sums
 constexpr int kQStages = 3;
 constexpr int kTmemCols = 512;
+constexpr long long kRoundBytes = 68ll << 20;  // of queries at most
 constexpr int kMinShare = 2;       // steps of a CTA at least
+constexpr int kMaxRounds = 8, kRoundSteps = 32;  // shares of a CTA at most, and steps of each at least
 
 struct SumsKernelParams {
   CUtensorMap q_map, k_map;
@@ -46,9 +51,9 @@ struct SumsKernelParams {
   const int* cu;
   int n_seqs;
   float* out;    // [batch, hkv, len]
-  float* part;   // [CTAs][2][kKeys]
+  float* part;   // [shares][2][kKeys]
   int n_items;   // per batch row and head
-  int ctas;
+  int ctas, rounds;
   int* status;
   int* mirror;
 };
@@ -94,7 +99,11 @@ __device__ __forceinline__ void item_prefix(const SumsKernelParams& p, long long
   __syncthreads();
 }
 
-__device__ __forceinline__ long long n_shares(long long total, int ctas) { return min(static_cast<long long>(ctas), max(1LL, total / kMinShare)); }
+// Shares of the work: `rounds` for each CTA, the ones of a round side by side, unless there is too little.
+__device__ __forceinline__ long long n_shares(long long total, const SumsKernelParams& p) {
+  const long long rounds = p.rounds == 1 ? 1 : max(1LL, min(static_cast<long long>(p.rounds), total / (static_cast<long long>(p.ctas) * kRoundSteps)));
+  return min(rounds * p.ctas, max(1LL, total / kMinShare));
+}
 __device__ __forceinline__ long long share_begin(long long total, long long shares, long long c) { return total * c / shares; }
 
 // An item, and how far into it a place is: steps are query heads of the group, then query tiles.
@@ -126,6 +135,26 @@ __device__ __forceinline__ Item item_at(const SumsKernelParams& p, const long lo
   while (step >= it.first + it.n) it.next(p);
   return it;
 }
+
+// A share: where it begins (`start` steps into an item), and its steps.
+struct Share {
+  int n, bh, kt, n_qt, start;
+};
+// The same, walked item by item by every role: steps [start, stop) of the item are this share's.
+struct Walk {
+  int left, bh, kt, n_qt, start, stop;
+  __device__ __forceinline__ Walk(const SumsKernelParams& p, const Share& s) : left(s.n), bh(s.bh), kt(s.kt), n_qt(s.n_qt), start(s.start) { cut(p); }
+  __device__ __forceinline__ int n(const SumsKernelParams& p) const { return n_qt * p.group; }
+  __device__ __forceinline__ void cut(const SumsKernelParams& p) { stop = start + min(left, n(p) - start); }
+  __device__ __forceinline__ void next(const SumsKernelParams& p) {
+    left -= stop - start;
+    start = 0;
+    if (left == 0) return;
+    if (++kt == p.n_items) kt = 0, ++bh;
+    n_qt = item_q_tiles(p, kt);
+    cut(p);
+  }
+};
 
 // 2^x for two values on the FMA pipe: x = n + f with n = round(x) and f in [-0.5, 0.5]; 2^f by the polynomial of degree 5 with
 // the least relative error there (7.5e-8, found by exchange of its extrema; 2.1e-7 in 32 bits), times 2^n from n's bits.  Below
@@ -159,12 +188,13 @@ struct Ctl {
   uint64_t k_full[2], k_free[2], q_full[kQStages], q_free[kQStages], s_ready[2][2], s_free[2][2], drained;  // (of the steps' parity, and of the two tiles)
   uint32_t tmem_base;
   int err;
+  Share share[kMaxRounds];  // of the CTA
 };
 
 constexpr int kSmemK = 0, kSmemQ = 4 * kTileBytes, kSmemLse = kSmemQ + kQStages * kTileBytes;
 constexpr int kSmemHalf = kSmemLse + 2 * kTile * 4, kSmemCtl = kSmemHalf + kKeys * 4;
-constexpr int kSmemBytes = kSmemCtl + 256;
-static_assert(sizeof(Ctl) <= 256 && kSmemBytes <= 232448, "shared memory budget");
+constexpr int kSmemBytes = kSmemCtl + 512;
+static_assert(sizeof(Ctl) <= 512 && kSmemBytes <= 232448, "shared memory budget");
 
 template <int kD, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1) weight_sums_kernel(const __grid_constant__ SumsKernelParams p) {
@@ -203,12 +233,12 @@ __global__ void __launch_bounds__(kThreads, 1) weight_sums_kernel(const __grid_c
   if (threadIdx.x == 0) ctl->err = (smem_u32(smem) & 1023u) ? 199 : status_code(p.status, p.mirror);
   item_prefix(p, s_prefix, s_prefix + kScan + 1);
   const long long total = s_prefix[kScan] * p.group * p.hkv * p.batch;
-  const long long shares = n_shares(total, p.ctas);
-  long long begin = 0, end = 0;
-  Item it = {};
-  if (blockIdx.x < shares && ctl->err == 0) {
-    begin = share_begin(total, shares, blockIdx.x), end = share_begin(total, shares, blockIdx.x + 1);
-    it = item_at(p, s_prefix, begin);
+  const long long shares = n_shares(total, p);
+  const int rounds = ctl->err != 0 || blockIdx.x >= shares ? 0 : (static_cast<int>(shares) - 1 - static_cast<int>(blockIdx.x)) / p.ctas + 1;
+  if (threadIdx.x < rounds) {
+    const long long share = blockIdx.x + static_cast<long long>(threadIdx.x) * p.ctas, begin = share_begin(total, shares, share);
+    const Item it = item_at(p, s_prefix, begin);
+    ctl->share[threadIdx.x] = {static_cast<int>(share_begin(total, shares, share + 1) - begin), it.bh, it.kt, it.n_qt, static_cast<int>(begin - it.first)};
   }
   tc_fence_before();
   fence_proxy_async_smem();  // (the prefix sums have been read: loads may land there)
@@ -218,105 +248,106 @@ __global__ void __launch_bounds__(kThreads, 1) weight_sums_kernel(const __grid_c
   volatile int* err = &ctl->err;
   constexpr uint32_t kTile16 = kTileBytes >> 4;
 
-  if (warp == 0 && lane == 0) {
-    // ---------------------------------------------------------------- loads
-    bool ok = true;
-    int g = 0, ni = 0;  // steps and items so far
-    for (long long at = begin; at < end && ok; it.next(p), ++ni) {
-      const int b = it.bh / p.hkv, h = it.bh - b * p.hkv, kb = ni & 1;
-      if (ni >= 2) ok = mbar_wait<200>(&ctl->k_free[kb], ((ni >> 1) - 1) & 1, err, kErrWaitProducer);
-      if (!ok) break;
-      const int t0 = it.kt * kKeys;
-      const int tiles = t0 + kTile < p.len ? 2 : 1;  // (a tile wholly behind the end: its rows are not looked at)
-      mbar_expect_tx(&ctl->k_full[kb], tiles * kLoadBytes);
-      for (int t = 0; t < tiles; ++t) {
-        uint8_t* const dst = sK + (kb * 2 + t) * kTileBytes;
-        tma_load_4d(dst, &p.k_map, &ctl->k_full[kb], 0, h, t0 + t * kTile, b);
-        if (kD > 64) tma_load_4d(dst + kBoxBytes, &p.k_map, &ctl->k_full[kb], 64, h, t0 + t * kTile, b);
-      }
-      const int stop = static_cast<int>(min(end, it.first + it.n) - it.first);
-      for (int i = static_cast<int>(at - it.first); i < stop; ++i, ++g) {
-        const int st = g % kQStages, hd = h * p.group + i / it.n_qt, q0 = t0 + i % it.n_qt * kTile;
-        if (g >= kQStages) ok = mbar_wait<200>(&ctl->q_free[st], (g / kQStages - 1) & 1, err, kErrWaitProducer);
+  if (warp < 4) {
+    setmaxnreg_dec<64>();
+    if (warp == 0 && lane == 0) {
+      // ---------------------------------------------------------------- loads
+      bool ok = true;
+      int g = 0, ni = 0;  // steps and items so far
+      for (int r = 0; r < rounds && ok; ++r)
+      for (Walk it(p, ctl->share[r]); it.left > 0 && ok; it.next(p), ++ni) {
+        const int b = it.bh / p.hkv, h = it.bh - b * p.hkv, kb = ni & 1;
+        if (ni >= 2) ok = mbar_wait<200>(&ctl->k_free[kb], ((ni >> 1) - 1) & 1, err, kErrWaitProducer);
         if (!ok) break;
-        uint8_t* const dst = sQ + st * kTileBytes;
-        mbar_expect_tx(&ctl->q_full[st], kLoadBytes);
-        tma_load_4d(dst, &p.q_map, &ctl->q_full[st], 0, hd, q0, b);
-        if (kD > 64) tma_load_4d(dst + kBoxBytes, &p.q_map, &ctl->q_full[st], 64, hd, q0, b);
-      }
-      at = it.first + stop;
-    }
-    if (!ok) {
-      // loads still on their way must not outlive the CTA's shared memory (each wait is limited)
-      int own = 0;
-      for (int i = max(0, g - kQStages); i < g; ++i) mbar_wait(&ctl->q_full[i % kQStages], (i / kQStages) & 1, &own, kErrWaitProducer);
-      for (int i = max(0, ni - 1); i <= ni; ++i)
-        if (i < ni || g > 0) mbar_wait(&ctl->k_full[i & 1], (i >> 1) & 1, &own, kErrWaitProducer);
-    }
-  } else if (warp == 1 && elect_one()) {
-    // ---------------------------------------------------------------- products
-    constexpr uint32_t id = idesc_f16(128, 128, kBf16 ? 1 : 0, 0, 0);
-    const uint64_t dK = smem_desc_sw128(smem_u32(sK), 16, 1024), dQ = smem_desc_sw128(smem_u32(sQ), 16, 1024);
-    bool ok = true;
-    int g = 0, ni = 0;
-    for (long long at = begin; at < end && ok; it.next(p), ++ni) {
-      const int kb = ni & 1;
-      ok = mbar_wait(&ctl->k_full[kb], (ni >> 1) & 1, err, kErrWaitMma);
-      const int stop = static_cast<int>(min(end, it.first + it.n) - it.first);
-      for (int i = static_cast<int>(at - it.first); i < stop && ok; ++i, ++g) {
-        const int st = g % kQStages, sb = g & 1;
-        ok = mbar_wait(&ctl->q_full[st], (g / kQStages) & 1, err, kErrWaitMma);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (ok && g >= 2) ok = mbar_wait(&ctl->s_free[sb][t], ((g >> 1) - 1) & 1, err, kErrWaitMma);
+        const int t0 = it.kt * kKeys;
+        const int tiles = t0 + kTile < p.len ? 2 : 1;  // (a tile wholly behind the end: its rows are not looked at)
+        mbar_expect_tx(&ctl->k_full[kb], tiles * kLoadBytes);
+        for (int t = 0; t < tiles; ++t) {
+          uint8_t* const dst = sK + (kb * 2 + t) * kTileBytes;
+          tma_load_4d(dst, &p.k_map, &ctl->k_full[kb], 0, h, t0 + t * kTile, b);
+          if (kD > 64) tma_load_4d(dst + kBoxBytes, &p.k_map, &ctl->k_full[kb], 64, h, t0 + t * kTile, b);
+        }
+        for (int i = it.start; i < it.stop; ++i, ++g) {
+          const int st = g % kQStages, hd = h * p.group + i / it.n_qt, q0 = t0 + i % it.n_qt * kTile;
+          if (g >= kQStages) ok = mbar_wait<200>(&ctl->q_free[st], (g / kQStages - 1) & 1, err, kErrWaitProducer);
           if (!ok) break;
-          tc_fence_after();
+          uint8_t* const dst = sQ + st * kTileBytes;
+          mbar_expect_tx(&ctl->q_full[st], kLoadBytes);
+          tma_load_4d(dst, &p.q_map, &ctl->q_full[st], 0, hd, q0, b);
+          if (kD > 64) tma_load_4d(dst + kBoxBytes, &p.q_map, &ctl->q_full[st], 64, hd, q0, b);
+        }
+      }
+      if (!ok) {
+        // loads still on their way must not outlive the CTA's shared memory (each wait is limited)
+        int own = 0;
+        for (int i = max(0, g - kQStages); i < g; ++i) mbar_wait(&ctl->q_full[i % kQStages], (i / kQStages) & 1, &own, kErrWaitProducer);
+        for (int i = max(0, ni - 1); i <= ni; ++i)
+          if (i < ni || g > 0) mbar_wait(&ctl->k_full[i & 1], (i >> 1) & 1, &own, kErrWaitProducer);
+      }
+    } else if (warp == 1 && elect_one()) {
+      // ---------------------------------------------------------------- products
+      constexpr uint32_t id = idesc_f16(128, 128, kBf16 ? 1 : 0, 0, 0);
+      const uint64_t dK = smem_desc_sw128(smem_u32(sK), 16, 1024), dQ = smem_desc_sw128(smem_u32(sQ), 16, 1024);
+      bool ok = true;
+      int g = 0, ni = 0;
+      for (int r = 0; r < rounds && ok; ++r)
+      for (Walk it(p, ctl->share[r]); it.left > 0 && ok; it.next(p), ++ni) {
+        const int kb = ni & 1;
+        ok = mbar_wait(&ctl->k_full[kb], (ni >> 1) & 1, err, kErrWaitMma);
+        for (int i = it.start; i < it.stop && ok; ++i, ++g) {
+          const int st = g % kQStages, sb = g & 1;
+          ok = mbar_wait(&ctl->q_full[st], (g / kQStages) & 1, err, kErrWaitMma);
 #pragma unroll
-          for (int k = 0; k < kD / 16; ++k) {
-            const uint32_t off = ((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4;
-            mma_ss(tmem + sb * 256 + t * 128, dK + (kb * 2 + t) * kTile16 + off, dQ + st * kTile16 + off, id, k > 0 ? 1u : 0u);
+          for (int t = 0; t < 2; ++t) {
+            if (ok && g >= 2) ok = mbar_wait(&ctl->s_free[sb][t], ((g >> 1) - 1) & 1, err, kErrWaitMma);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < kD / 16; ++k) {
+              const uint32_t off = ((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4;
+              mma_ss(tmem + sb * 256 + t * 128, dK + (kb * 2 + t) * kTile16 + off, dQ + st * kTile16 + off, id, k > 0 ? 1u : 0u);
+            }
+            mma_commit(&ctl->s_ready[sb][t]);
           }
-          mma_commit(&ctl->s_ready[sb][t]);
+          if (!ok) break;
+          mma_commit(&ctl->q_free[st]);
         }
-        if (!ok) break;
-        mma_commit(&ctl->q_free[st]);
+        mma_commit(&ctl->k_free[kb]);
       }
-      mma_commit(&ctl->k_free[kb]);
-      at = it.first + stop;
-    }
-    if (!ok) {
-      // products under way must not outlive the CTA's tensor memory (a limited wait)
-      int own = 0;
-      mma_commit(&ctl->drained);
-      mbar_wait(&ctl->drained, 0, &own, kErrWaitMma);
-    }
-  } else if (warp == 2) {
-    // ---------------------------------------------------------------- rows of -lse * log2(e)
-    bool ok = true;
-    int g = 0;
-    for (long long at = begin; at < end && ok; it.next(p)) {
-      const int b = it.bh / p.hkv, h = it.bh - b * p.hkv;
-      const int stop = static_cast<int>(min(end, it.first + it.n) - it.first);
-      for (int i = static_cast<int>(at - it.first); i < stop; ++i, ++g) {
-        const int sb = g & 1, hd = h * p.group + i / it.n_qt, q0 = it.kt * kKeys + i % it.n_qt * kTile;
-        const float* src = p.lse + b * p.l_sb + hd * p.l_sh + q0;
-        float x[4];
+      if (!ok) {
+        // products under way must not outlive the CTA's tensor memory (a limited wait)
+        int own = 0;
+        mma_commit(&ctl->drained);
+        mbar_wait(&ctl->drained, 0, &own, kErrWaitMma);
+      }
+    } else if (warp == 2) {
+      // ---------------------------------------------------------------- rows of -lse * log2(e)
+      bool ok = true;
+      int g = 0;
+      for (int r = 0; r < rounds && ok; ++r)
+      for (Walk it(p, ctl->share[r]); it.left > 0 && ok; it.next(p)) {
+        const int b = it.bh / p.hkv, h = it.bh - b * p.hkv;
+        for (int i = it.start; i < it.stop; ++i, ++g) {
+          const int sb = g & 1, hd = h * p.group + i / it.n_qt, q0 = it.kt * kKeys + i % it.n_qt * kTile;
+          const float* src = p.lse + b * p.l_sb + hd * p.l_sh + q0;
+          float x[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int r = k * 32 + lane;
-          x[k] = q0 + r < p.len ? src[r] * -1.4426950408889634f : -INFINITY;
-          if (x[k] == INFINITY) x[k] = -INFINITY;  // a query that saw nothing
+          for (int k = 0; k < 4; ++k) {
+            const int r = k * 32 + lane;
+            x[k] = q0 + r < p.len ? src[r] * -1.4426950408889634f : -INFINITY;
+            if (x[k] == INFINITY) x[k] = -INFINITY;  // a query that saw nothing
+          }
+          for (int t = 0; t < 2 && ok && g >= 2; ++t) ok = mbar_wait_w<100>(&ctl->s_free[sb][t], ((g >> 1) - 1) & 1, err, kErrWaitProducer);
+          if (!ok) break;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) sLse[sb * kTile + k * 32 + lane] = x[k];
+          __syncwarp();
+          if (lane < 2) mbar_arrive(&ctl->s_ready[sb][lane]);
         }
-        for (int t = 0; t < 2 && ok && g >= 2; ++t) ok = mbar_wait_w<100>(&ctl->s_free[sb][t], ((g >> 1) - 1) & 1, err, kErrWaitProducer);
-        if (!ok) break;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) sLse[sb * kTile + k * 32 + lane] = x[k];
-        __syncwarp();
-        if (lane < 2) mbar_arrive(&ctl->s_ready[sb][lane]);
       }
-      at = it.first + stop;
     }
-  } else if (warp >= 4) {
+  } else {
+    setmaxnreg_inc<104>();  // 128 x 64 + 512 x 104 <= 640 x 96 (the launch allocation)
     // ---------------------------------------------------------------- sums
     const int tile = (warp - 4) >> 3, half = (warp - 4) >> 2 & 1, key = tile * kTile + (warp & 3) * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -324,7 +355,8 @@ __global__ void __launch_bounds__(kThreads, 1) weight_sums_kernel(const __grid_c
     const float2 sl = make_float2(p.scale_log2, p.scale_log2);
     bool ok = true;
     int g = 0;
-    for (long long at = begin; at < end && ok; it.next(p)) {
+    for (int r = 0; r < rounds && ok; ++r)
+    for (Walk it(p, ctl->share[r]); it.left > 0 && ok; it.next(p)) {
       const int t0 = it.kt * kKeys, t = t0 + key;
       // the queries that see this key
       int lo = 0x7fffffff, hi = -1;
@@ -337,10 +369,8 @@ __global__ void __launch_bounds__(kThreads, 1) weight_sums_kernel(const __grid_c
       }
       const uint32_t seen = static_cast<uint32_t>(max(hi - lo + 1, 0));
       float sum = 0.f, lost = 0.f;
-      const int stop = static_cast<int>(min(end, it.first + it.n) - it.first);
-      const int start = static_cast<int>(at - it.first);
-      int qt = start % it.n_qt - 1;
-      for (int i = start; i < stop; ++i, ++g) {
+      int qt = it.start % it.n_qt - 1;
+      for (int i = it.start; i < it.stop; ++i, ++g) {
         if (++qt == it.n_qt) qt = 0;
         const int sb = g & 1, q0 = t0 + qt * kTile + half * 64;
         ok = mbar_wait_w(&ctl->s_ready[sb][tile], (g >> 1) & 1, err, kErrWaitSoftmax);
@@ -390,14 +420,13 @@ __global__ void __launch_bounds__(kThreads, 1) weight_sums_kernel(const __grid_c
       if (half == 0) sum += s_half[key];
       ok = all_sum_warps(ok);
       if (ok && half == 0) {
-        const bool whole = start == 0 && stop == it.n;
+        const bool whole = it.start == 0 && it.stop == it.n(p);
         if (whole) {
           if (t < p.len) p.out[static_cast<long long>(it.bh) * p.len + t] = sum;
         } else {
-          p.part[(static_cast<long long>(blockIdx.x) * 2 + (start == 0 ? 1 : 0)) * kKeys + key] = sum;
+          p.part[((blockIdx.x + static_cast<long long>(r) * p.ctas) * 2 + (it.start == 0 ? 1 : 0)) * kKeys + key] = sum;
         }
       }
-      at = it.first + stop;
     }
   }
   tc_fence_before();
@@ -416,7 +445,7 @@ __global__ void __launch_bounds__(kKeys) weight_sums_join_kernel(const __grid_co
   griddep_wait();
   item_prefix(p, s_prefix, s_prefix + kScan + 1);
   const long long total = s_prefix[kScan] * p.group * p.hkv * p.batch;
-  const long long shares = n_shares(total, p.ctas);
+  const long long shares = n_shares(total, p);
   if (blockIdx.x + 1 >= shares) return;
   const long long at = share_begin(total, shares, blockIdx.x + 1);
   const Item it = item_at(p, s_prefix, at);
@@ -428,7 +457,7 @@ __global__ void __launch_bounds__(kKeys) weight_sums_join_kernel(const __grid_co
   if (t < p.len) p.out[static_cast<long long>(it.bh) * p.len + t] = sum;
 }
 
-int64_t part_bytes(int ctas) { return static_cast<int64_t>(ctas) * 2 * kKeys * 4; }
+int64_t part_bytes(int shares) { return static_cast<int64_t>(shares) * 2 * kKeys * 4; }
 
 template <int kD, bool kBf16>
 cudaError_t launch_sums(const SumsKernelParams& kp, cudaStream_t s) {
@@ -445,8 +474,8 @@ cudaError_t launch_sums(const SumsKernelParams& kp, cudaStream_t s) {
   e = launch_kernel(kern, dim3(kp.ctas), kThreads, kSmemBytes, s, true, kp);
   if (e != cudaSuccess) return e;
   count_launches(1);
-  if (kp.ctas > 1) {
-    e = launch_kernel(weight_sums_join_kernel, dim3(kp.ctas - 1), kKeys, 0, s, true, kp);
+  if (kp.ctas * kp.rounds > 1) {
+    e = launch_kernel(weight_sums_join_kernel, dim3(kp.ctas * kp.rounds - 1), kKeys, 0, s, true, kp);
     if (e != cudaSuccess) return e;
     count_launches(1);
   }
@@ -458,6 +487,12 @@ int sums_ctas(const rswa_weight_sums_params_t& p) {
   const long long steps = static_cast<long long>(p.batch) * p.n_q_heads * ((p.len + kTile - 1) / kTile) * 8;
   const int sms = sm_count();
   return static_cast<int>(steps < sms ? steps : sms);
+}
+
+// Rounds: the queries of one fit into L2, with room for what else passes through
+int sums_rounds(const rswa_weight_sums_params_t& p) {
+  const long long bytes = static_cast<long long>(p.batch) * p.len * p.n_q_heads * p.head_dim * 2;
+  return static_cast<int>(std::min<long long>(kMaxRounds, (bytes + kRoundBytes - 1) / kRoundBytes));
 }
 
 int check_sums(const rswa_weight_sums_params_t* p) {
@@ -486,6 +521,14 @@ int check_sums(const rswa_weight_sums_params_t* p) {
     set_error("%s: positions overflow int32", what);
     return RSWA_E_UNSUPPORTED;
   }
+  // (a CTA counts its steps in 32 bits: 40 minutes of work.  At most: what the window spans for every item, and all query
+  // tiles for those with a sink token)
+  const double tiles = p->len / kTile + 1.0, items = p->len / kKeys + 1.0;
+  const double steps = items * std::min(tiles, p->window / static_cast<double>(kTile) + 4.0) + tiles * (p->n_sink / static_cast<double>(kKeys) + 2.0);
+  if (steps * p->n_q_heads * p->batch > 100.0 * 0x7fffffff) {
+    set_error("%s: too many tiles in one call", what);
+    return RSWA_E_UNSUPPORTED;
+  }
   if (p->cu_seqlens != nullptr && (p->batch != 1 || p->n_seqs <= 0)) {
     set_error("%s: packed (cu_seqlens) input needs batch == 1 and n_seqs > 0", what);
     return RSWA_E_ARG;
@@ -505,7 +548,7 @@ using namespace rswa;
 
 extern "C" int64_t rswa_weight_sums_workspace_bytes(const rswa_weight_sums_params_t* p) {
   const int rc = check_sums(p);
-  return rc != RSWA_OK ? rc : part_bytes(sums_ctas(*p));
+  return rc != RSWA_OK ? rc : part_bytes(sums_ctas(*p) * sums_rounds(*p));
 }
 
 extern "C" int rswa_weight_sums(const rswa_weight_sums_params_t* p, void* stream) {
@@ -518,8 +561,10 @@ extern "C" int rswa_weight_sums(const rswa_weight_sums_params_t* p, void* stream
   }
   SumsKernelParams kp;
   kp.ctas = sums_ctas(*p);
-  if (p->workspace == nullptr || p->workspace_bytes < part_bytes(kp.ctas)) {
-    set_error("%s: the workspace must hold %lld bytes", what, static_cast<long long>(part_bytes(kp.ctas)));
+  kp.rounds = sums_rounds(*p);
+  const int shares = kp.ctas * kp.rounds;
+  if (p->workspace == nullptr || p->workspace_bytes < part_bytes(shares)) {
+    set_error("%s: the workspace must hold %lld bytes", what, static_cast<long long>(part_bytes(shares)));
     return RSWA_E_ARG;
   }
   rc = make_tile_map(&kp.q_map, p->q, p->dtype, p->batch, p->len, p->n_q_heads, p->head_dim, p->q_stride_b, p->q_stride_t, p->q_stride_h);
