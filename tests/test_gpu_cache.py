@@ -416,6 +416,23 @@ def test_weight_sums_of_the_forward_kernels_and_run_to_run():
     assert torch.equal(got, ops.attn_weight_sums(q, k, lse, window, sink))
 
 
+@pytest.mark.parametrize("window,sink", [(300, 0), (2000, 4)])
+def test_weight_sums_of_more_queries_than_l2_holds(window, sink):
+    """All heads in one call, whose work is cut into rounds, against a call for each key/value head.  Tolerance: the sums of a
+    step are the same; compensated sums over steps err by 2 roundings, the halves' and up to three pieces' additions by 3
+    more, on either side."""
+    ops = _ops()
+    s, hq, hkv, d = 18500, 32, 2, 64
+    q, k = normal(1, s, hq, d, seed=1, dt="bf16").cuda(), normal(1, s, hkv, d, seed=2, dt="bf16").cuda()
+    lse = (normal(1, hq, s, seed=3, dt="bf16").float() + 4.0).cuda()
+    got = ops.attn_weight_sums(q, k, lse, window, sink)
+    g = hq // hkv
+    for h in range(hkv):
+        one = ops.attn_weight_sums(q[:, :, h * g:(h + 1) * g], k[:, :, h:h + 1], lse[:, h * g:(h + 1) * g], window, sink)
+        torch.testing.assert_close(got[:, h], one[:, 0], rtol=10 * 2.0 ** -24, atol=0)
+    assert torch.equal(got, ops.attn_weight_sums(q, k, lse, window, sink))
+
+
 EVICT = [
     # lens, heads, d, bs, budget, sink, recent
     ([100], 1, 64, 16, 40, 0, 0),
