@@ -501,6 +501,45 @@ def test_evict(case, kind):
             assert torch.equal(x, y)
 
 
+def test_evict_by_clusters_in_a_graph_and_on_two_streams():
+    """Long contexts, several CTAs a head: a captured call replayed with other lengths and weights, and eager calls on two
+    streams beside each other, give what single calls give."""
+    ops = _ops()
+    n, heads, bs, d, budget = 40000, 2, 64, 64, 3000
+    cache, table, _, _, _ = filled("int8", "bf16", [n], heads, bs, d, seed=5, spare=2 * 47 + 1)
+    used = set(table.flatten().tolist())
+    free = [i for i in range(cache.k.shape[0]) if i not in used]
+    table = table[:, :n // bs].contiguous().cuda()
+    new = [torch.tensor([free[i * 47:(i + 1) * 47]], dtype=torch.int32).cuda() for i in range(2)]
+    weights = [torch.rand(1, heads, n, generator=torch.Generator().manual_seed(i)).cuda() for i in range(3)]
+    lens = [torch.tensor([m], dtype=torch.int32).cuda() for m in (n, 25000, 2999)]
+    call = lambda m, w, to: ops.cache_evict(cache, table, m, w, budget, to, 4, 100)
+    want = [[x.clone() for x in call(lens[i], weights[i], new[0])] + [x.clone() for x in ops.cache_read(cache, new[0], lens[2] * 0 + min(budget, int(lens[i])), budget)]
+            for i in range(3)]
+    m, w = lens[0].clone(), weights[0].clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call(m, w, new[0])
+        back = ops.cache_read(cache, new[0], got[0], budget)
+    for i in (2, 1, 0):
+        m.copy_(lens[i]), w.copy_(weights[i])
+        graph.replay()
+        for x, y in zip([*got, *back], want[i]):
+            assert torch.equal(x, y)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    results = [None, None]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                results[i] = call(lens[i], weights[i], new[i])
+    torch.cuda.synchronize()
+    for i in range(2):
+        for x, y in zip(results[i], want[i]):
+            assert torch.equal(x, y)
+
+
 def test_evict_keeps_poison_and_reports_bad_tables():
     ops = _ops()
     cache, table, _, _, _ = filled("int8", "bf16", [64], 2, 16, 64, seed=1, spare=4)
