@@ -817,7 +817,9 @@ __global__ void __launch_bounds__(kAdd) cache_weights_kernel(const __grid_consta
 #pragma unroll
       for (int v = 0; v < kRows / 4; ++v) {
         const float* lse = s_lse + rt * kRows + v * 4;
-        sum[e] += ex2f(x[e][v].x - lse[0]) + ex2f(x[e][v].y - lse[1]) + ex2f(x[e][v].z - lse[2]) + ex2f(x[e][v].w - lse[3]);
+        // (a hidden slot's score is -inf: nothing from that row, not even where the row's log-sum-exp is NaN)
+        const auto part = [](float s, float l) { return s == -INFINITY ? 0.f : ex2f(s - l); };
+        sum[e] += part(x[e][v].x, lse[0]) + part(x[e][v].y, lse[1]) + part(x[e][v].z, lse[2]) + part(x[e][v].w, lse[3]);
       }
   }
 #pragma unroll

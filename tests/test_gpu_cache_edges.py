@@ -1,0 +1,66 @@
+"""The 8-bit key/value cache on the GPU where it could go wrong beside the listed forms: rows that are not finite, freed
+blocks, block tables that share their rows, scales from elsewhere, streams from elsewhere.
+
+Against the definitions in 64 bits (cache_ref.py), with the tolerances that test_gpu_cache.py derives; where a test needs more,
+it says why.
+"""
+import math
+
+import pytest
+import torch
+
+import cache_ref as R
+from test_gpu_cache import _ops, filled, host, make, normal
+
+pytestmark = pytest.mark.gpu
+
+
+def same_nan(got, want, what):
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), f"{what}: NaN in {torch.isnan(got).sum().item()} places, wanted in {torch.isnan(want).sum().item()}"
+
+
+def check_spoiled_attn(cache, table, lens, q, window, sink, more=0.0):
+    """out, log-sum-exp and weights against the definition: NaN exactly where that has NaN, the rest within the tolerances."""
+    n = table.shape[1] * cache.k.shape[2]
+    start = torch.rand(len(lens), cache.k.shape[1], n, generator=torch.Generator().manual_seed(1))
+    acc = start.cuda()
+    out, lse = (x.cpu().double() for x in _ops().cache_attn(q.cuda(), cache, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), window_size=window,
+                                                            num_sink_tokens=sink, weights=acc, return_lse=True))
+    acc = acc.cpu().double()
+    want, want_lse, w, size, most = R.attn(host(cache), table, lens, q.double(), window, sink)
+    want_acc = start.double()
+    want_acc[..., :w.shape[-1]] += w
+    same_nan(acc, want_acc, "weights"), same_nan(lse, want_lse, "lse"), same_nan(out, want, "out")
+    e = (q.shape[-1] + 8) * 2.0 ** -24 * most + more
+    eps = torch.finfo(q.dtype).eps / 2
+    ok = torch.isfinite(want)
+    tol = eps * want.abs() + (1 + eps) * (2.0 ** -11 + 2 * e + 2.0 ** -18) * size
+    err = (out - want).abs()
+    assert (err <= tol)[ok].all(), f"out: {(err / tol)[ok].max().item():.3g} of the tolerance"
+    ok = torch.isfinite(want_lse)
+    tol = e + 2.0 ** -20 * (1 + want_lse.abs())
+    assert torch.equal(torch.isfinite(lse), ok) and ((lse - want_lse).abs() <= tol)[ok].all(), f"lse: off by {(lse - want_lse).abs()[ok].max().item():.3g}"
+    ok = torch.isfinite(want_acc)
+    rows = q.shape[1] * q.shape[2]
+    tol = (2 * e + 2.0 ** -18 + rows * 2.0 ** -24) * (want_acc - start) + 2.0 ** -24 * want_acc
+    err = (acc - want_acc).abs()
+    assert (err <= tol)[ok].all(), f"weights: {(err / tol)[ok].max().item():.3g} of the tolerance"
+    return ok
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("bs", [16, 64])
+@pytest.mark.parametrize("what", ["query", "key", "old key"])
+def test_weights_of_slots_that_a_spoiled_row_does_not_see(what, bs, dt):
+    """A row that is NaN adds NaN to the slots that it sees, and nothing to the others of the same tiles: in front of the
+    window, behind the sinks, behind its own place, behind the sequence's end."""
+    lens, d, window, sink = [200, 37], 64, 75, 4
+    cache, table, _, _, _ = filled("int8", dt, lens, 2, bs, d, seed=4)
+    q = normal(2, 3, 4, d, seed=5, dt=dt)
+    if what == "query":
+        q[0, 1, 2, 7] = math.nan
+    else:  # the block of the newest slots, or one in the middle of the window that the last rows still see
+        cache.k_scale[table[0, (199 if what == "key" else 150) // bs].item(), 0] = math.nan
+    seen = check_spoiled_attn(cache, table, lens, q, window, sink)
+    assert not seen[0].all() and seen[1].all() and seen[0, :, 4:32].all() and seen[0, :, 200:].all()
+    check_spoiled_attn(cache, table, lens, q, None, 0)
