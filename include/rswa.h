@@ -356,6 +356,8 @@ int rswa_cache_read(const rswa_cache_read_params_t* p, void* stream);
  * dimension contiguous, all multiples of 8, 16-byte aligned); out [batch, q_len, Hq, head_dim] contiguous; lse
  * [batch, Hq, q_len] float (natural log) or NULL.  A query before the sequence's start, or of an empty one, gives a
  * zero row and lse -inf.
+ * A scale of V that is not finite makes NaN of the outputs that see its block; lse and weights come from K alone.
+ * NaN from a query or a scale of K stays with the rows that see it, and with the weights of the slots which these rows see.
  * weights (or NULL): float [batch, n_kv_heads, >= max_blocks * block_size], tokens contiguous; every slot seen has
  * the softmax weights added that it got from the queries and heads of its key/value head.  Needs lse.
  * `workspace`: rswa_cache_attn_workspace_bytes() of device memory, 256-byte aligned, for the time of the call.

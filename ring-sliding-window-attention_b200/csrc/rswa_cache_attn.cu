@@ -225,7 +225,7 @@ struct Layout {
   static constexpr int kThreads = kWarps * 32, kGroup = kAll ? kWarps : 4, kGroups = kWarps / kGroup;
   struct Ctl {
     uint64_t full[kWarps][2];           // K, V
-    float4 scale[kWarps][32][2];        // the looked-up tiles: of the first 16 tokens and the last 16 K's scale, log2 of V's, 1 / V's
+    float4 scale[kWarps][32][2];        // the looked-up tiles: of the first 16 tokens and the last 16 K's scale, log2 of V's, 1 / V's (negative: V's is not finite)
     int2 row[kWarps][32];               // and where their K and V lie
     float ml[kWarps][8 * kNT][2];       // reference and sum of every warp's piece
     int prefix[kScan + 1 + kScan / 32];
@@ -414,7 +414,11 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
   };
   auto put_scales = [&]() {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) ctl.scale[warp][lane][t] = make_float4(scale[0][t], __log2f(scale[1][t]), 1.f / scale[1][t], 0.f);
+    for (int t = 0; t < 2; ++t) {
+      // (V's scale is not finite: 1 for the sum of the weights, which depends on K alone, and marked by the sign of the reciprocal)
+      const bool spoiled = !(fabsf(scale[1][t]) <= 3.4028235e38f);
+      ctl.scale[warp][lane][t] = make_float4(scale[0][t], spoiled ? 0.f : __log2f(scale[1][t]), spoiled ? -1.f : 1.f / scale[1][t], 0.f);
+    }
     __syncwarp();
   };
   int loaded[2] = {0, 0};  // loads so far
@@ -643,10 +647,15 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
         const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const float a = ex2f(acc[t][nt][0] - m0), b = ex2f(acc[t][nt][1] - m1);
-          const float d = ex2f(acc[t][nt][2] - m0), e = ex2f(acc[t][nt][3] - m1);
-          l[nt][0] += a + d == 0.f ? 0.f : (a + d) * iv[t];
-          l[nt][1] += b + e == 0.f ? 0.f : (b + e) * iv[t];
+          float a = ex2f(acc[t][nt][0] - m0), b = ex2f(acc[t][nt][1] - m1);
+          float d = ex2f(acc[t][nt][2] - m0), e = ex2f(acc[t][nt][3] - m1);
+          l[nt][0] += a + d == 0.f ? 0.f : (a + d) * fabsf(iv[t]);
+          l[nt][1] += b + e == 0.f ? 0.f : (b + e) * fabsf(iv[t]);
+          if (iv[t] < 0.f) {  // values that are not finite: NaN for the rows that see them, whatever the weight
+            const float nan = __uint_as_float(0x7fffffffu);
+            a = acc[t][nt][0] == -INFINITY ? 0.f : nan, b = acc[t][nt][1] == -INFINITY ? 0.f : nan;
+            d = acc[t][nt][2] == -INFINITY ? 0.f : nan, e = acc[t][nt][3] == -INFINITY ? 0.f : nan;
+          }
           pf[t][nt][0] = transpose8(pack2<false>(a, b));
           pf[t][nt][1] = transpose8(pack2<false>(d, e));
         }

@@ -129,6 +129,9 @@ def cache_attn(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, lens:
     weights: float32 [batch, num_kv_heads, at least max_blocks * block_size], added to in place: the softmax weights that
     every slot got from the queries and heads of its key/value head (what cache_evict goes by; start it with
     attn_weight_sums of the prompt, or zeros).
+
+    NaN reaches the rows that see it and no others: from a query or a block of keys the output, the log-sum-exp and the weights of
+    the slots which the row sees, from a block of values the output alone.
     """
     return _call_cache("cache_attn", cache, q, block_table, lens, window_size, num_sink_tokens, softmax_scale, weights, return_lse)
 

@@ -64,3 +64,19 @@ def test_weights_of_slots_that_a_spoiled_row_does_not_see(what, bs, dt):
     seen = check_spoiled_attn(cache, table, lens, q, window, sink)
     assert not seen[0].all() and seen[1].all() and seen[0, :, 4:32].all() and seen[0, :, 200:].all()
     check_spoiled_attn(cache, table, lens, q, None, 0)
+
+
+@pytest.mark.parametrize("kind,dt", [("int8", "bf16"), ("e4m3", "fp16")])
+@pytest.mark.parametrize("bs", [16, 128])
+def test_values_that_are_not_finite_leave_weights_and_log_sum_exp_alone(bs, kind, dt):
+    """A block of V whose scale is NaN or infinite makes the outputs NaN that see it; what depends on K alone stays."""
+    lens, d, window, sink = [300, 50], 128, 135, 2
+    for bad in (math.nan, math.inf):
+        cache, table, _, _, _ = filled(kind, dt, lens, 2, bs, d, seed=6)
+        for b, slot, h in ((0, 145, 1), (0, 299, 0), (1, 0, 0)):
+            page = table[b, slot // bs].item()
+            cache.v_scale[page, h] = bad
+            cache.v.view(torch.uint8)[page, h] = 0  # (as cache_append stores them)
+        q = normal(2, 20, 4, d, seed=7, dt=dt)
+        check_spoiled_attn(cache, table, lens, q, window, sink)
+        check_spoiled_attn(cache, table, lens, q[:, :1], None, 0)
