@@ -285,7 +285,8 @@ float rswa_event_elapsed_ms(void* start, void* stop);
  * The cache: k and v [num_blocks, n_kv_heads, block_size, head_dim], one byte per element, and for each block and
  * head one float scale: value = stored * scale.  kind RSWA_CACHE_INT8: two's complement, -127..127; kind
  * RSWA_CACHE_E4M3: 4 exponent and 3 mantissa bits (no infinities, up to 448).  rswa_cache_append and
- * rswa_cache_evict write scales that are powers of two; the others take any positive ones.
+ * rswa_cache_evict write scales that are powers of two, 2^-100 or more; the others take any positive ones (rswa_cache_attn:
+ * a scale of V below 2^-100 counts as that; above 2^80 its log-sum-exp and weights lose digits).
  * block_size: 16, 32, 64 or 128 tokens; head_dim: 64 or 128; every base 16-byte aligned.
  *
  * Sequence b's tokens lie, in order, in the blocks named by row b of a block table (int32, device memory; rows

@@ -23,7 +23,9 @@
 // Queries and weights are fp16 operands: a bf16 query is scaled by a power of two to the top of the fp16 range (exact
 // but for elements 2^-28 smaller than the row's largest), the weights are at most 2^14 with 11 bits each.  The scale of
 // a V block goes into its tokens' exponents (s + log2 of the scale), so that the running reference covers both;
-// the sum of the weights takes it back out.  Scores, sums and the output are 32-bit.
+// the sum of the weights takes it back out.  Scores, sums and the output are 32-bit.  (The sum of the weights is kept in units
+// of 2^8 of the reference, and takes exponentials of its own from blocks of V with scales below 2^-20, such as blocks of zeros: with
+// the scale in it a weight falls out of the range of 32 bits where another block's V is 2^100 times larger.)
 //
 // Work: the 32-token tiles of all (sequence, key/value head, 8 or 16 query rows) in one order, cut evenly whatever the
 // lengths over groups of warps.  The warps of a group take its tiles in turn and add up at the end of each piece; each item
@@ -36,6 +38,7 @@
 // all of them.  The pieces of an item that is cut go to the workspace, and the group that delivers the last one joins them,
 // in order: results do not depend on timing.
 #include <atomic>
+#include <type_traits>
 
 #include "rswa_cache.cuh"
 
@@ -53,6 +56,10 @@ constexpr int kScan = 256;   // threads of the prefix sums over sequences
 constexpr int kAdd = 256;    // threads of a CTA that adds weights up
 constexpr float kRoom = 14.f;  // a weight may grow to 2^14 before the reference is raised (fp16 ends at 2^16)
 constexpr float kLow = 4.f;    // and is raised to the maximum minus 4, so that not every new maximum raises it
+constexpr float kSumUnit = 8.f;    // sums of weights are in units of 2^8: 2^21 tokens of weight 2^14 under V's least scale, 2^-100, stay finite
+constexpr float kSumScale = 1.f / 256;
+constexpr float kTinyV = -20.f;    // log2 of V's scale, below which the sum has exponentials of its own
+constexpr float kLeastV = 7.888609052210118e-31f;  // 2^-100, what V's scale counts as at least
 
 struct AttnKernelParams {
   CUtensorMap map[2];
@@ -225,7 +232,7 @@ struct Layout {
   static constexpr int kThreads = kWarps * 32, kGroup = kAll ? kWarps : 4, kGroups = kWarps / kGroup;
   struct Ctl {
     uint64_t full[kWarps][2];           // K, V
-    float4 scale[kWarps][32][2];        // the looked-up tiles: of the first 16 tokens and the last 16 K's scale, log2 of V's, 1 / V's (negative: V's is not finite)
+    float4 scale[kWarps][32][2];        // the looked-up tiles: of the first 16 tokens and the last 16 K's scale, log2 of V's, 2^-kSumUnit / V's (negative: see put_scales)
     int2 row[kWarps][32];               // and where their K and V lie
     float ml[kWarps][8 * kNT][2];       // reference and sum of every warp's piece
     int prefix[kScan + 1 + kScan / 32];
@@ -275,12 +282,12 @@ __device__ __forceinline__ void sync_group(int group) {
 template <int kD>
 __device__ __forceinline__ void store_row(const AttnKernelParams& p, int b, int h, int row, int d4, float4 x, float top, float sum) {
   const int i = row / p.group, hd = h * p.group + row - i * p.group;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum * kSumScale;
   uint16_t* const to = p.out + ((static_cast<long long>(b) * p.q_len + i) * p.hq + hd) * kD + d4 * 4;
   *reinterpret_cast<uint2*>(to) = p.bf16 ? make_uint2(pack2<true>(x.x * inv, x.y * inv), pack2<true>(x.z * inv, x.w * inv))
                                          : make_uint2(pack2<false>(x.x * inv, x.y * inv), pack2<false>(x.z * inv, x.w * inv));
   if (p.lse != nullptr && d4 == 0)
-    p.lse[(static_cast<long long>(b) * p.hq + hd) * p.q_len + i] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.6931471805599453f;
+    p.lse[(static_cast<long long>(b) * p.hq + hd) * p.q_len + i] = sum == 0.f ? -INFINITY : (top + kSumUnit + __log2f(sum)) * 0.6931471805599453f;
 }
 
 // The rows of the sequences that have nothing to attend to, by the first kPeers threads of every CTA.
@@ -310,9 +317,11 @@ __device__ __forceinline__ void join_pieces(const AttnKernelParams& p, float* me
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     const auto add = [&](float m, float l, float4 y) {  // a later piece
       const float next = fmaxf(top, m);
-      const float f = sum == 0.f ? 0.f : ex2f(top - next), w = l == 0.f ? 0.f : ex2f(m - next);
+      // (references may lie so far apart, by V's scales, that the factor is 0 where a sum times the factor is not)
+      const float fh = sum == 0.f ? 0.f : ex2f(0.5f * (top - next)), wh = l == 0.f ? 0.f : ex2f(0.5f * (m - next));
+      const float f = fh * fh, w = wh * wh;
       top = next;
-      sum = sum * f + l * w;
+      sum = sum * fh * fh + l * wh * wh;
       x.x = x.x * f + y.x * w, x.y = x.y * f + y.y * w, x.z = x.z * f + y.z * w, x.w = x.w * f + y.w * w;
     };
     if (row < p.rows && part < kParts) {
@@ -415,9 +424,11 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
   auto put_scales = [&]() {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      // (V's scale is not finite: 1 for the sum of the weights, which depends on K alone, and marked by the sign of the reciprocal)
+      // (V's scale is not finite: 1 for the sum of the weights, which depends on K alone.  Such scales and tiny ones have a
+      // negative reciprocal, with a logarithm of 0 or a negative one)
       const bool spoiled = !(fabsf(scale[1][t]) <= 3.4028235e38f);
-      ctl.scale[warp][lane][t] = make_float4(scale[0][t], spoiled ? 0.f : __log2f(scale[1][t]), spoiled ? -1.f : 1.f / scale[1][t], 0.f);
+      const float sv = spoiled ? 1.f : fmaxf(scale[1][t], kLeastV), lg = __log2f(sv), inv = 1.f / sv * kSumScale;
+      ctl.scale[warp][lane][t] = make_float4(scale[0][t], lg, spoiled || lg < kTinyV ? -inv : inv, 0.f);
     }
     __syncwarp();
   };
@@ -633,33 +644,42 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
             const float old = m[nt][k];
             const float next = x - kLow > old ? x - kLow : old;
-            const float f = next > old ? ex2f(old - next) : 1.f;
+            const float h = next > old ? ex2f(0.5f * (old - next)) : 1.f, f = h * h;
             m[nt][k] = next;
-            l[nt][k] *= f;
+            l[nt][k] = l[nt][k] * h * h;  // (not times h * h, see join_pieces)
 #pragma unroll
             for (int s = 0; s < kKS; ++s) o[nt][s][k] *= f, o[nt][s][k + 2] *= f;
           }
       }
       // ---- weights, as the right operand of V^T P^T
       uint32_t pf[2][kNT][2];
+      const auto weigh = [&](auto usual) {
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) {
-        const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+        for (int nt = 0; nt < kNT; ++nt) {
+          const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          float a = ex2f(acc[t][nt][0] - m0), b = ex2f(acc[t][nt][1] - m1);
-          float d = ex2f(acc[t][nt][2] - m0), e = ex2f(acc[t][nt][3] - m1);
-          l[nt][0] += a + d == 0.f ? 0.f : (a + d) * fabsf(iv[t]);
-          l[nt][1] += b + e == 0.f ? 0.f : (b + e) * fabsf(iv[t]);
-          if (iv[t] < 0.f) {  // values that are not finite: NaN for the rows that see them, whatever the weight
-            const float nan = __uint_as_float(0x7fffffffu);
-            a = acc[t][nt][0] == -INFINITY ? 0.f : nan, b = acc[t][nt][1] == -INFINITY ? 0.f : nan;
-            d = acc[t][nt][2] == -INFINITY ? 0.f : nan, e = acc[t][nt][3] == -INFINITY ? 0.f : nan;
+          for (int t = 0; t < 2; ++t) {
+            const float(&x)[4] = acc[t][nt];
+            float a = ex2f(x[0] - m0), b = ex2f(x[1] - m1), d = ex2f(x[2] - m0), e = ex2f(x[3] - m1);
+            if (decltype(usual)::value || iv[t] > 0.f || lv[t] == 0.f) {
+              l[nt][0] += (a + d) * fabsf(iv[t]);
+              l[nt][1] += (b + e) * fabsf(iv[t]);
+            } else {
+              const float u = lv[t] + kSumUnit;
+              l[nt][0] += ex2f(x[0] - m0 - u) + ex2f(x[2] - m0 - u);
+              l[nt][1] += ex2f(x[1] - m1 - u) + ex2f(x[3] - m1 - u);
+            }
+            if (!decltype(usual)::value && iv[t] < 0.f && lv[t] == 0.f) {  // NaN for the rows that see it, whatever the weight
+              const float nan = __uint_as_float(0x7fffffffu);
+              a = x[0] == -INFINITY ? 0.f : nan, b = x[1] == -INFINITY ? 0.f : nan;
+              d = x[2] == -INFINITY ? 0.f : nan, e = x[3] == -INFINITY ? 0.f : nan;
+            }
+            pf[t][nt][0] = transpose8(pack2<false>(a, b));
+            pf[t][nt][1] = transpose8(pack2<false>(d, e));
           }
-          pf[t][nt][0] = transpose8(pack2<false>(a, b));
-          pf[t][nt][1] = transpose8(pack2<false>(d, e));
         }
-      }
+      };
+      if (fminf(iv[0], iv[1]) > 0.f) weigh(std::true_type()); else weigh(std::false_type());
       // ---- output
       if (!dead) dead = !mbar_wait_w(full + 1, done & 1, &ctl.err, kErrWaitProducer);
       if (!kInt8 && slot + kTok > cc.s.len) {
@@ -729,9 +749,9 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
 #pragma unroll
         for (int w = 0; w < kGroup; ++w) {
           const float lw = ml[w][nt * 8 + r][1];
-          const float f = lw == 0.f ? 0.f : ex2f(ml[w][nt * 8 + r][0] - top);  // (0: no visible token)
+          const float fh = lw == 0.f ? 0.f : ex2f(0.5f * (ml[w][nt * 8 + r][0] - top)), f = fh * fh;  // (0: no visible token)
           const float4 y = *reinterpret_cast<const float4*>(merge + (w * 8 + r) * kD + ((d4 * 4) ^ (r / 2 * 8)));
-          sum += lw * f;
+          sum += lw * fh * fh;
           x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
         }
         if (row < p.rows) {

@@ -65,7 +65,8 @@ class KVCache:
     cache_append and cache_evict write scales that are powers of two, the least ones that hold a block's values: moving
     a token to another block or reading it back rounds nothing that the other scale can hold.  int8 has the smaller error
     where a block's values are of one magnitude, float8_e4m3fn where they are not.  Tensors filled elsewhere may have
-    any positive scales (and no NaN among float8_e4m3fn values: a NaN belongs into the scale).
+    any positive scales (V's from 2^-100 to 2^80, a smaller one counts as 2^-100 in cache_attn; and no NaN among float8_e4m3fn
+    values: a NaN belongs into the scale).
     """
     __slots__ = ("k", "v", "k_scale", "v_scale")
 

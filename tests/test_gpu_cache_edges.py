@@ -80,3 +80,18 @@ def test_values_that_are_not_finite_leave_weights_and_log_sum_exp_alone(bs, kind
         q = normal(2, 20, 4, d, seed=7, dt=dt)
         check_spoiled_attn(cache, table, lens, q, window, sink)
         check_spoiled_attn(cache, table, lens, q[:, :1], None, 0)
+
+
+@pytest.mark.parametrize("kind,bs", [("int8", 16), ("e4m3", 64)])
+@pytest.mark.parametrize("small,large", [(-100, -100), (-100, 0), (-100, 60), (-60, 40), (80, 80)])
+def test_values_of_very_different_magnitude(small, large, kind, bs):
+    """V's scales as far apart as 2^-100 (a block of zeros, or nearly) and 2^80: the log-sum-exp and the weights do not know about V.
+    `more`: exponents carry the scale's logarithm, up to 2^7 large; at most four roundings of half a step there, 2^-18 each
+    (2^-17 behind an addition), times ln 2 and 2."""
+    lens, d = [700, 90], 64
+    cache, table, _, _, _ = filled(kind, "bf16", lens, 2, bs, d, seed=8)
+    some = (torch.arange(cache.v.shape[0], device="cuda") % 3 == 0)[:, None]
+    cache.v_scale.copy_(torch.where(some, 2.0 ** large, 2.0 ** small))
+    q = normal(2, 2, 8, d, seed=9, dt="bf16")
+    check_spoiled_attn(cache, table, lens, q, None, 0, more=2.0 ** -15)
+    check_spoiled_attn(cache, table, lens, q[:, :1], 60, 1, more=2.0 ** -15)
