@@ -22,6 +22,7 @@
 // A thread's running sum is compensated: a key may be seen by 10^5 queries and more.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "rswa_common.cuh"
 #include "tc05.cuh"
@@ -388,21 +389,25 @@ __global__ void __launch_bounds__(kThreads, 1) weight_sums_kernel(const __grid_c
           for (int c = 0; c < 2; ++c) {
             tmem_ld_wait();
             if (c == 0) tmem_ld32(from + 32, x[1]);
-            if (masked) {
-              const uint32_t at0 = static_cast<uint32_t>(q0 + c * 32 - lo);
+            // (hidden pairs are taken out of the exponents, behind the log-sum-exps: one that is NaN is not theirs)
+            const uint32_t at0 = static_cast<uint32_t>(q0 + c * 32 - lo);
+            const auto add = [&](auto some_hidden) {
 #pragma unroll
-              for (int k = 0; k < 32; ++k) x[c][k] = at0 + k < seen ? x[c][k] : 0xff800000u;
-            }
-#pragma unroll
-            for (int k = 0; k < 32; k += 4) {
-              const float4 l = *reinterpret_cast<const float4*>(lse + c * 32 + k);
-              const float2 a = __ffma2_rn(make_float2(__uint_as_float(x[c][k]), __uint_as_float(x[c][k + 1])), sl, make_float2(l.x, l.y));
-              const float2 b = __ffma2_rn(make_float2(__uint_as_float(x[c][k + 2]), __uint_as_float(x[c][k + 3])), sl, make_float2(l.z, l.w));
-              const float2 ea = make_float2(ex2f(a.x), ex2f(a.y));
-              const float2 eb = k % 16 == 0 ? fma_exp2(b) : make_float2(ex2f(b.x), ex2f(b.y));
-              acc[k / 4 % 2 * 2] = __fadd2_rn(acc[k / 4 % 2 * 2], ea);
-              acc[k / 4 % 2 * 2 + 1] = __fadd2_rn(acc[k / 4 % 2 * 2 + 1], eb);
-            }
+              for (int k = 0; k < 32; k += 4) {
+                const float4 l = *reinterpret_cast<const float4*>(lse + c * 32 + k);
+                float2 a = __ffma2_rn(make_float2(__uint_as_float(x[c][k]), __uint_as_float(x[c][k + 1])), sl, make_float2(l.x, l.y));
+                float2 b = __ffma2_rn(make_float2(__uint_as_float(x[c][k + 2]), __uint_as_float(x[c][k + 3])), sl, make_float2(l.z, l.w));
+                if (decltype(some_hidden)::value) {
+                  a.x = at0 + k < seen ? a.x : -INFINITY, a.y = at0 + k + 1 < seen ? a.y : -INFINITY;
+                  b.x = at0 + k + 2 < seen ? b.x : -INFINITY, b.y = at0 + k + 3 < seen ? b.y : -INFINITY;
+                }
+                const float2 ea = make_float2(ex2f(a.x), ex2f(a.y));
+                const float2 eb = k % 16 == 0 ? fma_exp2(b) : make_float2(ex2f(b.x), ex2f(b.y));
+                acc[k / 4 % 2 * 2] = __fadd2_rn(acc[k / 4 % 2 * 2], ea);
+                acc[k / 4 % 2 * 2 + 1] = __fadd2_rn(acc[k / 4 % 2 * 2 + 1], eb);
+              }
+            };
+            if (masked) add(std::true_type()); else add(std::false_type());
           }
           const float2 s2 = __fadd2_rn(__fadd2_rn(acc[0], acc[1]), __fadd2_rn(acc[2], acc[3]));
           // (compensated: `lost` is what the last addition rounded away)

@@ -95,3 +95,32 @@ def test_values_of_very_different_magnitude(small, large, kind, bs):
     q = normal(2, 2, 8, d, seed=9, dt="bf16")
     check_spoiled_attn(cache, table, lens, q, None, 0, more=2.0 ** -15)
     check_spoiled_attn(cache, table, lens, q[:, :1], 60, 1, more=2.0 ** -15)
+
+
+def check_spoiled_sums(q, k, lse, window, sink, lens):
+    """Packed sums against the definition: NaN exactly where that has NaN.  (Tolerance: test_gpu_cache.py.)"""
+    cu = torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), dtype=torch.int32).cuda()
+    got = _ops().attn_weight_sums(q.cuda(), k.cuda(), lse.cuda(), window, sink, cu_seqlens=cu).cpu().double()
+    want, most, _ = R.weight_sums(q.double(), k.double(), lse, window, sink, None, lens)
+    same_nan(got, want, "sums")
+    e = (q.shape[-1] + 8) * 2.0 ** -24 * most
+    rel = e + 2.0 ** -24 * (most + lse[torch.isfinite(lse)].abs().max().item()) + 2.0 ** -20 + 128 * 2.0 ** -24 + 2.0 ** -23
+    ok = torch.isfinite(want)
+    assert ((got - want).abs() <= rel * want)[ok].all(), f"{((got - want).abs() / want)[ok & (want > 0)].max().item():.3g} instead of {rel:.3g}"
+    return got, want
+
+
+@pytest.mark.parametrize("dt,d", [("bf16", 64), ("fp16", 128)])
+def test_sums_of_keys_that_a_spoiled_query_does_not_see(dt, d):
+    """A NaN log-sum-exp spoils the keys that its query sees: none in front of the window, behind the query or in another sequence."""
+    lens, window, sink = [4, 4, 130, 600, 90], 100, 3
+    t = sum(lens)
+    q, k = normal(t, 4, d, seed=1, dt=dt), normal(t, 2, d, seed=2, dt=dt)
+    lse = 3 + normal(4, t, seed=3, dt="bf16").float()
+    for head, i in ((0, 5), (1, 60), (2, 500), (3, 137), (3, t - 1)):
+        lse[head, i] = math.nan
+    got, want = check_spoiled_sums(q, k, lse, window, sink, lens)
+    assert torch.isfinite(got[:, :4]).all() and torch.isnan(got[0, 4:6]).all()
+    # the query NaN besides, as it comes out of a model
+    q[5, 0], q[500, 2, 3] = math.nan, math.nan
+    check_spoiled_sums(q, k, lse, window, sink, lens)
