@@ -158,11 +158,11 @@ struct Walk {
 };
 
 // 2^x for two values on the FMA pipe: x = n + f with n = round(x) and f in [-0.5, 0.5]; 2^f by the polynomial of degree 5 with
-// the least relative error there (7.5e-8, found by exchange of its extrema; 2.1e-7 in 32 bits), times 2^n from n's bits.  Below
-// -125 (hidden scores are -inf) 2^-125; NaN stays NaN.
+// the least relative error there (7.5e-8, found by exchange of its extrema; 2.1e-7 in 32 bits), times 2^n from n's bits.  From
+// -126.5 down (hidden pairs are -inf) exactly 0, since n = -127 gives an exponent field of 0; NaN stays NaN.
 __device__ __forceinline__ float2 fma_exp2(float2 x) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-125.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-125.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.f));
   const float2 t = __fadd2_rn(x, make_float2(12582912.f, 12582912.f));  // 1.5 * 2^23: n lands in the low mantissa bits
   const float2 n = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
   const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
@@ -410,8 +410,23 @@ __global__ void __launch_bounds__(kThreads, 1) weight_sums_kernel(const __grid_c
             if (masked) add(std::true_type()); else add(std::false_type());
           }
           const float2 s2 = __fadd2_rn(__fadd2_rn(acc[0], acc[1]), __fadd2_rn(acc[2], acc[3]));
+          float s1 = s2.x + s2.y;
+          if (__any_sync(0xffffffffu, s1 != s1)) {
+            // once more, pair by pair: a query that saw nothing adds nothing, even where its scores are not finite
+            s1 = 0.f;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              tmem_ld32(from + c * 32, x[0]);
+              tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) {
+                const float l = lse[c * 32 + k];
+                if (static_cast<uint32_t>(q0 + c * 32 + k - lo) < seen && l != -INFINITY) s1 += ex2f(__fmaf_rn(__uint_as_float(x[0][k]), p.scale_log2, l));
+              }
+            }
+          }
           // (compensated: `lost` is what the last addition rounded away)
-          const float y = s2.x + s2.y - lost, z = sum + y;
+          const float y = s1 - lost, z = sum + y;
           lost = (z - sum) - y;
           sum = z;
         }

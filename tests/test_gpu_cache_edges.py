@@ -124,3 +124,31 @@ def test_sums_of_keys_that_a_spoiled_query_does_not_see(dt, d):
     # the query NaN besides, as it comes out of a model
     q[5, 0], q[500, 2, 3] = math.nan, math.nan
     check_spoiled_sums(q, k, lse, window, sink, lens)
+
+
+@pytest.mark.parametrize("dt,d", [("bf16", 128), ("fp16", 64)])
+def test_queries_that_saw_nothing_add_nothing(dt, d):
+    """log-sum-exp -inf: nothing from that query, to the last bit and whatever its scores are (the attention's own answer
+    for a row that is not finite)."""
+    lens, window, sink = [700, 400], 500, 2
+    t = sum(lens)
+    q, k = normal(t, 4, d, seed=1, dt=dt), normal(t, 2, d, seed=2, dt=dt)
+    lse = 3 + normal(4, t, seed=3, dt="bf16").float()
+    lse[:, 300:] = -math.inf
+    got, want = check_spoiled_sums(q, k, lse, window, sink, lens)
+    assert (got[:, 300:] == 0).all() and (want[:, :300] > 0).all()
+    q[320, 1, 5], q[699, 3], q[1000, 0, 0] = math.nan, math.nan, math.nan
+    k[310, 0, 9] = math.nan   # (seen by queries that add nothing)
+    check_spoiled_sums(q, k, lse, window, sink, lens)
+
+
+def test_sums_behind_the_attention_of_a_prompt_with_a_query_that_is_not_finite():
+    import ring_swa.compiled  # noqa: F401  (registers the operator)
+    n, hq, hkv, d, window, sink = 500, 4, 2, 128, 90, 2
+    q, k, v = (normal(1, n, h, d, seed=i, dt="bf16").cuda() for i, h in enumerate((hq, hkv, hkv)))
+    q[0, 333, 2, 7] = math.nan
+    _, lse = torch.ops.ring_swa.swa_fwd(q, k, v, window, sink, d ** -0.5, None)
+    assert torch.isneginf(lse[0, 2, 333])
+    got = _ops().attn_weight_sums(q, k, lse, window, sink)
+    want, _, _ = R.weight_sums(q[0].cpu().double(), k[0].cpu().double(), lse[0].cpu(), window, sink, None, [n])
+    assert torch.isfinite(want).all() and ((got[0].cpu().double() - want).abs() <= 1e-4 * want).all()  # (16-bit weights in the forward's sum)
