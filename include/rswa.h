@@ -356,7 +356,8 @@ int rswa_cache_read(const rswa_cache_read_params_t* p, void* stream);
  * t < n_sink), with window < 0 every t <= p.  q [batch, q_len, Hq, head_dim] 16-bit, strides in elements (head
  * dimension contiguous, all multiples of 8, 16-byte aligned); out [batch, q_len, Hq, head_dim] contiguous; lse
  * [batch, Hq, q_len] float (natural log) or NULL.  A query before the sequence's start, or of an empty one, gives a
- * zero row and lse -inf.
+ * zero row and lse -inf.  Entries of blocks without a slot that any of the queries sees are not looked at: blocks behind the
+ * window may have been given back.
  * A scale of V that is not finite makes NaN of the outputs that see its block; lse and weights come from K alone.
  * NaN from a query or a scale of K stays with the rows that see it, and with the weights of the slots which these rows see.
  * weights (or NULL): float [batch, n_kv_heads, >= max_blocks * block_size], tokens contiguous; every slot seen has

@@ -61,6 +61,8 @@ constexpr float kSumScale = 1.f / 256;
 constexpr float kTinyV = -20.f;    // log2 of V's scale, below which the sum has exponentials of its own
 constexpr float kLeastV = 7.888609052210118e-31f;  // 2^-100, what V's scale counts as at least
 
+constexpr int kNoTile = -1, kBlank = -1024;  // rows of the cache: of a tile that is not there, and in front of the first one (loads give zeros)
+
 struct AttnKernelParams {
   CUtensorMap map[2];
   CacheView c;
@@ -91,7 +93,8 @@ struct AttnKernelParams {
 // The tiles of one sequence: the ones its sink tokens lie in, then the ones from its oldest visible token on.
 // An item of n tiles counts as n + kOver (kOver ones that are not there, then its tiles), one without any as none.
 struct SeqTiles {
-  int len, n_sink_tiles, first, n;
+  int len, n_sink_tiles, n;
+  int oldest;  // the first slot in the window of any query
 };
 template <int kOver>
 __device__ __forceinline__ SeqTiles seq_tiles(const AttnKernelParams& p, int b) {
@@ -102,15 +105,14 @@ __device__ __forceinline__ SeqTiles seq_tiles(const AttnKernelParams& p, int b) 
     raise_status(p.status, p.mirror, kErrSeqLen);
     len = 0;
   }
-  const int oldest = p.window < 0 ? 0 : max(0, max(0, len - p.q_len) - p.window);
+  s.oldest = p.window < 0 ? 0 : max(0, max(0, len - p.q_len) - p.window);
   s.len = len;
-  s.first = oldest / kTok;
-  s.n_sink_tiles = min((min(p.n_sink, len) + kTok - 1) / kTok, s.first);
-  const int n = s.n_sink_tiles + (len + kTok - 1) / kTok - s.first;
+  s.n_sink_tiles = min((min(p.n_sink, len) + kTok - 1) / kTok, s.oldest / kTok);
+  const int n = s.n_sink_tiles + (len + kTok - 1) / kTok - s.oldest / kTok;
   s.n = n > 0 ? n + kOver : 0;
   return s;
 }
-__device__ __forceinline__ int tile_slot(const SeqTiles& s, int i) { return (i < s.n_sink_tiles ? i : s.first + i - s.n_sink_tiles) * kTok; }
+__device__ __forceinline__ int tile_slot(const SeqTiles& s, int i) { return (i < s.n_sink_tiles ? i : s.oldest / kTok + i - s.n_sink_tiles) * kTok; }
 
 // Where the work of a group begins and ends: equal shares of all tiles.  Not more of them than there is a tile per warp for,
 // but one for each item at least: a group that takes short items one after the other pays for each of them.
@@ -387,7 +389,7 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
   const int box = min(p.c.bs, kTok);
 
   // The tiles of this warp, counted: tile i is the share's tile wg + i * kGroup.  Looks 32 of them up, one a lane.
-  // (The warp is told of a tile that is not there by a row of -1.)
+  // (The warp is told of a tile that is not there by a row of kNoTile.)
   const int n_own = (end - begin - wg + kGroup - 1) / kGroup;
   int page[2], tokens;  // of this lane's tile
   auto look_up = [&](int i) {
@@ -396,17 +398,25 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
     __syncwarp();
     if (at < end) {
       const auto lc = cursor_at<kOver>(p, ctl.prefix, at);
-      int2 row = make_int2(-1, -1);
+      int2 row = make_int2(kNoTile, kNoTile);
       if (lc.i >= kOver) {
         const int bs = p.c.bs, slot = tile_slot(lc.s, lc.i - kOver), h = lc.item / p.row_tiles, j = slot / bs;
-        // a tile is part of one block, or two blocks of 16; the second may lie behind the sequence's end: not looked at
+        // a tile is part of one block, or two blocks of 16, of which one may have no slot that anybody sees (behind the sinks, in
+        // front of the window, behind the end): that one is not looked at, and loads zeros
         // (an entry that is no block has been reported; any block will do then)
-        page[0] = max(0, table_entry(p.table, p.table_stride, lc.b, j, p.c.num_blocks, p.status, p.mirror)) * p.c.hkv + h;
-        page[1] = page[0];
-        if (bs < kTok && slot + bs < lc.s.len)
-          page[1] = max(0, table_entry(p.table, p.table_stride, lc.b, j + 1, p.c.num_blocks, p.status, p.mirror)) * p.c.hkv + h;
+        const int* const entry = p.table + lc.b * p.table_stride + j;
+        const int e0 = entry[0], e1 = entry[bs < kTok && slot + bs < lc.s.len];  // (one latency; what is not looked at may be anything)
+        const auto block = [&](int e) {
+          if (e >= 0 && e < p.c.num_blocks) return e * p.c.hkv + h;
+          raise_status(p.status, p.mirror, kErrBlockTable);
+          return h;
+        };
+        const auto seen = [&](int from) { return from < lc.s.len && (from < p.n_sink || from + 16 > lc.s.oldest); };
+        if (bs >= kTok || seen(slot)) page[0] = block(e0);
+        if (bs >= kTok) page[1] = page[0];
+        else if (seen(slot + 16)) page[1] = block(e1);
         tokens = lc.s.len - slot;
-        row = make_int2(page[0] * bs + slot % bs, page[1] * bs + slot % bs);
+        row = make_int2(page[0] < 0 ? kBlank : page[0] * bs + slot % bs, page[1] < 0 ? kBlank : page[1] * bs + slot % bs);
       }
       ctl.row[warp][lane] = row;
     }
@@ -416,7 +426,7 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
   auto fetch_scales = [&]() {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const bool some = 16 * t < tokens;  // (tokens behind the end: their block may not even have a scale)
+      const bool some = 16 * t < tokens && page[t] >= 0;  // (tokens behind the end: their block may not even have a scale)
       scale[0][t] = some ? p.c.scale[0][page[t]] : 1.f;
       scale[1][t] = some ? p.c.scale[1][page[t]] : 1.f;
     }
@@ -450,7 +460,7 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
         fetch_scales();
         put_scales();
       }
-      if (ctl.row[warp][i & 31].x >= 0) break;
+      if (ctl.row[warp][i & 31].x != kNoTile) break;
       ++i;
     }
     return i;
@@ -487,7 +497,7 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
   if (n_own > 0) {
     look_up(0);
     fetch_scales();
-    while (own_i < min(n_own, 32) && ctl.row[warp][own_i].x < 0) ++own_i;
+    while (own_i < min(n_own, 32) && ctl.row[warp][own_i].x == kNoTile) ++own_i;
     if (own_i < min(n_own, 32)) {
       load(own_i, 0);
       load(own_i, 1);

@@ -125,7 +125,8 @@ def cache_attn(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, lens:
     it sees slot t <= p if p - t <= window_size or t < num_sink_tokens, with window_size None every t <= p.  The mask is that
     of ring_sliding_window_attn and ring_streaming_llm_attn.  Returns out like q, and with return_lse also the log-sum-exp
     [batch, num_q_heads, queries] float32; a query that sees nothing (an empty sequence, or one shorter than
-    `queries`) gives zeros and -inf.  At most 8192 queries and heads of one key/value head together.
+    `queries`) gives zeros and -inf.  At most 8192 queries and heads of one key/value head together.  Blocks none of whose slots
+    any query sees may have been given back: their entries of block_table are not looked at.
 
     weights: float32 [batch, num_kv_heads, at least max_blocks * block_size], added to in place: the softmax weights that
     every slot got from the queries and heads of its key/value head (what cache_evict goes by; start it with

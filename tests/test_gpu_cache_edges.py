@@ -152,3 +152,34 @@ def test_sums_behind_the_attention_of_a_prompt_with_a_query_that_is_not_finite()
     got = _ops().attn_weight_sums(q, k, lse, window, sink)
     want, _, _ = R.weight_sums(q[0].cpu().double(), k[0].cpu().double(), lse[0].cpu(), window, sink, None, [n])
     assert torch.isfinite(want).all() and ((got[0].cpu().double() - want).abs() <= 1e-4 * want).all()  # (16-bit weights in the forward's sum)
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("bs", [16, 32, 64])
+def test_blocks_behind_the_window_may_be_given_back(bs, kind):
+    """Entries of blocks without a slot that any query sees are not looked at, for every block size: the same bits, nothing reported."""
+    from ring_swa import _kernels as K
+    ops = _ops()
+    lens, d = [1000, 333, 70, 5], 64
+    cache, table, _, _, _ = filled(kind, "bf16", lens, 2, bs, d, seed=2)
+    n = torch.tensor(lens, dtype=torch.int32).cuda()
+    for window, sink, queries in ((200, 0, 1), (111, 1, 1), (250, 17, 4), (0, 0, 1), (40, 33, 2)):
+        freed = table.clone()
+        for i, m in enumerate(lens):
+            for j in range((m + bs - 1) // bs):
+                if j * bs >= sink and (j + 1) * bs <= max(0, m - queries) - window:
+                    freed[i, j] = -1
+        assert (freed != table).any()
+        q = normal(4, queries, 8, d, seed=3, dt="bf16").cuda()
+        ws = [torch.zeros(4, 2, table.shape[1] * bs, device="cuda") for _ in range(2)]
+        a, b = (ops.cache_attn(q, cache, t.cuda(), n, window_size=window, num_sink_tokens=sink, weights=w, return_lse=True)
+                for t, w in ((table, ws[0]), (freed, ws[1])))
+        K.check_device_status()
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and torch.equal(*ws)
+        assert torch.isfinite(a[0]).all()
+        # an entry that is seen is still looked at
+        bad = freed.clone()
+        bad[0, (lens[0] - 1) // bs] = -1
+        ops.cache_attn(q, cache, bad.cuda(), n, window_size=window, num_sink_tokens=sink)
+        with pytest.raises(RuntimeError, match="code 110"):
+            K.check_device_status()
