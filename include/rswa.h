@@ -291,9 +291,10 @@ float rswa_event_elapsed_ms(void* start, void* stop);
  *
  * Sequence b's tokens lie, in order, in the blocks named by row b of a block table (int32, device memory; rows
  * table_stride entries apart, max_blocks of them each); its slot t is token t % block_size of the row's entry
- * t / block_size.  Entries behind the last one that a length reaches are not looked at.  An entry that is looked
- * at and is no block of the cache, and a length that is negative or beyond the table, raise the status word: the call
- * then reads and writes nothing out of bounds, and what it returns for that sequence means nothing.
+ * t / block_size.  Rows may be the same memory (stride 0) where their blocks are only read.  Entries behind the last one that
+ * a length reaches are not looked at.  An entry that is looked at and is no block of the cache, and a length that is negative
+ * or beyond the table, raise the status word: the call then reads and writes nothing out of bounds, and what it returns for
+ * that sequence means nothing.
  */
 #define RSWA_CACHE_INT8 0
 #define RSWA_CACHE_E4M3 1

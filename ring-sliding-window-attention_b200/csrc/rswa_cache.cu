@@ -297,13 +297,13 @@ CacheView cache_view(const rswa_cache_t& c) {
   return v;
 }
 
-int check_table(const rswa_block_table_t& t, const int32_t* lens, const int32_t* status, int block_size, const char* what) {
+int check_table(const rswa_block_table_t& t, bool written, const int32_t* lens, const int32_t* status, int block_size, const char* what) {
   if (t.batch < 0 || t.max_blocks < 0 || (t.batch > 0 && ((t.entries == nullptr && t.max_blocks > 0) || lens == nullptr)) || status == nullptr) {
     set_error("%s: block table, lens and status are required", what);
     return RSWA_E_ARG;
   }
-  if (t.stride < t.max_blocks && t.batch > 1) {
-    set_error("%s: rows of the block table overlap", what);
+  if (written ? t.stride < t.max_blocks && t.batch > 1 : t.stride < 0) {
+    set_error("%s: rows of a block table of blocks to write to overlap", what);
     return RSWA_E_ARG;
   }
   if (static_cast<long long>(t.max_blocks) * block_size > 0x7fffff00LL) {
@@ -324,7 +324,7 @@ extern "C" int rswa_cache_append(const rswa_cache_append_params_t* p, void* stre
     return RSWA_E_ARG;
   }
   int rc = check_cache(p->cache, what);
-  if (rc == RSWA_OK) rc = check_table(p->table, p->lens, p->status, p->cache.block_size, what);
+  if (rc == RSWA_OK) rc = check_table(p->table, true, p->lens, p->status, p->cache.block_size, what);
   if (rc != RSWA_OK) return rc;
   if (p->dtype != RSWA_DTYPE_BF16 && p->dtype != RSWA_DTYPE_FP16) {
     set_error("%s: dtype must be bf16 (0) or fp16 (1), got %d", what, p->dtype);
@@ -381,7 +381,7 @@ extern "C" int rswa_cache_read(const rswa_cache_read_params_t* p, void* stream) 
     return RSWA_E_ARG;
   }
   int rc = check_cache(p->cache, what);
-  if (rc == RSWA_OK) rc = check_table(p->table, p->lens, p->status, p->cache.block_size, what);
+  if (rc == RSWA_OK) rc = check_table(p->table, false, p->lens, p->status, p->cache.block_size, what);
   if (rc != RSWA_OK) return rc;
   if (p->dtype != RSWA_DTYPE_BF16 && p->dtype != RSWA_DTYPE_FP16) {
     set_error("%s: dtype must be bf16 (0) or fp16 (1), got %d", what, p->dtype);

@@ -45,7 +45,7 @@
 namespace rswa {
 
 int make_rows_map(CUtensorMap* map, const void* base, long long rows, int row_bytes, int box_rows);
-int check_table(const rswa_block_table_t& t, const int32_t* lens, const int32_t* status, int block_size, const char* what);
+int check_table(const rswa_block_table_t& t, bool written, const int32_t* lens, const int32_t* status, int block_size, const char* what);
 
 using namespace tc05;
 
@@ -986,7 +986,7 @@ extern "C" int rswa_cache_attn(const rswa_cache_attn_params_t* p, void* stream) 
   const char* what = "rswa_cache_attn";
   int rc = check_attn(p);
   if (rc == RSWA_OK) rc = check_cache(p->cache, what);
-  if (rc == RSWA_OK) rc = check_table(p->table, p->lens, p->status, p->cache.block_size, what);
+  if (rc == RSWA_OK) rc = check_table(p->table, false, p->lens, p->status, p->cache.block_size, what);
   if (rc != RSWA_OK) return rc;
   if (p->dtype != RSWA_DTYPE_BF16 && p->dtype != RSWA_DTYPE_FP16) {
     set_error("%s: dtype must be bf16 (0) or fp16 (1), got %d", what, p->dtype);

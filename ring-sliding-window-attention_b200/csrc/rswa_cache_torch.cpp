@@ -101,7 +101,7 @@ void check_table(const at::Tensor& table, const at::Tensor& lens, int64_t block_
 rswa_block_table_t table_struct(const at::Tensor& table) {
   rswa_block_table_t t;
   t.entries = table.const_data_ptr<int32_t>();
-  // (rows of a table that is one row of another one, repeated, may lie on each other: it is only read)
+  // (a row expanded over the batch is passed as it is; the library refuses it where blocks are written to)
   t.stride = table.size(0) > 1 ? table.stride(0) : table.size(1);
   t.batch = static_cast<int32_t>(table.size(0)), t.max_blocks = static_cast<int32_t>(table.size(1));
   return t;

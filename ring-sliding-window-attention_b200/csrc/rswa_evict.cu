@@ -6,7 +6,7 @@
 
 namespace rswa {
 
-int check_table(const rswa_block_table_t& t, const int32_t* lens, const int32_t* status, int block_size, const char* what);
+int check_table(const rswa_block_table_t& t, bool written, const int32_t* lens, const int32_t* status, int block_size, const char* what);
 
 namespace {
 
@@ -428,8 +428,8 @@ extern "C" int rswa_cache_evict(const rswa_cache_evict_params_t* p, void* stream
     return RSWA_E_ARG;
   }
   int rc = check_cache(p->cache, what);
-  if (rc == RSWA_OK) rc = check_table(p->table, p->lens, p->status, p->cache.block_size, what);
-  if (rc == RSWA_OK) rc = check_table(p->new_table, p->lens, p->status, p->cache.block_size, what);
+  if (rc == RSWA_OK) rc = check_table(p->table, false, p->lens, p->status, p->cache.block_size, what);
+  if (rc == RSWA_OK) rc = check_table(p->new_table, true, p->lens, p->status, p->cache.block_size, what);
   if (rc != RSWA_OK) return rc;
   if (p->budget <= 0 || p->n_sink < 0 || p->n_recent < 0 || static_cast<int64_t>(p->n_sink) + p->n_recent > p->budget) {
     set_error("%s: budget must be positive and hold the sink tokens and the newest ones (budget %d, %d and %d)", what, p->budget, p->n_sink, p->n_recent);

@@ -19,7 +19,8 @@ and, for a cache that is kept to a number of tokens by what the model has attend
     lens, weights, kept = cache_evict(cache, block_table, lens, weights, budget, new_block_table, 4, 512)
 
 block_table [batch, max_blocks] and lens [batch] are int32 tensors of the caller's on the cache's device: slot t of
-sequence b is token t % block_size of block block_table[b, t // block_size].  Nothing here changes lens, copies it to the
+sequence b is token t % block_size of block block_table[b, t // block_size]; a row may be expanded over the batch where its
+blocks are only read.  Nothing here changes lens, copies it to the
 host or waits for the device, so that a step can be captured into a CUDA graph and replayed with other lengths.  Positions
 are slots: after an eviction the tokens that stayed count as neighbours.
 

@@ -183,3 +183,30 @@ def test_blocks_behind_the_window_may_be_given_back(bs, kind):
         ops.cache_attn(q, cache, bad.cuda(), n, window_size=window, num_sink_tokens=sink)
         with pytest.raises(RuntimeError, match="code 110"):
             K.check_device_status()
+
+
+def test_a_block_table_whose_rows_are_one():
+    """Sequences that share all their blocks (one prompt, several questions): a row expanded over the batch, where it is only read."""
+    ops = _ops()
+    lens, bs, d, batch = [300], 16, 64, 5
+    cache, table, _, _, _ = filled("int8", "bf16", lens, 2, bs, d, seed=2, spare=100)
+    one, n = table.cuda(), torch.tensor([300, 17, 299, 0, 160], dtype=torch.int32).cuda()
+    many, apart = one.expand(batch, -1), one.repeat(batch, 1)
+    q = normal(batch, 2, 4, d, seed=3, dt="bf16").cuda()
+    assert torch.equal(ops.cache_attn(q, cache, many, n), ops.cache_attn(q, cache, apart, n))
+    for x, y in zip(ops.cache_read(cache, many, n, 300), ops.cache_read(cache, apart, n, 300)):
+        assert torch.equal(x, y)
+    free = sorted(set(range(cache.k.shape[0])) - set(table.flatten().tolist()))
+    new = torch.tensor(free[:5 * batch], dtype=torch.int32).view(batch, 5).cuda()
+    w = torch.rand(batch, 2, table.shape[1] * bs, generator=torch.Generator().manual_seed(0)).cuda()
+    a = [x.clone() for x in ops.cache_evict(cache, many, n, w, 80, new, 1, 3)]
+    kept = [x.clone() for x in ops.cache_read(cache, new, a[0], 80)]
+    b = ops.cache_evict(cache, apart, n, w, 80, new, 1, 3)
+    for x, y in zip([*a, *kept], [*b, *ops.cache_read(cache, new, b[0], 80)]):
+        assert torch.equal(x, y)
+    # where blocks are written to, rows have to be their own
+    k = normal(batch, 1, 2, d, seed=4, dt="bf16").cuda()
+    with pytest.raises(ValueError, match="overlap"):
+        ops.cache_append(cache, k, k, many, n)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.cache_evict(cache, many, n, w, 80, new[:1].expand(batch, -1), 1, 3)
