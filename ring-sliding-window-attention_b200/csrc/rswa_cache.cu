@@ -130,7 +130,8 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const __grid_con
   most = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
   const float amax = bf16 ? __uint_as_float(most << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(most)));
   const float need = scale_for<kInt8>(amax);
-  const bool grows = first == 0 || need > before || need != need;
+  // (a scale from elsewhere need not be a power of two: what counts is whether the values fit, at a scale with a finite reciprocal)
+  const bool grows = first == 0 || amax > (kInt8 ? 127.f : 448.f) * before || before < kLeastScale || need != need;
   const float after = grows ? need : before;
   const bool poisoned = after != after;
   const float inv = 1.f / after;

@@ -24,6 +24,8 @@ enum : int {
   kErrSeqLen = 111,      // a length or an offset that is negative, or beyond what the table, the tokens given or the weights hold
 };
 
+constexpr float kLeastScale = 7.888609052210118e-31f;  // 2^-100, of those that are written here
+
 struct CacheView {
   uint8_t* data[2];   // k, v
   float* scale[2];

@@ -59,7 +59,6 @@ constexpr float kLow = 4.f;    // and is raised to the maximum minus 4, so that 
 constexpr float kSumUnit = 8.f;    // sums of weights are in units of 2^8: 2^21 tokens of weight 2^14 under V's least scale, 2^-100, stay finite
 constexpr float kSumScale = 1.f / 256;
 constexpr float kTinyV = -20.f;    // log2 of V's scale, below which the sum has exponentials of its own
-constexpr float kLeastV = 7.888609052210118e-31f;  // 2^-100, what V's scale counts as at least
 
 constexpr int kNoTile = -1, kBlank = -1024;  // rows of the cache: of a tile that is not there, and in front of the first one (loads give zeros)
 
@@ -431,13 +430,13 @@ __global__ void __launch_bounds__((Layout<kD, kNT, kAll>::kThreads), 1) cache_at
       scale[1][t] = some ? p.c.scale[1][page[t]] : 1.f;
     }
   };
-  auto put_scales = [&]() {
+  auto put_scales = [&]() {  // (V's counts as kLeastScale at least)
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       // (V's scale is not finite: 1 for the sum of the weights, which depends on K alone.  Such scales and tiny ones have a
       // negative reciprocal, with a logarithm of 0 or a negative one)
       const bool spoiled = !(fabsf(scale[1][t]) <= 3.4028235e38f);
-      const float sv = spoiled ? 1.f : fmaxf(scale[1][t], kLeastV), lg = __log2f(sv), inv = 1.f / sv * kSumScale;
+      const float sv = spoiled ? 1.f : fmaxf(scale[1][t], kLeastScale), lg = __log2f(sv), inv = 1.f / sv * kSumScale;
       ctl.scale[warp][lane][t] = make_float4(scale[0][t], lg, spoiled || lg < kTinyV ? -inv : inv, 0.f);
     }
     __syncwarp();

@@ -210,3 +210,44 @@ def test_a_block_table_whose_rows_are_one():
         ops.cache_append(cache, k, k, many, n)
     with pytest.raises(ValueError, match="overlap"):
         ops.cache_evict(cache, many, n, w, 80, new[:1].expand(batch, -1), 1, 3)
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_a_scale_from_elsewhere_is_kept_while_the_new_tokens_fit(kind):
+    """Blocks filled elsewhere, whose scales are no powers of two: a new token that they hold leaves scale and older tokens as
+    they are; one that they do not hold moves the block to the least power of two, rounded once.  (Bytes: within half a step, and
+    2^-22 for the reciprocal's and the product's roundings.)"""
+    ops = _ops()
+    top = R.TOP[kind]
+    heads, bs, d, used = 2, 32, 64, 20
+    sizes = torch.tensor([0.75, 0.9, 1.37e-3, 3.1, 2.0 ** -130, 2.0 ** -100])
+    blocks = len(sizes)
+    cache = make(kind, blocks, heads, bs, d, seed=1)
+    g = torch.Generator().manual_seed(2)
+    stored = torch.randint(-100, 101, (2, blocks, heads, bs, d), generator=g).float()
+    for x, s, y in ((cache.k, cache.k_scale, stored[0]), (cache.v, cache.v_scale, stored[1])):
+        x.copy_(y.to(R.TORCH[kind]))
+        s.copy_(sizes[:, None])
+    before = host(cache)
+    table = torch.arange(blocks, dtype=torch.int32)[:, None].cuda()
+    n = torch.full((blocks,), used, dtype=torch.int32).cuda()
+    new = torch.rand(2, blocks, heads, d, generator=g) * 2 - 1
+    new[..., 0] = 1
+    # k: 0.98 of what the scale holds; v: 1.3 times as much
+    k, v = ((x * m * top * sizes[:, None, None]).bfloat16() for x, m in zip(new, (0.98, 1.3)))
+    ops.cache_append(cache, k[:, None].cuda(), v[:, None].cuda(), table, n)
+    got = host(cache)
+    for name, x in (("k", k), ("v", v)):
+        for b in range(blocks):
+            least = R.scale_for(x[b].double().abs().max().item(), kind)
+            old = sizes[b].item()
+            fits = name == "k" and old >= 2.0 ** -100
+            want = old if fits else least
+            assert (got[name + "_scale"][b] == want).all(), (name, old, got[name + "_scale"][b])
+            held = got[name][b]
+            rows = torch.cat([before[name][b][:, :used] * old / want, x[b].double()[:, None] / want], 1)
+            if fits:
+                assert torch.equal(held[:, :used], before[name][b][:, :used])
+            step = torch.ones_like(rows) if kind == "int8" else torch.exp2((torch.frexp(rows.abs().clamp_min(2.0 ** -6)).exponent - 4).double())
+            assert ((held[:, :used + 1] - rows).abs() <= 0.5 * step + 2.0 ** -22 * rows.abs()).all()
+            assert torch.equal(held[:, used + 1:], before[name][b][:, used + 1:])
