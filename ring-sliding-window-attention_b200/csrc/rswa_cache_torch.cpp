@@ -129,12 +129,17 @@ void written(const at::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
-// The zeroed counters of rswa_cache_attn.  Calls on one stream follow one another and share them; a call that is being
-// captured gets its own from the graph's memory, zeroed by the graph each time, since the graph may run beside anything.
+// The zeroed counters of rswa_cache_attn.  Calls on one of torch's streams follow one another and share them, for as long as the
+// process lives.  Calls that are being captured (the graph may run beside anything), and those on streams that torch did not make,
+// get their own, zeroed on the stream each time: a handle from elsewhere may be another stream for every thread, or be given to
+// another stream while work of the one that had it still runs.  (torch identifies its own streams by numbers, those by the handle.)
 at::Tensor counters(int dev, const at::TensorOptions& options) {
-  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev).stream();
+  const c10::cuda::CUDAStream current = c10::cuda::getCurrentCUDAStream(dev);
+  const cudaStream_t stream = current.stream();
+  const bool foreign = stream != nullptr && current.id() == static_cast<c10::StreamId>(reinterpret_cast<intptr_t>(stream));
   cudaStreamCaptureStatus st;
-  if (cudaStreamIsCapturing(stream, &st) != cudaSuccess || st != cudaStreamCaptureStatusNone) return at::zeros({RSWA_CACHE_ATTN_COUNTERS}, options.dtype(at::kInt));
+  if (foreign || cudaStreamIsCapturing(stream, &st) != cudaSuccess || st != cudaStreamCaptureStatusNone)
+    return at::zeros({RSWA_CACHE_ATTN_COUNTERS}, options.dtype(at::kInt));
   static std::mutex mutex;
   static auto* kept = new std::map<std::pair<int, cudaStream_t>, at::Tensor>();  // (never freed: the process may end before its streams do)
   const std::lock_guard<std::mutex> lock(mutex);

@@ -251,3 +251,33 @@ def test_a_scale_from_elsewhere_is_kept_while_the_new_tokens_fit(kind):
             step = torch.ones_like(rows) if kind == "int8" else torch.exp2((torch.frexp(rows.abs().clamp_min(2.0 ** -6)).exponent - 4).double())
             assert ((held[:, :used + 1] - rows).abs() <= 0.5 * step + 2.0 ** -22 * rows.abs()).all()
             assert torch.equal(held[:, used + 1:], before[name][b][:, used + 1:])
+
+
+def test_streams_from_elsewhere_leave_nothing_behind():
+    """A stream that another library made may be destroyed, and its handle given to another stream, while its work still runs:
+    nothing that two calls must not share is kept under the handle."""
+    import gc
+    from cuda.bindings import runtime as rt
+    ops = _ops()
+    lens, bs, d = [9000], 64, 128
+    cache, table, _, _, _ = filled("int8", "bf16", lens, 2, bs, d, seed=1)
+    args = (normal(1, 1, 8, d, seed=2, dt="bf16").cuda(), cache, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
+    want = ops.cache_attn(*args)
+    torch.cuda.synchronize()
+    gc.collect()
+    held = torch.cuda.memory_allocated()
+    handles = []
+    for _ in range(4):  # four that live at once: handles that no earlier call has seen
+        err, s = rt.cudaStreamCreateWithFlags(rt.cudaStreamNonBlocking)
+        assert int(err) == 0
+        handles.append(s)
+    for s in handles:
+        with torch.cuda.stream(torch.cuda.ExternalStream(int(s))):
+            outs = [ops.cache_attn(*args) for _ in range(3)]
+        rt.cudaStreamSynchronize(s)
+        assert all(torch.equal(x, want) for x in outs)
+        del outs
+    gc.collect()
+    assert torch.cuda.memory_allocated() == held
+    for s in handles:
+        rt.cudaStreamDestroy(s)
