@@ -44,12 +44,14 @@ def _call(name: str, device: torch.device, *args):
     if _native is None:
         _native = K.native_module()
     fn = getattr(_native, name)
-    result = fn(*args)
-    if result is False:  # no status word yet, or an error of an earlier call to raise
+    for _ in range(8):  # (more than twice where other threads' calls are reported meanwhile)
+        result = fn(*args)
+        if result is not False:
+            return result
+        # no status word yet, or an error of an earlier call to raise
         K.status_word(device)
         K.raise_if_reported(device)
-        result = fn(*args)
-    return result
+    raise RuntimeError(f"ring_swa.ops.{name}: errors of earlier calls on {device} are being reported; this call did nothing")
 
 
 def _call_cache(name: str, cache: "KVCache", *args):

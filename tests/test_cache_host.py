@@ -1,0 +1,50 @@
+"""Host side of the operators on the 8-bit key/value cache that needs no GPU."""
+import pytest
+import torch
+
+from ring_swa import _kernels as K
+from ring_swa import ops
+from ring_swa.ops import kv_cache
+
+
+def test_a_call_that_finds_another_reported_error_is_made_again(monkeypatch):
+    """False stands for a call that did nothing, and never reaches the caller: not where another call's error is reported between
+    the look at the first one and the second attempt either."""
+    cache = ops.KVCache.empty(4, 2, block_size=16, head_dim=64, device="cpu")
+    table, lens = torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    answers, looks = [False, False, "done"], []
+
+    class Native:
+        @staticmethod
+        def cache_read(*args):
+            return answers.pop(0)
+
+    monkeypatch.setattr(kv_cache, "_native", Native)
+    monkeypatch.setattr(K, "status_word", lambda device: looks.append("word"))
+    monkeypatch.setattr(K, "raise_if_reported", lambda device: looks.append("look"))
+    assert ops.cache_read(cache, table, lens, 1) == "done"
+    assert looks == ["word", "look"] * 2 and not answers
+
+    def report(device):
+        raise RuntimeError("code 110")
+
+    answers.append(False)
+    monkeypatch.setattr(K, "raise_if_reported", report)
+    with pytest.raises(RuntimeError, match="110"):
+        ops.cache_read(cache, table, lens, 1)
+
+
+def test_a_call_that_can_never_be_made_raises(monkeypatch):
+    cache = ops.KVCache.empty(4, 2, block_size=16, head_dim=64, device="cpu")
+
+    class Native:
+        @staticmethod
+        def cache_append(*args):
+            return False
+
+    monkeypatch.setattr(kv_cache, "_native", Native)
+    monkeypatch.setattr(K, "status_word", lambda device: None)
+    monkeypatch.setattr(K, "raise_if_reported", lambda device: None)
+    kv = torch.zeros(3, 1, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="did nothing"):
+        ops.cache_append(cache, kv, kv, torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32))
