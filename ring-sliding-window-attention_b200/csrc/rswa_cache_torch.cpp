@@ -152,9 +152,13 @@ at::Tensor counters(int dev, const at::TensorOptions& options) {
 void check_weights(const at::Tensor& w, int64_t batch, int64_t heads, int64_t tokens, const char* what, const char* name) {
   TORCH_CHECK_VALUE(w.scalar_type() == at::kFloat && w.dim() == 3 && w.size(0) == batch && w.size(1) == heads && w.size(2) >= tokens, what, ": ", name,
                     " must be float32 [batch, num_kv_heads, at least max_blocks * block_size = ", tokens, "], got ", w.sizes());
-  TORCH_CHECK_VALUE((w.size(2) <= 1 || w.stride(2) == 1) && (w.size(1) <= 1 || w.stride(1) >= w.size(2)) &&
-                        (w.size(0) <= 1 || w.stride(0) >= (w.size(1) - 1) * w.stride(1) + w.size(2)),
-                    what, ": ", name, " must be contiguous along the tokens, without rows that overlap");
+  // rows apart in either order of sequences and heads
+  const auto apart = [&](int inner, int outer) {
+    return (w.size(inner) <= 1 || w.stride(inner) >= w.size(2)) &&
+           (w.size(outer) <= 1 || w.stride(outer) >= (w.size(inner) - 1) * (w.size(inner) <= 1 ? 0 : w.stride(inner)) + w.size(2));
+  };
+  TORCH_CHECK_VALUE((w.size(2) <= 1 || w.stride(2) == 1) && (apart(1, 0) || apart(0, 1)), what, ": ", name,
+                    " must be contiguous along the tokens, without rows that overlap");
 }
 
 }  // namespace

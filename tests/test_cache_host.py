@@ -48,3 +48,18 @@ def test_a_call_that_can_never_be_made_raises(monkeypatch):
     kv = torch.zeros(3, 1, 2, 64, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="did nothing"):
         ops.cache_append(cache, kv, kv, torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32))
+
+
+def test_weights_in_either_order_of_sequences_and_heads():
+    """[heads, batch, slots] transposed has no rows that overlap; it comes as far as the look at the device."""
+    cache = ops.KVCache.empty(4, 2, block_size=16, head_dim=64, device="cpu")
+    q, table, lens = torch.zeros(3, 1, 4, 64, dtype=torch.bfloat16), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    for w in (torch.zeros(2, 3, 32).transpose(0, 1), torch.zeros(2, 3, 40)[..., 3:35].transpose(0, 1), torch.zeros(3, 4, 32)[:, ::2]):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            ops.cache_attn(q, cache, table, lens, weights=w)
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            ops.cache_evict(cache, table, lens, w, 16, table)
+    for w in (torch.zeros(2, 1, 32).expand(2, 3, 32).transpose(0, 1), torch.zeros(1, 3, 32).expand(2, 3, 32).transpose(0, 1),
+              torch.zeros(200).as_strided((3, 2, 32), (16, 32, 1)), torch.zeros(200).as_strided((3, 2, 32), (32, 32, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.cache_attn(q, cache, table, lens, weights=w)

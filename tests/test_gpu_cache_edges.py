@@ -281,3 +281,19 @@ def test_streams_from_elsewhere_leave_nothing_behind():
     assert torch.cuda.memory_allocated() == held
     for s in handles:
         rt.cudaStreamDestroy(s)
+
+
+def test_weights_laid_out_by_heads():
+    ops = _ops()
+    lens, bs, d = [300, 40, 77], 32, 64
+    cache, table, _, _, _ = filled("int8", "bf16", lens, 2, bs, d, seed=2, spare=20)
+    n, q = torch.tensor(lens, dtype=torch.int32).cuda(), normal(3, 2, 4, d, seed=3, dt="bf16").cuda()
+    a = torch.rand(3, 2, table.shape[1] * bs, generator=torch.Generator().manual_seed(0)).cuda()
+    b = torch.zeros(2, 3, a.shape[2] + 3, device="cuda")[..., :a.shape[2]].transpose(0, 1).copy_(a)
+    for w in (a, b):
+        ops.cache_attn(q, cache, table.cuda(), n, weights=w)
+    assert torch.equal(a, b) and not b.is_contiguous()
+    free = sorted(set(range(cache.k.shape[0])) - set(table.flatten().tolist()))
+    new = torch.tensor(free[:6], dtype=torch.int32).view(3, 2).cuda()
+    for x, y in zip(*([z.clone() for z in ops.cache_evict(cache, table.cuda(), n, w, 50, new, 1, 3)] for w in (a, b))):
+        assert torch.equal(x, y)
