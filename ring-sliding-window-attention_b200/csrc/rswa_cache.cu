@@ -307,7 +307,7 @@ int check_table(const rswa_block_table_t& t, bool written, const int32_t* lens, 
     set_error("%s: rows of a block table of blocks to write to overlap", what);
     return RSWA_E_ARG;
   }
-  if (static_cast<long long>(t.max_blocks) * block_size > 0x7fffff00LL) {
+  if (static_cast<long long>(t.max_blocks) * block_size > 0x7ff00000LL) {
     set_error("%s: positions overflow int32", what);
     return RSWA_E_UNSUPPORTED;
   }

@@ -63,3 +63,25 @@ def test_weights_in_either_order_of_sequences_and_heads():
               torch.zeros(200).as_strided((3, 2, 32), (16, 32, 1)), torch.zeros(200).as_strided((3, 2, 32), (32, 32, 1))):
         with pytest.raises(ValueError, match="overlap"):
             ops.cache_attn(q, cache, table, lens, weights=w)
+
+
+def test_tables_whose_slots_come_close_to_32_bits_are_refused():
+    """The kernels step up to 2^14 slots beyond a sequence's end before they compare."""
+    from ring_swa import _C
+    lib, call = _C.lib(), {"append": _C.CacheAppendParams, "read": _C.CacheReadParams, "attn": _C.CacheAttnParams, "evict": _C.CacheEvictParams}
+    for name, params in call.items():
+        for blocks, refused in (((1 << 24) - 4, True), ((1 << 24) - (1 << 13), False)):
+            p = params()
+            c = p.cache
+            c.k = c.v = c.k_scale = c.v_scale = 4096  # (looked at no further: the call ends with the checks)
+            c.num_blocks, c.n_kv_heads, c.block_size, c.head_dim = 1, 1, 128, 64
+            p.lens = p.status = p.table.entries = 4096
+            p.table.batch, p.table.max_blocks, p.table.stride = 1, blocks, blocks
+            p.n_q_heads = 1
+            if name == "evict":
+                p.new_table = p.table
+                p.budget = -1  # the refusal behind it
+            else:
+                p.dtype = 7
+            assert getattr(lib, "rswa_cache_" + name)(p, None) < 0
+            assert (b"overflow" in lib.rswa_last_error()) == refused, (name, blocks, lib.rswa_last_error())
