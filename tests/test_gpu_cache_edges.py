@@ -297,3 +297,43 @@ def test_weights_laid_out_by_heads():
     new = torch.tensor(free[:6], dtype=torch.int32).view(3, 2).cuda()
     for x, y in zip(*([z.clone() for z in ops.cache_evict(cache, table.cuda(), n, w, 50, new, 1, 3)] for w in (a, b))):
         assert torch.equal(x, y)
+
+
+def test_sums_of_one_key_head_for_all_and_of_a_prompt_without_a_window():
+    """A key expanded over the heads' dimension, as a slice of a batch; against the 64-bit sums of the same."""
+    b, s, hq, d = 2, 2500, 4, 64
+    fused = normal(b, s, hq + 1, d, seed=1, dt="bf16")
+    q, k = fused[:, :, :hq], fused[:, :, hq:]
+    for heads in (1, 3):   # (an expanded dimension has to be laid out before a tensor map takes it)
+        kk = k.expand(b, s, heads, d)
+        qq = q[:, :, :heads]
+        lse = torch.empty(b, heads, s)
+        for i in range(b):
+            for h in range(heads):
+                x = (qq[i, :, h].double() @ k[i, :, 0].double().T) * d ** -0.5
+                lse[i, h] = x.masked_fill(torch.ones(s, s).triu(1).bool(), -math.inf).logsumexp(1).float()
+        got = _ops().attn_weight_sums(qq.cuda(), kk.cuda(), lse.cuda(), None).cpu().double()
+        for i in range(b):
+            want, most, _ = R.weight_sums(qq[i].double(), kk[i].double(), lse[i], None, 0, None, [s])
+            rel = (d + 8) * 2.0 ** -24 * most + 2.0 ** -24 * (most + lse.abs().max().item()) + 2.0 ** -20 + 128 * 2.0 ** -24 + 2.0 ** -23
+            assert ((got[i] - want).abs() <= rel * want).all()
+
+
+def test_sums_of_a_prompt_are_what_its_attention_over_a_cache_adds_up():
+    """Every query of a short prompt through cache_attn(weights=) and the prompt through attn_weight_sums, on the values that the
+    cache holds.  Tolerances of both sides: 2 e + 2^-18 + rows * 2^-24 and e + 2^-20 + 2^-16 (test_gpu_cache.py), the log-sum-exp's
+    e + 2^-20 (1 + |lse|) besides."""
+    ops = _ops()
+    n, hq, hkv, d, bs, window, sink = 150, 8, 2, 128, 32, 60, 3
+    cache, table, _, _, _ = filled("int8", "bf16", [n], hkv, bs, d, seed=3)
+    lens = torch.tensor([n], dtype=torch.int32).cuda()
+    k, _ = ops.cache_read(cache, table.cuda(), lens, n)      # (int8 times a power of two: exact in bf16)
+    q = normal(1, n, hq, d, seed=4, dt="bf16")
+    w = torch.zeros(1, hkv, table.shape[1] * bs, device="cuda")
+    _, lse = ops.cache_attn(q.cuda(), cache, table.cuda(), lens, window_size=window, num_sink_tokens=sink, weights=w, return_lse=True)
+    got = ops.attn_weight_sums(q.cuda(), k, lse, window, sink)
+    _, want_lse, want, _, most = R.attn(host(cache), table, [n], q.double(), window, sink)
+    e = (d + 8) * 2.0 ** -24 * most
+    rel = 2 * e + 2.0 ** -18 + n * hq * 2.0 ** -24 + 2.0 ** -16 + 2.0 ** -20 * (1 + want_lse.abs().max().item())
+    for x in (got.cpu().double(), w[..., :n].cpu().double()):
+        assert ((x - want).abs() <= rel * want).all()
