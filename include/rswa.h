@@ -287,7 +287,7 @@ float rswa_event_elapsed_ms(void* start, void* stop);
  * RSWA_CACHE_E4M3: 4 exponent and 3 mantissa bits (no infinities, up to 448).  rswa_cache_append and
  * rswa_cache_evict write scales that are powers of two, 2^-100 or more; the others take any positive ones (rswa_cache_attn:
  * a scale of V below 2^-100 counts as that; above 2^80 its log-sum-exp and weights lose digits).
- * block_size: 16, 32, 64 or 128 tokens; head_dim: 64 or 128; every base 16-byte aligned.
+ * block_size: 16, 32, 64 or 128 tokens; head_dim: 64 or 128; k and v 16-byte aligned.
  *
  * Sequence b's tokens lie, in order, in the blocks named by row b of a block table (int32, device memory; rows
  * table_stride entries apart, max_blocks of them each); its slot t is token t % block_size of the row's entry

@@ -281,9 +281,9 @@ int check_cache(const rswa_cache_t& c, const char* what) {
     set_error("%s: at most 32767 key/value heads", what);
     return RSWA_E_UNSUPPORTED;
   }
-  if (c.k == nullptr || c.v == nullptr || c.k_scale == nullptr || c.v_scale == nullptr || off16(c.k) || off16(c.v) || off16(c.k_scale) ||
-      off16(c.v_scale)) {
-    set_error("%s: the cache's tensors must be there and 16-byte aligned", what);
+  if (c.k == nullptr || c.v == nullptr || c.k_scale == nullptr || c.v_scale == nullptr || off16(c.k) || off16(c.v) ||
+      ((reinterpret_cast<uintptr_t>(c.k_scale) | reinterpret_cast<uintptr_t>(c.v_scale)) & 3) != 0) {
+    set_error("%s: the cache's tensors must be there, keys and values 16-byte aligned", what);
     return RSWA_E_ARG;
   }
   return RSWA_OK;
@@ -307,6 +307,7 @@ int check_table(const rswa_block_table_t& t, bool written, const int32_t* lens, 
     set_error("%s: rows of a block table of blocks to write to overlap", what);
     return RSWA_E_ARG;
   }
+  // (the kernels may step up to 2^14 slots beyond a sequence's end before they compare)
   if (static_cast<long long>(t.max_blocks) * block_size > 0x7ff00000LL) {
     set_error("%s: positions overflow int32", what);
     return RSWA_E_UNSUPPORTED;

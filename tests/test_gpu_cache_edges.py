@@ -337,3 +337,23 @@ def test_sums_of_a_prompt_are_what_its_attention_over_a_cache_adds_up():
     rel = 2 * e + 2.0 ** -18 + n * hq * 2.0 ** -24 + 2.0 ** -16 + 2.0 ** -20 * (1 + want_lse.abs().max().item())
     for x in (got.cpu().double(), w[..., :n].cpu().double()):
         assert ((x - want).abs() <= rel * want).all()
+
+
+def test_scales_of_a_layer_among_others():
+    """k_scale and v_scale as slices of one tensor for all layers: aligned to 4 bytes, no more."""
+    ops = _ops()
+    lens, bs, d = [70, 21], 16, 64
+    cache, table, k, v, cu = filled("e4m3", "bf16", lens, 1, bs, d, seed=3, spare=6)
+    blocks = cache.k.shape[0]
+    both = torch.full((3, 2, blocks, 1), math.nan, device="cuda").flatten()[1:1 + 4 * blocks].view(2, 2, blocks, 1)
+    layer = ops.KVCache(cache.k.clone(), cache.v.clone(), both[1, 0], both[1, 1])
+    assert (layer.k_scale.data_ptr() | layer.v_scale.data_ptr()) % 16 != 0
+    n, t = torch.tensor(lens, dtype=torch.int32).cuda(), table.cuda()
+    ops.cache_append(layer, k.cuda(), v.cuda(), t, n * 0, cu_seqlens=cu.cuda())
+    q = normal(2, 1, 4, d, seed=4, dt="bf16").cuda()
+    assert torch.equal(ops.cache_attn(q, layer, t, n), ops.cache_attn(q, cache, t, n))
+    free = sorted(set(range(blocks)) - set(table.flatten().tolist()))
+    new, w = torch.tensor(free[:4], dtype=torch.int32).view(2, 2).cuda(), torch.rand(2, 1, table.shape[1] * bs, device="cuda")
+    a, b = (ops.cache_evict(c, t, n, w, 20, new) for c in (cache, layer))
+    for x, y in zip([*a, *ops.cache_read(cache, new, a[0], 20)], [*b, *ops.cache_read(layer, new, b[0], 20)]):
+        assert torch.equal(x, y)
