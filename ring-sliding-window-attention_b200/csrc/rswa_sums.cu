@@ -12,7 +12,9 @@
 // 2 * head_dim FLOPs and one exponential per (query head, pair): at 128 elements the exponentials (16 per clock and SM,
 // 2048 cycles a step) outweigh the products (1024).  One pair in eight is computed on the FMA pipe (fma_exp2): none
 // 624 us, 1/8 621, 1/4 631 (16384 tokens, 32/8 heads, window 4096): the card is at its power cap there when call follows
-// call (548 us on a cool one), and an exponential on the FMA pipe costs more than it saves beyond that.
+// call (548 us on a cool one), and an exponential on the FMA pipe costs more than it saves beyond that.  Besides, 6 us go for the
+// look at each step's sum: a NaN may come from a query that has to be left out, and is added up again pair by pair (with the
+// queries left out in the ordinary code 15 us).
 //
 // Work: the steps of all (batch row, key/value head, 256 keys) in one order, cut into equal shares, one per CTA and round,
 // whatever the mask makes of an item's length (a sink token is seen by its whole sequence): nothing is longer than the rest.

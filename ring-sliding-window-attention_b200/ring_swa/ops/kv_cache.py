@@ -133,7 +133,9 @@ def cache_attn(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, lens:
 
     weights: float32 [batch, num_kv_heads, at least max_blocks * block_size], added to in place: the softmax weights that
     every slot got from the queries and heads of its key/value head (what cache_evict goes by; start it with
-    attn_weight_sums of the prompt, or zeros).
+    attn_weight_sums of the prompt, or zeros).  Such a call holds, while it runs, 32 bytes per slot of block_table (of the window
+    and the sinks where there is a window), sequence, head and 8 queries and heads of a key/value head: a table much wider than
+    the sequences costs memory.
 
     NaN reaches the rows that see it and no others: from a query or a block of keys the output, the log-sum-exp and the weights of
     the slots which the row sees, from a block of values the output alone.
